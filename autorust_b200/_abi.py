@@ -25,6 +25,8 @@ AR_ERR_CUDA = -6
 AR_ERR_DEVICE_WAIT = -7
 AR_ERR_NO_DEVICE = -8
 AR_ERR_TOO_LARGE = -9
+AR_ERR_PAGE = -10
+KV_INT8, KV_E4M3 = 0, 1
 SAGE_STATIC_SCRATCH_BYTES = 32 << 20
 
 # Every symbol include/ar_attn.h declares; tests check that the library exports each one.
@@ -50,12 +52,29 @@ SYMBOLS = (
     "ar_sage_attention_prequantized_fp8",
     "ar_sage_forward_static",
     "ar_add_layernorm",
+    "ar_kv_cache_append",
+    "ar_kv_cache_read",
+    "ar_kv_cache_attention_workspace_bytes",
+    "ar_kv_cache_attention",
     "ar_attn_last_status",
     "ar_attn_plan",
     "ar_attn_selections",
     "ar_attn_launch_count",
     "ar_attn_strerror",
 )
+
+
+class KvPool(ctypes.Structure):
+    """ar_kv_pool"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("k_mean", ctypes.c_void_p), ("pages", ctypes.c_int64), ("Hkv", ctypes.c_int64), ("D", ctypes.c_int64),
+                ("page", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    """ar_kv_batch"""
+    _fields_ = [("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("table_pages", ctypes.c_int64), ("B", ctypes.c_int64), ("T", ctypes.c_int64)]
 
 
 class AttnLibraryError(RuntimeError):
@@ -120,6 +139,15 @@ def load() -> ctypes.CDLL:
     L.ar_sage_attention_prequantized_fp8.restype = ci
     L.ar_sage_forward_static.argtypes = [ci, p, p, p, p, p, i64, i64, i64, i64, i64, ci, p]
     L.ar_sage_forward_static.restype = ci
+    pool, batch = ctypes.POINTER(KvPool), ctypes.POINTER(KvBatch)
+    L.ar_kv_cache_append.argtypes = [pool, batch, ci, p, p, p, p, p]
+    L.ar_kv_cache_append.restype = ci
+    L.ar_kv_cache_read.argtypes = L.ar_kv_cache_append.argtypes
+    L.ar_kv_cache_read.restype = ci
+    L.ar_kv_cache_attention_workspace_bytes.argtypes = [pool, batch, ci, i64, i64, ci]
+    L.ar_kv_cache_attention_workspace_bytes.restype = sz
+    L.ar_kv_cache_attention.argtypes = [pool, batch, ci, p, p, p, p, i64, i64, ci, p, sz, p]
+    L.ar_kv_cache_attention.restype = ci
     L.ar_attn_last_status.argtypes = [p, p]
     L.ar_attn_last_status.restype = ci
     L.ar_attn_plan.argtypes = [ci, i64, i64, i64, i64, i64, ci, ctypes.POINTER(ctypes.c_int32)]

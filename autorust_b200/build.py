@@ -36,7 +36,7 @@ NVCC_FLAGS = [
 ]
 
 KERNEL_SOURCES = ["attn_fwd_tc.cu", "attn_fwd_short.cu", "attn_fwd_exact.cu", "attn_train.cu", "attn_train_tc.cu", "sage_prologue.cu", "api.cu",
-                  "sage_static.cu", "encoder_norm.cu"]
+                  "sage_static.cu", "encoder_norm.cu", "kv_cache.cu", "kv_cache_write.cu", "kv_cache_attn.cu"]
 
 
 def _nvcc() -> str:

@@ -20,8 +20,9 @@ std::atomic<uint64_t> g_launches;
 // launch cannot erase what an earlier one reported.
 __device__ __align__(256) uint32_t g_status_word[64];
 
-// 1 when the current device is compute capability 10.x.
-bool device_ok() {
+}  // namespace
+
+bool ar::device_ok() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
@@ -36,6 +37,9 @@ bool device_ok() {
   if (dev < 64) cache[dev] = ok ? 1 : 2;
   return ok;
 }
+
+namespace {
+using ar::device_ok;
 
 // Dense [B, H, S, D] tensor: rank-4 map with boxes of 128 rows x 128 bytes (ar::make_tile_map).
 bool make_map(CUtensorMap* m, const void* ptr, CUtensorMapDataType dt, int esize, int64_t B, int64_t H, int64_t S,
@@ -150,7 +154,6 @@ SageLayout sage_layout(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t S,
   return L;
 }
 
-// Lets other translation units of the library feed the launch counters.
 void count_launches(int mode, int kernels) {
   g_launches += (uint64_t)kernels;
   if (mode >= 0 && mode < 6) g_selected[mode]++;
@@ -698,6 +701,7 @@ int ar_attn_last_status(void* workspace, void* cu_stream) {
   if (cudaMemcpy(&host, status, sizeof(host), cudaMemcpyDeviceToHost) != cudaSuccess) return AR_ERR_CUDA;
   // (word 0 as well: the ticket that an expired launch left there must not meet a later launch with the same number)
   if (host != 0 && !workspace && cudaMemset(library_words(), 0, 2 * sizeof(uint32_t)) != cudaSuccess) return AR_ERR_CUDA;
+  if (!workspace && host == ar::STATUS_PAGE) return AR_ERR_PAGE;
   return host == 0 ? AR_OK : AR_ERR_DEVICE_WAIT;
 }
 
@@ -751,6 +755,7 @@ const char* ar_attn_strerror(int status) {
     case AR_ERR_CUDA: return "CUDA call failed";
     case AR_ERR_DEVICE_WAIT: return "a bounded device-side wait expired";
     case AR_ERR_NO_DEVICE: return "no sm_100 device is current";
+    case AR_ERR_PAGE: return "a page number or length outside the cache";
     case AR_ERR_TOO_LARGE: return "problem exceeds the library's built-in scratch (ar_sage_forward_static)";
     default: return "unknown status";
   }

@@ -77,6 +77,10 @@ bool attn_tc_has(int mode, int D);
 // The library's own status block on the current device (api.cu): word 0 is the launch status of calls that bring
 // no workspace, word 1 accumulates every expiry of a bounded wait until the host reads and clears it.
 // False when the address cannot be resolved.
+// 1 when the current device is compute capability 10.x.
+bool device_ok();
+// Lets other translation units of the library feed the launch counters.
+void count_launches(int mode, int kernels);
 bool library_status_words(uint32_t** launch_word, uint32_t** sticky_word);
 
 // Layout of the Sage workspace (offsets in bytes from its start; every section 256-byte aligned, the first 256 bytes
@@ -144,6 +148,43 @@ struct TrainTcPlan {
 TrainTcPlan train_tc_plan(int B, int Hq, int Hkv, int S, int D, int causal);
 // Launches dQ and dK/dV; *launches is incremented by the number of kernels.
 cudaError_t launch_attn_train_backward_tc(const TrainBwdTcArgs& a, cudaStream_t stream, int* launches);
+
+// The 8-bit key/value cache (kv_cache.cu: checks and dispatch; kv_cache_write.cu, kv_cache_attn.cu: kernels).
+constexpr uint32_t STATUS_PAGE = 0x40000000u;  // accumulator bit: a page or a length outside the cache
+struct KvPool {
+  uint8_t *k, *v;            // codes [pages, Hkv, 1 << page_log2, D]
+  float *k_scale, *v_scale;  // [pages, Hkv]
+  const float* k_mean;       // [Hkv, D] or null
+  int pages, Hkv, D, page_log2, e4m3;
+};
+struct KvBatch {
+  const int *page_table, *lengths, *starts;  // starts null: one row per sequence
+  long long table_stride;
+  int table_pages, B, T;
+  uint32_t* sticky;
+};
+struct KvRows {  // a packed [T, H, D] tensor: element strides of token and head
+  void* p;
+  long long st, sh;
+};
+cudaError_t launch_kv_append(const KvPool& pool, const KvBatch& batch, int dtype, const KvRows& k, const KvRows& v,
+                             cudaStream_t stream);
+cudaError_t launch_kv_read(const KvPool& pool, const KvBatch& batch, int dtype, const KvRows& k, const KvRows& v,
+                           cudaStream_t stream);
+struct KvAttnArgs {
+  KvPool pool;
+  KvBatch batch;
+  KvRows q, o;
+  int dtype, Hq, max_length, causal;
+  float* partial;  // workspace; null where the plan needs none
+};
+// How a call divides its tokens: chunks of `chunk` keys, at most `chunks` of them per row.
+struct KvAttnPlan {
+  int chunk, chunks;
+  size_t workspace;
+};
+KvAttnPlan kv_attn_plan(const KvPool& pool, int B, int T, int dtype, int Hq, int max_length, int causal);
+cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches);
 
 // Sage prologue (sage_prologue.cu).
 struct PrologueArgs {

@@ -1,0 +1,79 @@
+// Device helpers that the kernels of the 8-bit key/value cache share: which sequence and tile a CTA works on, and what the codes
+// stand for.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "ar_kernels.h"
+
+namespace ar {
+
+// starts[b] held inside [0, T]: the arrays lie in device memory, the host has not seen them.
+__device__ __forceinline__ int kv_start(const KvBatch& s, int b) {
+  return s.starts ? min(max(s.starts[b], 0), s.T) : b;
+}
+
+// A CTA's place in a grid over the tiles of all sequences, whose sizes only the device knows.  A sequence with n rows has
+// at most floor(n * rows_per / tile) + slack tiles; so that the first tile of sequence b may stand at
+// base(b) = floor(start(b) * rows_per / tile) + slack * b, and floor(T * rows_per / tile) + slack * B places hold them
+// all.  The sequence of a place is the last one with base(b) <= place, looked for by a whole warp, 32 candidates at a
+// time; a place past its sequence's tiles stays empty.
+struct KvPlace {
+  int b, tile;     // sequence, tile within it
+  int row0, n;     // its rows of the packed tensors
+  int length;      // tokens of the sequence, the call's counted in (a negative one counts as 0)
+};
+__device__ __forceinline__ long long kv_base(const KvBatch& s, int b, int rows_per, int tile_log2, int slack) {
+  return (((long long)kv_start(s, b) * rows_per) >> tile_log2) + (long long)slack * b;
+}
+__device__ __forceinline__ KvPlace kv_place(const KvBatch& s, int place, int rows_per, int tile_log2, int slack) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = s.B;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int b = lo + lane * step;
+    const bool le = b < hi && kv_base(s, b, rows_per, tile_log2, slack) <= place;
+    const int seen = max(__popc(__ballot_sync(0xffffffffu, le)), 1);
+    lo += (seen - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  KvPlace p;
+  p.b = lo;
+  p.row0 = kv_start(s, lo);
+  p.n = s.starts ? max(kv_start(s, lo + 1) - p.row0, 0) : 1;
+  p.tile = (int)(place - kv_base(s, lo, rows_per, tile_log2, slack));  // (may be negative in front of starts[0])
+  p.length = max(s.lengths[lo], 0);
+  return p;
+}
+// Places of such a grid.
+inline long long kv_places(long long B, long long T, long long rows_per, int tile_log2, int slack) {
+  return ((T * rows_per) >> tile_log2) + slack * B;
+}
+
+__device__ __forceinline__ void kv_report(const KvBatch& s) {
+  if (s.sticky) atomicOr(s.sticky, STATUS_PAGE);
+}
+// The page that holds block `blk` of sequence b's tokens, or -1 (reported by the caller) where there is none.
+__device__ __forceinline__ int kv_page(const KvPool& pool, const KvBatch& s, int b, int blk) {
+  if (blk < 0 || blk >= s.table_pages) return -1;
+  const int page = s.page_table[(long long)b * s.table_stride + blk];
+  return page >= 0 && page < pool.pages ? page : -1;
+}
+
+// ---- codes ----
+// An E4M3 pattern moved into an f16 (sign, and the 7 other bits one place to the right) is its value times 2^-8, subnormals
+// included: the exponent biases are 7 and 15.
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  const uint32_t h = ((code & 0x80u) << 8) | ((code & 0x7fu) << 7);
+  return __half2float(__ushort_as_half((unsigned short)h)) * 256.0f;
+}
+__device__ __forceinline__ float kv_value(uint32_t code, int e4m3) {
+  return e4m3 ? e4m3_value(code) : (float)(int)(int8_t)code;
+}
+// Two values -> two E4M3 codes, round to nearest even (the caller keeps them inside +-448).
+__device__ __forceinline__ uint32_t e4m3_codes(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+}  // namespace ar

@@ -5,6 +5,7 @@ libar_attn.so and raises when the library or a B200 is missing.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
@@ -362,6 +363,149 @@ def add_layernorm(x: torch.Tensor, residual: torch.Tensor | None, gamma: torch.T
                                 float(eps), _abi.DTYPE_BF16, st.cuda_stream)
     _abi.check(rc, "ar_add_layernorm")
     return (s_out if s_out is not None else x), y
+
+
+@dataclass
+class KvCache:
+    """The pool of an 8-bit key/value cache (ar_kv_pool): k, v [pages, Hkv, page, D] codes -- int8, or uint8 tensors of E4M3
+    bit patterns -- and k_scale, v_scale [pages, Hkv] float32, one scale for each page of tokens and kv head.  k_mean
+    [Hkv, D] float32: an offset that is taken off the keys before they are quantised (None: none).  kv_cache makes one;
+    the tensors are the caller's and may be saved, copied and sliced by page."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_mean: torch.Tensor | None = None
+
+    def __post_init__(self):
+        k = self.k
+        if k.dim() != 4 or k.dtype not in (torch.int8, torch.uint8) or not k.is_contiguous():
+            raise ValueError("k must be a contiguous [pages, Hkv, page, D] tensor of int8 or uint8 (E4M3) codes")
+        if not k.is_cuda:
+            raise ValueError("the cache must be CUDA tensors: there is no CPU path")
+        _check_dense("v", self.v, k.shape, k.dtype, k.device)
+        _check_dense("k_scale", self.k_scale, k.shape[:2], torch.float32, k.device)
+        _check_dense("v_scale", self.v_scale, k.shape[:2], torch.float32, k.device)
+        if self.k_mean is not None:
+            _check_dense("k_mean", self.k_mean, (k.shape[1], k.shape[3]), torch.float32, k.device)
+
+    @property
+    def fp8(self) -> bool:
+        return self.k.dtype == torch.uint8
+
+    def _pool(self) -> _abi.KvPool:
+        pages, Hkv, page, D = self.k.shape
+        return _abi.KvPool(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                           None if self.k_mean is None else self.k_mean.data_ptr(), pages, Hkv, D, page,
+                           _abi.KV_E4M3 if self.fp8 else _abi.KV_INT8)
+
+
+def kv_cache(pages: int, kv_heads: int, page: int, D: int, fp8: bool = False, k_mean: torch.Tensor | None = None,
+             device="cuda") -> KvCache:
+    """An empty pool of `pages` pages of `page` tokens (16, 32, 64 or 128), D = 64 or 128."""
+    code = torch.uint8 if fp8 else torch.int8
+    k, v = (torch.zeros((pages, kv_heads, page, D), dtype=code, device=device) for _ in range(2))
+    ks, vs = (torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
+    return KvCache(k, v, ks, vs, k_mean)
+
+
+def _kv_batch(cache: KvCache, page_table, lengths, starts, tokens: int) -> _abi.KvBatch:
+    dev = cache.k.device
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev or page_table.stride(1) != 1:
+        raise ValueError("page_table must be a [B, pages] int32 tensor on the cache's device with contiguous rows")
+    B = page_table.shape[0]
+    _check_dense("lengths", lengths, (B,), torch.int32, dev)
+    if starts is not None:
+        _check_dense("starts", starts, (B + 1,), torch.int32, dev)
+    elif tokens != B:
+        raise ValueError(f"without starts every sequence has one token: {tokens} tokens for {B} sequences")
+    return _abi.KvBatch(page_table.data_ptr(), lengths.data_ptr(), None if starts is None else starts.data_ptr(),
+                        page_table.stride(0), page_table.shape[1], B, tokens)
+
+
+def _kv_rows(name: str, t: torch.Tensor, shape, dtype, device):
+    """Strides of a packed [T, H, D] view."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or t.stride(2) != 1:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device} with a contiguous last dimension")
+    return (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+
+
+def kv_cache_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    starts: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> None:
+    """Quantises the call's new tokens into the cache (ar_kv_cache_append).  k, v [T, Hkv, D], float32 or bfloat16 views with
+    a contiguous last dimension; sequence b's tokens are the rows starts[b] .. starts[b + 1] (None: one each) and become
+    its last ones -- lengths counts them in.  Token t lies on page page_table[b, t // page]."""
+    L = _abi.load()
+    if k.dim() != 3:
+        raise ValueError("k and v must be [T, Hkv, D]")
+    shape, dtype = (k.shape[0], cache.k.shape[1], cache.k.shape[3]), _dtype_code(k)
+    ks = _kv_rows("k", k, shape, k.dtype, cache.k.device)
+    vs = _kv_rows("v", v, shape, k.dtype, cache.k.device)
+    batch, pool = _kv_batch(cache, page_table, lengths, starts, k.shape[0]), cache._pool()
+    with torch.cuda.device(cache.k.device):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        rc = L.ar_kv_cache_append(pool, batch, dtype, k.data_ptr(), ks, v.data_ptr(), vs, s.cuda_stream)
+    _abi.check(rc, "ar_kv_cache_append")
+
+
+def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None, tokens: int,
+                  dtype: torch.dtype = torch.bfloat16, out=None, stream: torch.cuda.Stream | None = None):
+    """The last starts[b + 1] - starts[b] tokens of every sequence as the values the codes stand for (ar_kv_cache_read):
+    (k, v) [tokens, Hkv, D] of `dtype`.  With starts = running sums of lengths that is everything.  out: (k, v) to write into,
+    views with a contiguous last dimension; rows that belong to no sequence are left as they were."""
+    L = _abi.load()
+    shape, dev = (int(tokens), cache.k.shape[1], cache.k.shape[3]), cache.k.device
+    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    code = _dtype_code(k)
+    ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
+    batch, pool = _kv_batch(cache, page_table, lengths, starts, int(tokens)), cache._pool()
+    with torch.cuda.device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        rc = L.ar_kv_cache_read(pool, batch, code, k.data_ptr(), ks, v.data_ptr(), vs, s.cuda_stream)
+    _abi.check(rc, "ar_kv_cache_read")
+    return k, v
+
+
+def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                       starts: torch.Tensor | None = None, causal: bool = True, max_length: int | None = None,
+                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                       stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """o = softmax(q k^T / sqrt(D)) v over the cached tokens of each row's sequence (ar_kv_cache_attention).  q [T, Hq, D],
+    float32 or bfloat16, packed like the k of kv_cache_append: a sequence's rows are its last tokens, and with `causal`
+    each sees the keys up to itself.  max_length: a bound on lengths, for dividing the work (None: the page table's width).
+    `workspace` is a uint8 CUDA tensor of kv_cache_attention_workspace bytes; one is allocated when needed and none is given."""
+    L = _abi.load()
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    T, Hq, D = q.shape
+    dev, code = cache.k.device, _dtype_code(q)
+    qs = _kv_rows("q", q, (T, Hq, cache.k.shape[3]), q.dtype, dev)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    os = _kv_rows("out", out, (T, Hq, D), q.dtype, dev)
+    batch, pool = _kv_batch(cache, page_table, lengths, starts, T), cache._pool()
+    bound = page_table.shape[1] * cache.k.shape[2] if max_length is None else int(max_length)
+    need = int(L.ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, bound, int(causal)))
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    have = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    with torch.cuda.device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        rc = L.ar_kv_cache_attention(pool, batch, code, q.data_ptr(), qs, out.data_ptr(), os, Hq, bound, int(causal),
+                                     workspace.data_ptr() if have else None, have, s.cuda_stream)
+    _abi.check(rc, "ar_kv_cache_attention")
+    if workspace is not None:
+        workspace.record_stream(s)
+    return out
+
+
+def kv_cache_attention_workspace(cache: KvCache, tokens: int, Hq: int, sequences: int, max_length: int,
+                                 dtype: torch.dtype = torch.bfloat16, causal: bool = True) -> int:
+    """Bytes of scratch that kv_cache_attention needs for these sizes."""
+    # (the addresses are placeholders: the size depends on the extents only)
+    batch = _abi.KvBatch(16, 16, 16, max_length, max(1, -(-max_length // cache.k.shape[2])), sequences, tokens)
+    code = _abi.DTYPE_F32 if dtype == torch.float32 else _abi.DTYPE_BF16
+    return int(_abi.load().ar_kv_cache_attention_workspace_bytes(cache._pool(), batch, code, Hq, max_length, int(causal)))
 
 
 def last_status(workspace: torch.Tensor | None = None) -> int:

@@ -66,7 +66,9 @@ enum ar_attn_status {
   AR_ERR_CUDA = -6,        /* a CUDA runtime / driver call failed (launch, tensor map) */
   AR_ERR_DEVICE_WAIT = -7, /* a bounded wait inside a kernel ran out (see ar_attn_last_status) */
   AR_ERR_NO_DEVICE = -8,   /* no sm_100 device is current */
-  AR_ERR_TOO_LARGE = -9    /* problem exceeds the built-in scratch of ar_sage_forward_static */
+  AR_ERR_TOO_LARGE = -9,   /* problem exceeds the built-in scratch of ar_sage_forward_static */
+  AR_ERR_PAGE = -10        /* a cache call met a page number outside the pool, or a length outside the page table or
+                              above max_length (see ar_kv_cache_append) */
 };
 
 /* ABI version; bumped on any signature change.  (No counterpart in the reference.) */
@@ -263,13 +265,84 @@ int ar_sage_attention_prequantized_fp8(const uint8_t* q8, const uint8_t* k8, con
 int ar_sage_forward_static(int dtype, const void* q, const void* k, const void* v, void* o, const float* mask,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t S, int64_t D, int causal, void* cu_stream);
 
+/* ---- 8-bit key/value cache: keys and values that stay between calls, quantised as they are written, for attention of new
+ * tokens over everything before them (token generation, chunks of a prompt, verification of proposed tokens).  The
+ * reference has no cache (its attention takes whole sequences, src/models/flash_attention.rs:348-702); the granularity is
+ * ar_sage_quantize's, one scale for each block of tokens and kv head, here for keys and values.
+ *
+ * The pool is cut into pages of `page` tokens, and a page of one kv head is the block that shares a scale:
+ *   k, v              [pages, Hkv, page, D] codes, dense, 16-byte aligned: int8, or E4M3 bit patterns
+ *   k_scale, v_scale  [pages, Hkv] f32; a code stands for code * scale
+ *   k_mean            [Hkv, D] f32 or NULL: an offset per kv head and channel that is subtracted from the keys before they
+ *                     are quantised and added when they are read back (the smoothing of ar_sage_quantize with a mean
+ *                     that is fixed beforehand; attention does not depend on it: it moves all logits of a row alike)
+ * page is 16, 32, 64 or 128; D is 64 or 128. */
+enum ar_kv_format { AR_KV_INT8 = 0, AR_KV_E4M3 = 1 };
+typedef struct ar_kv_pool {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  const float* k_mean;
+  int64_t pages, Hkv, D;
+  int32_t page, format;
+} ar_kv_pool;
+
+/* The sequences of a call (device arrays, read by the kernels; nothing is copied to the host, so that a captured call sees
+ * what they hold when it is replayed).
+ *   page_table [B, table_stride] int32, of which the first table_pages entries of a row count: token t of sequence b lies in
+ *              row t % page of page page_table[b][t / page].  Entries past a sequence's length are not read.
+ *   lengths    [B] int32: the tokens of a sequence, those of this call counted in.
+ *   starts     [B + 1] int32, or NULL: rows starts[b] .. starts[b + 1] of the call's packed [T, H, D] tensors belong to
+ *              sequence b, in order and not overlapping; NULL: T = B, one row each.
+ * Row i of a sequence's n rows stands at position lengths[b] - n + i: the call's rows are the last tokens.  A row whose
+ * position is negative is padding (an idle slot of a fixed batch has length 0): it is not written, reads back as zeros and
+ * its attention is zero.  Rows in front of starts[0] and from starts[B] on are neither read nor written. */
+typedef struct ar_kv_batch {
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int64_t table_stride, table_pages, B, T;
+} ar_kv_batch;
+
+/* Writes the call's tokens into the pool.  k, v: [T, Hkv, D] of `dtype`, D contiguous, element strides {token, head}
+ * (slices of a fused projection need no copy); strides times the element size are multiples of 16 bytes.
+ * A page's scale is the smallest that covers what it has received: with a the largest |value| among the call's tokens for
+ * it, s1 = a / 127 (INT8), or the least power of two >= a / 448 (E4M3), at least 2^-60; s = s1 for a page that holds no
+ * earlier token of the sequence, else max(s0, s1).  New codes are rn(x * (1 / s)); when s > s0 the earlier codes become
+ * rn(code * (s0 / s)) -- exact for E4M3 but in its subnormal range, and for INT8 one more rounding whenever the scale
+ * grows.  A value that is not finite makes the scale of its page and head NaN: the page reads back as NaN.
+ * A page written by a call must belong to one sequence of that call (sequences may share full pages they only read).
+ * A page number outside [0, pages) or a position past table_pages * page is skipped on the device and reported by
+ * ar_attn_last_status(NULL, ..) as AR_ERR_PAGE; nothing outside the pool is touched. */
+int ar_kv_cache_append(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, void* cu_stream);
+
+/* The inverse: the values the codes stand for, rounded once to `dtype`, in rows of k_out and v_out [T, Hkv, D] (element
+ * strides {token, head}) -- with the arguments of an append what that call wrote, with starts = running sums of lengths
+ * whole sequences.  Positions on pages that do not exist come back as zeros and are reported as above. */
+int ar_kv_cache_read(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, void* k_out, const int64_t* k_strides,
+                     void* v_out, const int64_t* v_strides, void* cu_stream);
+
+/* o = softmax(q k^T / sqrt(D)) v over the cached tokens of each row's sequence: q, o [T, Hq, D] of `dtype` (element strides
+ * {token, head}), query head h reads kv head h / (Hq / Hkv); with `causal` a row sees the keys up to its own position, else all of its
+ * sequence's.  A row that sees no key is zero.  Keys on pages that do not exist are left out and reported as above.
+ * max_length: a bound on lengths[b] (table_pages * page always is one); it sets how the tokens are divided over the GPU
+ * and the workspace, and tokens from max_length on are left out and reported.
+ * workspace: ar_kv_cache_attention_workspace_bytes(), 16-byte aligned, may be NULL when that is 0; its contents need not
+ * survive or be cleared between calls, calls that overlap in time need one each.  One fixed order of summation: a
+ * call's results depend on its sizes, not on timing. */
+size_t ar_kv_cache_attention_workspace_bytes(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, int64_t Hq,
+                                             int64_t max_length, int causal);
+int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* q,
+                          const int64_t* q_strides, void* o, const int64_t* o_strides, int64_t Hq, int64_t max_length,
+                          int causal, void* workspace, size_t workspace_bytes, void* cu_stream);
+
 /* Synchronises `cu_stream` and reads a device status word: AR_OK, or AR_ERR_DEVICE_WAIT when a bounded wait
  * expired inside a kernel (the launch then returned without finishing its tile; later CTAs of that launch leave at
  * once).  Stands where the reference has only `cuStreamSynchronize`'s error (src/runtime/ops_cuda.rs:1013-1016).
  * workspace != NULL (a workspace, or the word given as `status_word`): the status of the LAST launch that used it --
  * every launch clears its word first.  workspace == NULL: the library's accumulator on the current device, into
  * which every expiry of every launch is OR-ed as well; reading it clears it, so one call after a batch of launches
- * covers all of them. */
+ * covers all of them.  The accumulator also collects what the cache calls report: AR_ERR_PAGE when nothing else was. */
 int ar_attn_last_status(void* workspace, void* cu_stream);
 
 /* Number of launches per kernel family since the library was loaded: the
