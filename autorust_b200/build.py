@@ -100,7 +100,8 @@ def build_wait_test(force: bool = False) -> Path:
     for s in srcs:
         if s.name in WAIT_SOURCES:
             o = out_dir / (s.stem + ".o")
-            _run([_nvcc(), *NVCC_FLAGS, *WAIT_TEST_FLAGS, "-c", str(s), "-o", str(o)])
+            if force or _newer(o, [s] + _headers()):
+                _run([_nvcc(), *NVCC_FLAGS, *WAIT_TEST_FLAGS, "-c", str(s), "-o", str(o)])
         else:
             o = LIB / (s.stem + ".o")
         objs.append(str(o))

@@ -178,9 +178,9 @@ struct KvAttnArgs {
   int dtype, Hq, max_length, causal;
   float* partial;  // workspace; null where the plan needs none
 };
-// How a call divides its tokens: chunks of `chunk` keys, at most `chunks` of them per row.
+// How a call is divided: row tiles of `rows` rows, over `ctas` CTAs that take equal shares of all keys (0: one CTA per tile).
 struct KvAttnPlan {
-  int chunk, chunks;
+  int rows, ctas;
   size_t workspace;
 };
 KvAttnPlan kv_attn_plan(const KvPool& pool, int B, int T, int dtype, int Hq, int max_length, int causal);
