@@ -59,6 +59,23 @@ __device__ __forceinline__ int kv_page(const KvPool& pool, const KvBatch& s, int
   return page >= 0 && page < pool.pages ? page : -1;
 }
 
+// Programmatic dependent launch: a kernel's launch, and its way to griddepcontrol.wait, which comes before its first access to
+// memory, lie under the last CTAs of the kernel before it.
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 // ---- codes ----
 // An E4M3 pattern moved into an f16 (sign, and the 7 other bits one place to the right) is its value times 2^-8, subnormals
 // included: the exponent biases are 7 and 15.

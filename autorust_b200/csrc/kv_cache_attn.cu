@@ -5,9 +5,8 @@
 // Scales are constants of a page, so the products run on the codes themselves.
 //   QK   INT8: integer MMAs on the codes as they lie in memory, no conversion; q in fixed point, multiples of 2^-21 of
 //        the binade of its row's largest element (a bf16 q exactly, but for elements 2^-14 below it), as three signed 8-bit
-//        digits: the sums are exact.  E4M3: codes converted to f16,
-//        which holds them exactly; q scaled by a power of two per row to f16 (bf16 exactly, but for elements 2^-14 below the row's
-//        largest), f32 tensors as two f16 terms.
+//        digits: the sums are exact.  E4M3: codes converted to f16, which holds them exactly; q scaled by a power of two per
+//        row to f16 (bf16 with the same exception), f32 tensors as two f16 terms.
 //   PV   codes as f16 (exact: 8 and 4 significant bits of 11), P in f16, rounded to nearest; f32 tensors as two f16 terms.
 // Accumulators, maxima and sums are 32 bits.
 //
@@ -16,8 +15,10 @@
 // that accumulators are rescaled rarely) and e_ref is the exponent of the piece's first page; P = u * f < 2^15, and the row
 // sum takes u * 2^(e_ref - e).  O is then in units of 2^(m - 12 + e_ref), the sum l in units of 2^(m - 12).
 //
-// The products are transposed, S^T = K Q^T and O^T = V^T P^T, so that the rows of Q are the narrow side of the MMA (8 columns per
-// tile): the query heads of one kv head's group next to one another, then the next token.
+// Rows go in tiles of 8: the query heads of one kv head's group next to one another, then the next token.  S = Q K^T has the
+// digits or terms of 8 rows on the 16-row side of the MMA (two digits of the same rows side by side: one thread gets both
+// sums), O^T = V^T P^T has the rows on its 8-column side; S leaves a thread with the very elements of P that the second product
+// wants from it.
 //
 // What bounds it: memory, 26 bytes of codes per clock and SM.  A 16-token block of D = 128 then has 157 clocks, in which the ALU pipe (64
 // lanes per clock) converts V -- 96 instructions for INT8 -- and the MMAs take 32 to 48.  So each warp works by itself:
@@ -28,6 +29,8 @@
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
 
+#include <type_traits>
+
 namespace ar {
 namespace {
 using namespace arptx;
@@ -36,7 +39,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int GROUP = 32;       // keys of a warp's step: two blocks of 16, the smallest page
 constexpr int WARPS = 4;
 constexpr int SMS = 148;
-constexpr int LEAST_UNITS = 4;  // groups of a share: one per warp
+constexpr int LEAST_UNITS = 8;   // of a share
+// A row tile counts as its groups and START_UNITS more: beginning a piece (page numbers, Q, the first codes, the join of the
+// warps at its end) takes a CTA about as long as that many groups.
+constexpr int START_UNITS = 6;
 constexpr float P_SHIFT = 12.0f, LAG = 2.0f;
 constexpr int E_LIMIT = 100;    // largest |e - e_ref|
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60, the least scale a page is given
@@ -47,10 +53,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
@@ -59,11 +65,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t w) {  // of an 8 x 8 matrix of 16-bit elements spread over the warp
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
-  return r;
-}
 // The two codes of the low (HI = 0) or high half of w -> f16x2.  INT8 (w with the sign bits flipped, so the bytes are code +
 // 128): the byte under the exponent of 1024 is 1152 + code.
 template <bool E4M3, int HI>
@@ -129,19 +130,41 @@ __device__ __forceinline__ Seen kv_seen(const KvAttnArgs& a, int length, int n) 
   return s;
 }
 
+// Division by a number that the host knows (n < 2^31): by multiplication with its rounded-up reciprocal (Granlund and
+// Montgomery, "Division by invariant integers using multiplication").
+struct Divider {
+  uint32_t m;
+  int s1, s2;
+  __device__ __forceinline__ int operator()(int n) const {
+    const uint32_t t = __umulhi(m, (uint32_t)n);
+    return (int)((t + (((uint32_t)n - t) >> s1)) >> s2);
+  }
+};
+Divider divider(uint32_t d) {
+  int l = 0;
+  while ((1ull << l) < d) l++;
+  return Divider{(uint32_t)((((1ull << l) - d) << 32) / d + 1), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+}
+
 // A sequence as the division of the work sees it: `tiles` row tiles per kv head, `groups` groups of keys each (the last row's;
 // earlier rows of a causal call see fewer).
 struct Work {
   int row0, n, length, tiles, groups;
+  __device__ __forceinline__ uint32_t tile_units() const { return (uint32_t)groups + START_UNITS; }
+  __device__ __forceinline__ uint32_t units(int Hkv) const { return (uint32_t)tiles * tile_units() * Hkv; }
 };
+template <int ROWS>
+__device__ __forceinline__ void divide(const KvAttnArgs& a, int G, Work& w) {
+  w.tiles = (w.n * G + ROWS - 1) / ROWS;
+  w.groups = max(1, (kv_seen(a, w.length, w.n).total + GROUP - 1) / GROUP);
+}
 template <int ROWS>
 __device__ __forceinline__ Work work_of(const KvAttnArgs& a, int G, int b) {
   Work w;
   w.row0 = kv_start(a.batch, b);
   w.n = a.batch.starts ? max(kv_start(a.batch, b + 1) - w.row0, 0) : 1;
   w.length = max(a.batch.lengths[b], 0);
-  w.tiles = (int)(((long long)w.n * G + ROWS - 1) / ROWS);
-  w.groups = max(1, (kv_seen(a, w.length, w.n).total + GROUP - 1) / GROUP);
+  divide<ROWS>(a, G, w);
   return w;
 }
 
@@ -158,78 +181,81 @@ struct Cut {
 };
 
 template <int D, bool E4M3, bool F32, int NT>
-__global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_kernel(const KvAttnArgs a, int whole) {
+__global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_kernel(const KvAttnArgs a, const Divider by_g, int whole) {
   using S = Sh<D, NT>;
   constexpr int ROWS = S::ROWS;
-  constexpr int QREGS = E4M3 ? (F32 ? 2 : 1) * (D / 16) * 2 : 3 * (D / 32) * 2;
+  // Operands of the QK product, rows 0-7 | 8-15.  E4M3: one row tile, its f16 terms (high | low); two bf16 tiles, one beside the
+  // other; two f32 tiles, (high | low) each.  INT8: (digit 2 | digit 1) of each tile, then digit 0 of (tile 0 | tile 1).
+  constexpr int QOPS = E4M3 ? (NT == 2 && F32 ? 2 : 1) : NT + 1;
+  constexpr int QSTEPS = E4M3 ? D / 16 : D / 32;
   constexpr int MT = D / 16;  // 16-channel tiles of O^T
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long scan[WARPS];
-  __shared__ long long found[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * S::RING;
   float* ml = (float*)(smem + S::ML);
   float* scales = (float*)(smem + S::SCALES) + warp * S::STAGES * 4;
   const int G = a.Hq / a.pool.Hkv, Hkv = a.pool.Hkv;
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // whatever came before in the stream is done and visible
+  asm volatile("griddepcontrol.launch_dependents;");  // what comes next may take its places as CTAs leave; it waits for all of this
+
   // ---- this CTA's share: units [u, u_end) of the groups of all row tiles, or one whole row tile ----
+  // Every warp works it out for itself, without a barrier; 32-bit numbers, which the host has checked the sizes for.
   int b = 0;
-  long long u = 0, u_end = 0, base = 0;  // base: first unit of sequence b
-  int shares = 1;                        // CTAs that have one: share i is [all * i / shares, all * (i + 1) / shares)
+  uint32_t u = 0, u_end = 0, base = 0;     // base: first unit of sequence b
+  uint32_t per_share = 1, longer = 0;      // shares of per_share units, the first `longer` ones have one more
+  int shares = 1, kv_tile = 0;
   Work w;
   if (whole) {
     const KvPlace p = kv_place(a.batch, blockIdx.x, G, NT == 1 ? 3 : 4, 1);
     if (p.tile < 0 || (long long)p.tile * ROWS >= (long long)p.n * G) return;
     b = p.b;
-    w = work_of<ROWS>(a, G, b);
-    u = ((long long)blockIdx.y * w.tiles + p.tile) * w.groups;
-    u_end = u + w.groups;
+    kv_tile = p.tile;
+    w = Work{p.row0, p.n, p.length, 0, 0};
+    divide<ROWS>(a, G, w);
+    u = 0;
+    u_end = w.tile_units();
   } else {
-    const int per = (a.batch.B + WARPS * 32 - 1) / (WARPS * 32);
-    const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch.B);
-    long long mine = 0;
+    const int per = (a.batch.B + 31) / 32;
+    const int b0 = lane * per, b1 = min(b0 + per, a.batch.B);
+    uint32_t mine = 0;
+    Work x{0, 0, 0, 0, 0};
     for (int i = b0; i < b1; i++) {
-      const Work x = work_of<ROWS>(a, G, i);
-      mine += (long long)x.tiles * x.groups * Hkv;
+      x = work_of<ROWS>(a, G, i);
+      mine += x.units(Hkv);
     }
-    long long upto = mine;
+    uint32_t upto = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, s);
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, s);
       if (lane >= s) upto += v;
     }
-    if (lane == 31) scan[warp] = upto;
-    __syncthreads();
-    long long all = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; i++) {
-      if (i < warp) upto += scan[i];
-      all += scan[i];
-    }
-    shares = (int)max(1ll, min((long long)gridDim.x, all / LEAST_UNITS));
-    u = all * blockIdx.x / shares;
-    u_end = all * (blockIdx.x + 1) / shares;
-    if (blockIdx.x >= shares || all == 0) {
+    const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
+    shares = max(1, (int)min((uint32_t)gridDim.x, all / LEAST_UNITS));
+    per_share = all / shares;
+    longer = all - per_share * shares;
+    u = per_share * blockIdx.x + min(blockIdx.x, longer);
+    u_end = u + per_share + (blockIdx.x < longer ? 1u : 0u);
+    uint32_t at = upto - mine;
+    const uint32_t has = __ballot_sync(0xffffffffu, u >= at && u < upto);
+    if (blockIdx.x >= shares || has == 0) {
       if (threadIdx.x == 0) ((Cut*)a.partial)[blockIdx.x].last = -1;
       return;
     }
-    long long at = upto - mine;
-    if (u >= at && u < upto) {
-      for (int i = b0; i < b1; i++) {
-        const Work x = work_of<ROWS>(a, G, i);
-        const long long next = at + (long long)x.tiles * x.groups * Hkv;
-        if (u < next) {
-          found[0] = i;
-          found[1] = at;
-          break;
-        }
-        at = next;
+    const int src = __ffs(has) - 1;
+    if (per > 1 && lane == src) {  // which of this lane's sequences
+      for (b = b0; b < b1; b++) {
+        x = work_of<ROWS>(a, G, b);
+        if (u - at < x.units(Hkv)) break;
+        at += x.units(Hkv);
       }
     }
-    __syncthreads();
-    b = (int)found[0];
-    base = found[1];
-    w = work_of<ROWS>(a, G, b);
+    b = __shfl_sync(0xffffffffu, per > 1 ? b : b0, src);
+    base = __shfl_sync(0xffffffffu, at, src);
+    w.row0 = __shfl_sync(0xffffffffu, x.row0, src);
+    w.n = __shfl_sync(0xffffffffu, x.n, src);
+    w.length = __shfl_sync(0xffffffffu, x.length, src);
+    divide<ROWS>(a, G, w);
   }
   bool begun_cut = false;
 
@@ -240,16 +266,55 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
   const int lane_v1 = (lane >> 3 << 7) | (((lane & 7) ^ line_swizzle<D, true>((lane >> 3) + 4)) << 4);
 
   while (true) {  // a piece of one row tile
-    const int idx = (int)((u - base) / w.groups), g_begin = (int)(u - base - (long long)idx * w.groups);
-    const int g_end = (int)min((long long)w.groups, g_begin + (u_end - u));
-    const int h = idx / w.tiles, r0 = (idx - h * w.tiles) * ROWS, rn = min(ROWS, w.n * G - r0);
+    int h, tile;
+    uint32_t from = 0;  // units of the tile in front of this share
+    if (whole) {
+      h = blockIdx.y;
+      tile = kv_tile;
+    } else {
+      const uint32_t idx = (u - base) / w.tile_units();
+      from = u - base - idx * w.tile_units();
+      h = (int)(idx / (uint32_t)w.tiles);
+      tile = (int)(idx - h * w.tiles);
+    }
+    const uint32_t to = min(w.tile_units(), from + (u_end - u));
+    const int g_begin = max((int)from - START_UNITS, 0), g_end = (int)to - START_UNITS;
+    if (g_end <= 0) break;  // the share ends before the tile's first group: the next one begins the tile
+    const int r0 = tile * ROWS, rn = min(ROWS, w.n * G - r0);
     const Seen seen = kv_seen(a, w.length, w.n);
-    const int end = seen.limit((r0 + rn - 1) / G);    // keys that some row of the tile sees
-    const int lim_low = seen.limit(r0 / G);           // that all of them see
+    const int end = seen.limit(by_g(r0 + rn - 1));    // keys that some row of the tile sees
+    const int lim_low = seen.limit(by_g(r0));           // that all of them see
     if (seen.total < w.length && g_begin == 0 && threadIdx.x == 0) kv_report(a.batch);
     const int* table = a.batch.page_table + (long long)b * a.batch.table_stride;
     const int stop = min(g_end, (end + GROUP - 1) / GROUP);  // groups past the tile's last key are empty
     const int steps = (stop - g_begin - warp + WARPS - 1) / WARPS;  // (may be negative)
+
+    // ---- Q is asked for before the codes, which would keep it waiting: row g of each tile of 8; word j of a thread's channels
+    // starts at channel(j) ----
+    auto channel = [&](int j) { return (j >> 2) * 64 + c * 16 + (j & 3) * 4; };
+    float qv[NT][D / 16][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = r0 + nt * 8 + g;
+      const int token = by_g(r);
+      const long long at = (w.row0 + (long long)token) * a.q.st + (long long)(h * G + (r - token * G)) * a.q.sh;
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) {
+        float(&v)[4] = qv[nt][j];
+        if (nt * 8 + g >= rn) {
+          v[0] = v[1] = v[2] = v[3] = 0.f;
+        } else if constexpr (F32) {
+          const float4 x = *(const float4*)((const float*)a.q.p + at + channel(j));
+          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+          const uint2 x = *(const uint2*)((const __nv_bfloat16*)a.q.p + at + channel(j));
+          v[0] = __uint_as_float(x.x << 16);
+          v[1] = __uint_as_float(x.x & 0xffff0000u);
+          v[2] = __uint_as_float(x.y << 16);
+          v[3] = __uint_as_float(x.y & 0xffff0000u);
+        }
+      }
+    }
 
     // ---- the ring: page numbers are read one step ahead ----
     auto page_of = [&](int key) {
@@ -257,6 +322,13 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       const int pg = table[key >> log2];
       return pg >= 0 && pg < a.pool.pages ? pg : -1;
     };
+    // e_ref: the exponent of the piece's first V scale
+    auto exponent_of = [](float s) {  // a NaN keeps its NaN in the factor
+      const int e = (int)((__float_as_uint(s) >> 23) & 0xffu) - 127;
+      return e == 128 ? 0 : max(e, -60);
+    };
+    int e_ref = 0;
+    const int page0 = page_of(g_begin * GROUP);
     int next_page[2];
     auto look = [&](int it) {
       const int key0 = (g_begin + warp + it * WARPS) * GROUP;
@@ -302,57 +374,31 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       cp_async_commit();
     };
     look(0);
+    if (page0 >= 0) e_ref = exponent_of(a.pool.v_scale[(long long)page0 * Hkv + h]);
 #pragma unroll
     for (int it = 0; it < S::STAGES - 1; it++) {
       fetch(it);
       look(it + 1);
     }
 
-    // ---- Q: row g of each tile of 8; word j of a thread's channels starts at channel(j) ----
-    auto channel = [&](int j) { return (j >> 2) * 64 + c * 16 + (j & 3) * 4; };
-    uint32_t qr[NT][QREGS];
-    float row_c[NT][2];  // of rows 2c, 2c + 1: logit in the log2 domain = accumulator * row_c * s_k
-    int lim[NT][2];
+    uint32_t qa[QOPS][QSTEPS][4] = {};
+    float row_c[NT];  // of row g: logit in the log2 domain = accumulator * row_c * s_k
+    int lim[NT];      // keys that row g sees
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = r0 + nt * 8 + g;
-      const bool in = nt * 8 + g < rn;
-      const int token = r / G;
-      const long long at = (w.row0 + (long long)token) * a.q.st + (long long)(h * G + (r - token * G)) * a.q.sh;
-      float v[D / 16][4];
-      float top = 0.f;
+      float(&v)[D / 16][4] = qv[nt];
+      lim[nt] = nt * 8 + g < rn ? seen.limit(by_g(r0 + nt * 8 + g)) : 0;
+      uint32_t top = 0;  // bits of the largest |q|; infinities and NaN are the largest patterns
 #pragma unroll
-      for (int j = 0; j < D / 16; j++) {
-        if (!in) {
-          v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
-        } else if constexpr (F32) {
-          const float4 x = *(const float4*)((const float*)a.q.p + at + channel(j));
-          v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
-        } else {
-          const uint2 x = *(const uint2*)((const __nv_bfloat16*)a.q.p + at + channel(j));
-          v[j][0] = __uint_as_float(x.x << 16);
-          v[j][1] = __uint_as_float(x.x & 0xffff0000u);
-          v[j][2] = __uint_as_float(x.y << 16);
-          v[j][3] = __uint_as_float(x.y & 0xffff0000u);
-        }
+      for (int j = 0; j < D / 16; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(v[j][i]));
-      }
-      bool odd = false;  // NaN or infinity in the row: the integer digits cannot carry it
-      if constexpr (!E4M3) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 16; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) sum += v[j][i] * 0.f;
-        odd = sum != 0.f;  // (a NaN: 0 * inf, 0 * NaN)
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^-e brings the largest element below 2; both factors are normal f32 numbers
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);
+      const int e = min(max((int)(top >> 23) - 127, -100), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      float mine = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      row_c[nt] = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
       if constexpr (E4M3) {
 #pragma unroll
         for (int j = 0; j < D / 16; j++)
@@ -360,119 +406,90 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           for (int i = 0; i < 2; i++) {
             const float x0 = v[j][2 * i] * down, x1 = v[j][2 * i + 1] * down;
             const uint32_t x = pack_half2(x0, x1);
-            qr[nt][j * 2 + i] = x;
-            if constexpr (F32) qr[nt][(D / 16) * 2 + j * 2 + i] = pack_half2((x0 - half_lo(x)) * 2048.0f, (x1 - half_hi(x)) * 2048.0f);
+            if constexpr (F32) {
+              qa[nt][j][2 * i] = x;
+              qa[nt][j][2 * i + 1] = pack_half2((x0 - half_lo(x)) * 2048.0f, (x1 - half_hi(x)) * 2048.0f);
+            } else {
+              qa[0][j][2 * i + nt] = x;
+            }
           }
       } else {
-        mine *= 1.0f / 2097152.0f;
-        odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 28) & 15u) != 0;
-        if (odd) mine = __uint_as_float(0x7fc00000u);
+        const bool odd = top >= 0x7f800000u;  // the integer digits cannot carry it
+        row_c[nt] = odd ? __uint_as_float(0x7fc00000u) : row_c[nt] * (1.0f / 2097152.0f);
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
-          uint32_t d0 = 0, d1 = 0, d2 = 0;
+          int x0[4], x1[4], x2[4];  // |x0| <= 2^22 and its signed digits: the low bytes of x0, x1 and x2, |x2| <= 64
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const int x = odd ? 0 : __float2int_rn(v[j][i] * down * 2097152.0f);  // |x| <= 2^22
-            const int x1 = (x + 128) >> 8, x2 = (x1 + 128) >> 8;                  // |x2| <= 64
-            d0 |= (uint32_t)((x - (x1 << 8)) & 0xff) << (8 * i);
-            d1 |= (uint32_t)((x1 - (x2 << 8)) & 0xff) << (8 * i);
-            d2 |= (uint32_t)(x2 & 0xff) << (8 * i);
+            x0[i] = odd ? 0 : __float2int_rn(v[j][i] * down * 2097152.0f);
+            x1[i] = (x0[i] + 128) >> 8;
+            x2[i] = (x1[i] + 128) >> 8;
           }
-          qr[nt][j] = d0;
-          qr[nt][D / 16 + j] = d1;
-          qr[nt][D / 8 + j] = d2;
+          auto low_bytes = [](const int (&x)[4]) { return __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410); };
+          const uint32_t d0 = low_bytes(x0), d1 = low_bytes(x1), d2 = low_bytes(x2);
+          qa[nt][j >> 1][(j & 1) * 2] = d2;
+          qa[nt][j >> 1][(j & 1) * 2 + 1] = d1;
+          qa[NT][j >> 1][(j & 1) * 2 + nt] = d0;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        row_c[nt][i] = __shfl_sync(0xffffffffu, mine, (2 * c + i) * 4);
-        const int rr = nt * 8 + 2 * c + i;
-        lim[nt][i] = rr < rn ? seen.limit((r0 + rr) / G) : 0;
-      }
-    }
-
-    // e_ref: the exponent of the piece's first V scale
-    auto exponent_of = [](float s) {  // a NaN keeps its NaN in the factor
-      const int e = (int)((__float_as_uint(s) >> 23) & 0xffu) - 127;
-      return e == 128 ? 0 : max(e, -60);
-    };
-    int e_ref = 0;
-    if (stop > g_begin) {
-      const int pg = page_of(g_begin * GROUP);
-      if (pg >= 0) e_ref = exponent_of(a.pool.v_scale[(long long)pg * Hkv + h]);
     }
 
     float o[NT][MT][4];
-    float m[NT][2], l[NT][2];  // l: of this thread's keys only, until the end
+    float m[NT], l[NT];  // of row g; l: of this thread's keys only, until the end
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
       for (int i = 0; i < MT; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      m[nt] = -INFINITY;
+      l[nt] = 0.f;
     }
 
-    for (int it = 0; it < steps; it++) {
-      fetch(it + S::STAGES - 1);
-      look(it + S::STAGES);
-      cp_async_wait<S::STAGES - 1>();
-      __syncwarp();
+    // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out.
+    auto step = [&](auto edge_c, int it) {
+      constexpr bool EDGE = decltype(edge_c)::value;
       const uint8_t* kt = ring + (it % S::STAGES) * 2 * S::TILE;
       const uint8_t* vt = kt + S::TILE;
       const float4 sc = *(const float4*)(scales + (it % S::STAGES) * 4);
       const int key0 = (g_begin + warp + it * WARPS) * GROUP;
 
-      // S^T = K Q^T: blocks of 16 keys, thread (g, c) has keys g, g + 8 and rows 2c, 2c + 1
-      float s[NT][2][4];
+      // S = Q K^T: tiles of 8 keys, thread (g, c) has row g and keys 2c, 2c + 1
+      float s[NT][4][2];
 #pragma unroll
-      for (int blk = 0; blk < 2; blk++) {
-        uint32_t ka[2][D / 16];  // 4 codes each of keys g and g + 8
+      for (int n8 = 0; n8 < 4; n8++) {
+        uint32_t kw[D / 16];  // 4 codes each of key g
 #pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int i = 0; i < D / 64; i++) {
-            const uint4 v = *(const uint4*)(kt + piece_at<D, false>(blk * 16 + x * 8 + g, c + i * 4));
-            ka[x][i * 4] = v.x; ka[x][i * 4 + 1] = v.y; ka[x][i * 4 + 2] = v.z; ka[x][i * 4 + 3] = v.w;
-          }
+        for (int i = 0; i < D / 64; i++) {
+          const uint4 v = *(const uint4*)(kt + piece_at<D, false>(n8 * 8 + g, c + i * 4));
+          kw[i * 4] = v.x; kw[i * 4 + 1] = v.y; kw[i * 4 + 2] = v.z; kw[i * 4 + 3] = v.w;
+        }
         if constexpr (E4M3) {
+          float t[QOPS][4] = {};
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) s[nt][blk][0] = s[nt][blk][1] = s[nt][blk][2] = s[nt][blk][3] = 0.f;
-          float t[NT][4];
-          if constexpr (F32) {
+          for (int j = 0; j < QSTEPS; j++) {
+            const uint32_t b0 = expand2<true, 0>(kw[j]), b1 = expand2<true, 1>(kw[j]);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) t[nt][0] = t[nt][1] = t[nt][2] = t[nt][3] = 0.f;
+            for (int i = 0; i < QOPS; i++) mma_f16(t[i], qa[i][j], b0, b1);
           }
 #pragma unroll
-          for (int j = 0; j < D / 16; j++) {
-            const uint32_t f[4] = {expand2<true, 0>(ka[0][j]), expand2<true, 0>(ka[1][j]), expand2<true, 1>(ka[0][j]), expand2<true, 1>(ka[1][j])};
+          for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              mma_f16(s[nt][blk], f, qr[nt][j * 2], qr[nt][j * 2 + 1]);
-              if constexpr (F32) mma_f16(t[nt], f, qr[nt][(D / 16 + j) * 2], qr[nt][(D / 16 + j) * 2 + 1]);
+            for (int i = 0; i < 2; i++) {
+              if constexpr (F32)
+                s[nt][n8][i] = fmaf(t[nt][2 + i], 1.0f / 2048.0f, t[nt][i]);
+              else
+                s[nt][n8][i] = t[0][2 * nt + i];
             }
-          }
-          if constexpr (F32) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) s[nt][blk][i] = fmaf(t[nt][i], 1.0f / 2048.0f, s[nt][blk][i]);
-          }
         } else {
+          int t[QOPS][4] = {};
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            int t[3][4];
+          for (int j = 0; j < QSTEPS; j++)
 #pragma unroll
-            for (int d = 0; d < 3; d++) {
-              t[d][0] = t[d][1] = t[d][2] = t[d][3] = 0;
+            for (int i = 0; i < QOPS; i++) mma_s8(t[i], qa[i][j], kw[2 * j], kw[2 * j + 1]);
+          // each digit's sum is at most 2^21: the two low ones fit 32 bits together
 #pragma unroll
-              for (int j = 0; j < D / 32; j++)
-                mma_s8(t[d], ka[0][2 * j], ka[1][2 * j], ka[0][2 * j + 1], ka[1][2 * j + 1], qr[nt][d * (D / 16) + 2 * j],
-                       qr[nt][d * (D / 16) + 2 * j + 1]);
-            }
-            // each digit's sum is below 2^21: the two low ones fit 32 bits together
+          for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[nt][blk][i] = fmaf((float)t[2][i], 65536.0f, (float)(t[1][i] * 256 + t[0][i]));
-          }
+            for (int i = 0; i < 2; i++) s[nt][n8][i] = fmaf((float)t[nt][i], 65536.0f, (float)(t[nt][2 + i] * 256 + t[NT][2 * nt + i]));
         }
       }
 
@@ -492,76 +509,63 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           w_l[blk] = __uint_as_float((uint32_t)(127 - rel) << 23);
         }
       }
-      const bool edge = key0 + GROUP > lim_low || sk[0] < 0.f || sk[1] < 0.f;
-      float mx[NT][2];
+      float mx[NT];
       bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      for (int nt = 0; nt < NT; nt++) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-          float top = -INFINITY;
+        for (int n8 = 0; n8 < 4; n8++) {
+          const float k = row_c[nt] * sk[n8 >> 1];
 #pragma unroll
-          for (int blk = 0; blk < 2; blk++) {
-            const float k = row_c[nt][r] * sk[blk];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-              float v = fmaf(s[nt][blk][x * 2 + r], k, ex[blk]);
-              if (edge && (key0 + blk * 16 + x * 8 + g >= lim[nt][r] || sk[blk] < 0.f)) v = -INFINITY;
-              s[nt][blk][x * 2 + r] = v;
-              top = fmaxf(top, v);
-            }
+          for (int i = 0; i < 2; i++) {
+            float v = fmaf(s[nt][n8][i], k, ex[n8 >> 1]);
+            if (EDGE && (key0 + n8 * 8 + 2 * c + i >= lim[nt] || sk[n8 >> 1] < 0.f)) v = -INFINITY;
+            s[nt][n8][i] = v;
+            top = fmaxf(top, v);
           }
-          mx[nt][r] = top;
-          grow = grow || top > m[nt][r] + LAG;
         }
+        mx[nt] = top;
+        grow = grow || top > m[nt] + LAG;
+      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+          float top = mx[nt];
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float m_new = fmaxf(m[nt], top);
+          const float alpha = m[nt] == -INFINITY ? 0.f : ex2f(m[nt] - m_new);
+          m[nt] = m_new;
+          l[nt] *= alpha;
+          // the accumulators of this thread are rows 2c and 2c + 1
+          const float al[2] = {__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4)};
 #pragma unroll
-          for (int r = 0; r < 2; r++) {
-            float top = mx[nt][r];
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float m_new = fmaxf(m[nt][r], top);
-            const float alpha = m[nt][r] == -INFINITY ? 0.f : ex2f(m[nt][r] - m_new);
-            m[nt][r] = m_new;
-            l[nt][r] *= alpha;
+          for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-              o[nt][i][r] *= alpha;
-              o[nt][i][r + 2] *= alpha;
-            }
-          }
+            for (int x = 0; x < 4; x++) o[nt][i][x] *= al[x & 1];
+        }
       }
-      uint32_t ph[NT][2][2], pl[F32 ? NT : 1][2][2];
+      uint32_t ph[NT][4], pl[F32 ? NT : 1][4];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        float sum[2] = {0.f, 0.f};
+        const float ref = m[nt] == -INFINITY ? 0.f : m[nt] - P_SHIFT;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-          const float ref = m[nt][r] == -INFINITY ? 0.f : m[nt][r] - P_SHIFT;
+        for (int n8 = 0; n8 < 4; n8++) {
 #pragma unroll
-          for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const float p = ex2f(s[nt][blk][x * 2 + r] - ref);
-              sum[r][blk] += p;
-              s[nt][blk][x * 2 + r] = p * f[blk];
-              // a row that does not see the key takes 0 * f: a page's NaN must not reach it
-              if (edge && key0 + blk * 16 + x * 8 + g >= lim[nt][r]) s[nt][blk][x * 2 + r] = 0.f;
-            }
-          l[nt][r] += sum[r][0] * w_l[0] + sum[r][1] * w_l[1];
-        }
-#pragma unroll
-        for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const float x0 = s[nt][blk][x * 2], x1 = s[nt][blk][x * 2 + 1];
-            const uint32_t p = pack_half2(x0, x1);
-            ph[nt][blk][x] = transpose8x8(p);
-            if constexpr (F32) pl[nt][blk][x] = transpose8x8(pack_half2(x0 - half_lo(p), x1 - half_hi(p)));
+          for (int i = 0; i < 2; i++) {
+            const float p = ex2f(s[nt][n8][i] - ref);
+            sum[n8 >> 1] += p;
+            s[nt][n8][i] = p * f[n8 >> 1];
+            // a row that does not see the key takes 0 * f: a page's NaN must not reach it
+            if (EDGE && key0 + n8 * 8 + 2 * c + i >= lim[nt]) s[nt][n8][i] = 0.f;
           }
+          const float x0 = s[nt][n8][0], x1 = s[nt][n8][1];
+          ph[nt][n8] = pack_half2(x0, x1);
+          if constexpr (F32) pl[nt][n8] = pack_half2(x0 - half_lo(ph[nt][n8]), x1 - half_hi(ph[nt][n8]));
+        }
+        l[nt] += sum[0] * w_l[0] + sum[1] * w_l[1];
       }
 
       // O^T += V^T P^T, 16 keys per step: tokens 2c, 2c + 1, 2c + 8, 2c + 9, channels 16g .. or 8g ..; tile i has channels 2i, 2i + 1 of those
@@ -587,11 +591,23 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           const uint32_t va[4] = {expand2<E4M3, 0>(lo), expand2<E4M3, 1>(lo), expand2<E4M3, 0>(hi), expand2<E4M3, 1>(hi)};
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            if constexpr (F32) mma_f16(o[nt][i], va, pl[nt][blk][0], pl[nt][blk][1]);
-            mma_f16(o[nt][i], va, ph[nt][blk][0], ph[nt][blk][1]);
+            if constexpr (F32) mma_f16(o[nt][i], va, pl[nt][2 * blk], pl[nt][2 * blk + 1]);
+            mma_f16(o[nt][i], va, ph[nt][2 * blk], ph[nt][2 * blk + 1]);
           }
         }
       }
+    };
+
+    for (int it = 0; it < steps; it++) {
+      fetch(it + S::STAGES - 1);
+      look(it + S::STAGES);
+      cp_async_wait<S::STAGES - 1>();
+      __syncwarp();
+      const float* sc = scales + (it % S::STAGES) * 4;
+      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || sc[0] < 0.f || sc[2] < 0.f)
+        step(std::true_type{}, it);
+      else
+        step(std::false_type{}, it);
       __syncwarp();  // the stage is read: the next fetch may overwrite it
     }
     cp_async_wait<0>();
@@ -601,7 +617,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
     // r at k ^ ((r >> 1) & 3) ----
     float* acc = (float*)ring;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
       for (int r = 0; r < 2; r++) {
         const int row = nt * 8 + 2 * c + r;
@@ -609,12 +625,12 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
         for (int k = 0; k < MT / 2; k++)
           *(float4*)(acc + row * D + (((g * (D / 32) + k) ^ c) << 2)) =
               make_float4(o[nt][2 * k][r], o[nt][2 * k][r + 2], o[nt][2 * k + 1][r], o[nt][2 * k + 1][r + 2]);
-        float sum = l[nt][r];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (g == 0) *(float2*)(ml + (warp * ROWS + row) * 2) = make_float2(m[nt][r], sum);
       }
+      float sum = l[nt];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (c == 0) *(float2*)(ml + (warp * ROWS + nt * 8 + g) * 2) = make_float2(m[nt], sum);
+    }
     __syncthreads();
     const bool first = g_begin == 0, last = g_end == w.groups;
     const bool direct = first && last;
@@ -625,15 +641,9 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
         begun_cut = true;
         if (threadIdx.x == 0) {
           // the last unit of the tile lies with the CTA whose share holds it
-          const long long tail = base + (long long)(idx + 1) * w.groups - 1;
-          int cta = blockIdx.x + 1;
-          if (u_end <= tail) {
-            const long long all = scan[0] + scan[1] + scan[2] + scan[3];
-            cta = (int)(tail * shares / all);  // a close guess
-            while (all * cta / shares > tail) cta--;
-            while (all * (cta + 1) / shares <= tail) cta++;
-          }
-          ((Cut*)a.partial)[blockIdx.x] = Cut{w.row0, r0, (uint32_t)rn | (uint32_t)h << 16, cta};
+          const uint32_t tail = u - from + w.tile_units() - 1, split = (per_share + 1) * longer;
+          const uint32_t cta = tail < split ? tail / (per_share + 1) : longer + (tail - split) / per_share;
+          ((Cut*)a.partial)[blockIdx.x] = Cut{w.row0, r0, (uint32_t)rn | (uint32_t)h << 16, (int)min(cta, (uint32_t)shares - 1)};
         }
       }
     }
@@ -659,7 +669,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
         ll += x[v].y * scale;
       }
       if (direct) {
-        const int token = (r0 + r) / G, head = h * G + (r0 + r) - token * G;
+        const int token = by_g(r0 + r), head = h * G + (r0 + r) - token * G;
         const float inv = ll != 0.f ? __uint_as_float((uint32_t)(127 + e_ref) << 23) / ll : 0.f;
         const long long dst = (w.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + piece * 4;
         if constexpr (F32)
@@ -672,83 +682,109 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       }
     }
 
-    u += g_end - g_begin;
+    u += to - from;
     if (u >= u_end) break;
     __syncthreads();  // the ring is the next piece's
-    if (u - base >= (long long)w.tiles * w.groups * Hkv) {  // the next sequence with rows
+    if (u - base >= w.units(Hkv)) {  // the next sequence with rows
       base = u;
-      do {
-        b++;
-        w = work_of<ROWS>(a, G, b);
-      } while (w.tiles == 0);
+      w.tiles = 0;
+      while (w.tiles == 0 && ++b < a.batch.B) w = work_of<ROWS>(a, G, b);
+      if (b >= a.batch.B) break;  // (starts that overlap: more rows than there are)
     }
   }
   if (!whole && !begun_cut && threadIdx.x == 0) ((Cut*)a.partial)[blockIdx.x].last = -1;
 }
 
 // Joins the pieces of the cut tile that CTA i of the kernel above begins: o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p, with
-// A and M the largest of A_p = m_p + e_p and of m_p (log2).  A row is shared by JOIN_WARPS / ROWS warps, the pieces in order.
-constexpr int JOIN_WARPS = 16;
+// A and M the largest of A_p = m_p + e_p and of m_p (log2).  A row is shared by up to JOIN_WARPS / rows warps: each takes every
+// so-manieth piece, eight at a time, against maxima of its own, and the row's first warp joins them, always in the same order.
+constexpr int JOIN_WARPS = 16, JOIN_STEP = 8;
 template <int D, bool F32, int NT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) kv_join_kernel(const KvAttnArgs a) {
-  constexpr int ROWS = 8 * NT, SPLIT = JOIN_WARPS / ROWS, V = D / 32;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) kv_join_kernel(const KvAttnArgs a, const Divider by_g) {
+  constexpr int ROWS = 8 * NT, V = D / 32;
   __shared__ float acc[JOIN_WARPS][D];
-  __shared__ float sums[JOIN_WARPS];
+  __shared__ float4 sums[JOIN_WARPS];  // A, M, l
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the kernel above has left and is visible
+  asm volatile("griddepcontrol.launch_dependents;");
   const Cut cut = ((const Cut*)a.partial)[blockIdx.x];
   if (cut.last < 0) return;
   const int G = a.Hq / a.pool.Hkv;
   const int rn = (int)(cut.rows_head & 0xffffu), h = (int)(cut.rows_head >> 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = warp % ROWS, part = warp / ROWS;
+  const int width = rn <= 1 ? 1 : rn <= 2 ? 2 : rn <= 4 ? 4 : rn <= 8 ? 8 : 16;  // warps side by side
+  const int r = warp & (width - 1), part = warp / width, split = JOIN_WARPS / width;
   const int pieces = cut.last - (int)blockIdx.x + 1;
   const float* places = a.partial + gridDim.x * (sizeof(Cut) / 4);
-  auto place = [&](int p) {  // the first piece is the owner's second place, the others are first places
-    return places + (long long)(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * place_floats<D, ROWS>();
-  };
   float A = -INFINITY, M = -INFINITY, l = 0.f;
   float x[V];
 #pragma unroll
   for (int d = 0; d < V; d++) x[d] = 0.f;
   if (r < rn) {
-    for (int p = lane; p < pieces; p += 32) {
-      const float2 e = *(const float2*)(place(p) + ROWS * D + r * 4);
-      A = fmaxf(A, e.x);
-      M = fmaxf(M, e.y);
-    }
+    for (int p0 = part; p0 < pieces; p0 += split * JOIN_STEP) {
+      float4 e[JOIN_STEP];
+      float y[JOIN_STEP][V];
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      A = fmaxf(A, __shfl_xor_sync(0xffffffffu, A, s));
-      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-    }
-#pragma unroll 4
-    for (int p = part; p < pieces; p += SPLIT) {
-      const float* src = place(p);
-      const float4 e = *(const float4*)(src + ROWS * D + r * 4);
-      const bool none = e.y == -INFINITY && e.z == 0.f;
-      const float wo = none ? 0.f : ex2f(e.x - A), wl = none ? 0.f : ex2f(e.y - M);
-      l += e.z * wl;
-      if constexpr (D == 128) {
-        const float4 y = *(const float4*)(src + r * D + lane * 4);
-        x[0] += y.x * wo; x[1] += y.y * wo; x[2] += y.z * wo; x[3] += y.w * wo;
-      } else {
-        const float2 y = *(const float2*)(src + r * D + lane * 2);
-        x[0] += y.x * wo; x[1] += y.y * wo;
+      for (int i = 0; i < JOIN_STEP; i++) {
+        const int p = p0 + i * split;
+        e[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+#pragma unroll
+        for (int d = 0; d < V; d++) y[i][d] = 0.f;
+        if (p < pieces) {  // the first piece is the owner's second place, the others are first places
+          const float* src = places + (long long)(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * place_floats<D, ROWS>();
+          e[i] = *(const float4*)(src + ROWS * D + r * 4);
+          if constexpr (D == 128) {
+            const float4 v = *(const float4*)(src + r * D + lane * 4);
+            y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
+          } else {
+            const float2 v = *(const float2*)(src + r * D + lane * 2);
+            y[i][0] = v.x; y[i][1] = v.y;
+          }
+        }
+      }
+      float A_new = A, M_new = M;
+#pragma unroll
+      for (int i = 0; i < JOIN_STEP; i++) {
+        A_new = fmaxf(A_new, e[i].x);
+        M_new = fmaxf(M_new, e[i].y);
+      }
+      const float old_o = A == -INFINITY ? 0.f : ex2f(A - A_new), old_l = M == -INFINITY ? 0.f : ex2f(M - M_new);
+      // (0 * NaN is wanted: a NaN row has no maximum)
+      l = M == -INFINITY && l == 0.f ? 0.f : l * old_l;
+#pragma unroll
+      for (int d = 0; d < V; d++) x[d] *= old_o;
+      A = A_new;
+      M = M_new;
+#pragma unroll
+      for (int i = 0; i < JOIN_STEP; i++) {
+        const bool none = e[i].y == -INFINITY && e[i].z == 0.f;
+        const float wo = none || A == -INFINITY ? 0.f : ex2f(e[i].x - A), wl = none || M == -INFINITY ? 0.f : ex2f(e[i].y - M);
+        l += e[i].z * wl;
+#pragma unroll
+        for (int d = 0; d < V; d++) x[d] += y[i][d] * wo;
       }
     }
   }
 #pragma unroll
   for (int d = 0; d < V; d++) acc[warp][lane * V + d] = x[d];
-  if (lane == 0) sums[warp] = l;
+  if (lane == 0) sums[warp] = make_float4(A, M, l, 0.f);
   __syncthreads();
   if (part != 0 || r >= rn) return;
+  for (int k = 1; k < split; k++) {
+    A = fmaxf(A, sums[r + k * width].x);
+    M = fmaxf(M, sums[r + k * width].y);
+  }
+  l = 0.f;
 #pragma unroll
-  for (int s = 1; s < SPLIT; s++) {
-    l += sums[r + s * ROWS];
+  for (int d = 0; d < V; d++) x[d] = 0.f;
+  for (int k = 0; k < split; k++) {
+    const float4 e = sums[r + k * width];
+    const float wo = e.x == -INFINITY ? 0.f : ex2f(e.x - A), wl = e.y == -INFINITY ? 0.f : ex2f(e.y - M);
+    l += e.z * wl;
 #pragma unroll
-    for (int d = 0; d < V; d++) x[d] += acc[r + s * ROWS][lane * V + d];
+    for (int d = 0; d < V; d++) x[d] += acc[r + k * width][lane * V + d] * wo;
   }
   const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
-  const int token = (cut.r0 + r) / G, head = h * G + (cut.r0 + r) - token * G;
+  const int token = by_g(cut.r0 + r), head = h * G + (cut.r0 + r) - token * G;
   const long long dst = (cut.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + lane * V;
 #pragma unroll
   for (int d = 0; d < V; d += 2) {
@@ -767,13 +803,12 @@ cudaError_t launch(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t str
   if (e != cudaSuccess) return e;
   const dim3 grid = plan.ctas ? dim3((unsigned)plan.ctas)
                               : dim3((unsigned)kv_places(a.batch.B, a.batch.T, a.Hq / a.pool.Hkv, NT == 1 ? 3 : 4, 1), (unsigned)a.pool.Hkv);
-  kern<<<grid, WARPS * 32, S::BYTES, stream>>>(a, plan.ctas == 0);
-  e = cudaGetLastError();
+  const Divider by_g = divider((uint32_t)(a.Hq / a.pool.Hkv));
+  e = launch_early(kern, grid, dim3(WARPS * 32), S::BYTES, stream, a, by_g, plan.ctas == 0 ? 1 : 0);
   if (e != cudaSuccess) return e;
   ++*launches;
   if (plan.ctas) {
-    kv_join_kernel<D, F32, NT><<<(unsigned)plan.ctas, JOIN_WARPS * 32, 0, stream>>>(a);
-    e = cudaGetLastError();
+    e = launch_early(kv_join_kernel<D, F32, NT>, dim3((unsigned)plan.ctas), dim3(JOIN_WARPS * 32), 0, stream, a, by_g);
     if (e == cudaSuccess) ++*launches;
   }
   return e;
@@ -793,7 +828,7 @@ KvAttnPlan kv_attn_plan(const KvPool& pool, int B, int T, int dtype, int Hq, int
   p.rows = (long long)T * G <= 8ll * B ? 8 : 16;
   const long long tiles = kv_places(B, T, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
   p.ctas = SMS * (p.rows == 8 ? Sh<128, 1>::CTAS_PER_SM : Sh<128, 2>::CTAS_PER_SM);
-  if (max_length <= WHOLE_KEYS || tiles >= 16 * p.ctas) p.ctas = 0;
+  if (max_length <= WHOLE_KEYS || tiles >= 16 * p.ctas || tiles * ((max_length + GROUP - 1) / GROUP + START_UNITS) > 0xffffffffll) p.ctas = 0;
   p.workspace = (size_t)p.ctas * (sizeof(Cut) + 2 * sizeof(float) * p.rows * (pool.D + 4));
   return p;
 }
