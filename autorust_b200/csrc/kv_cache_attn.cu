@@ -41,8 +41,8 @@ constexpr int WARPS = 4;
 constexpr int SMS = 148;
 constexpr int LEAST_UNITS = 8;   // of a share
 // A row tile counts as its groups and START_UNITS more: beginning a piece (page numbers, Q, the first codes, the join of the
-// warps at its end) takes a CTA about as long as that many groups.
-constexpr int START_UNITS = 6;
+// warps at its end) takes a CTA about as long as that many groups (64 ragged sequences: 75 us with 4, 66 with 9, 67 with 12).
+constexpr int START_UNITS = 9;
 constexpr float P_SHIFT = 12.0f, LAG = 2.0f;
 constexpr int E_LIMIT = 100;    // largest |e - e_ref|
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60, the least scale a page is given
@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
   float* scales = (float*)(smem + S::SCALES) + warp * S::STAGES * 4;
   const int G = a.Hq / a.pool.Hkv, Hkv = a.pool.Hkv;
 
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // whatever came before in the stream is done and visible
   asm volatile("griddepcontrol.launch_dependents;");  // what comes next may take its places as CTAs leave; it waits for all of this
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // whatever came before in the stream is done and visible
 
   // ---- this CTA's share: units [u, u_end) of the groups of all row tiles, or one whole row tile ----
   // Every warp works it out for itself, without a barrier; 32-bit numbers, which the host has checked the sizes for.
@@ -546,7 +546,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
             for (int x = 0; x < 4; x++) o[nt][i][x] *= al[x & 1];
         }
       }
-      uint32_t ph[NT][4], pl[F32 ? NT : 1][4];
+      uint32_t ph[NT][4];
+      [[maybe_unused]] uint32_t pl[F32 ? NT : 1][4];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         float sum[2] = {0.f, 0.f};
@@ -695,103 +696,108 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
   if (!whole && !begun_cut && threadIdx.x == 0) ((Cut*)a.partial)[blockIdx.x].last = -1;
 }
 
-// Joins the pieces of the cut tile that CTA i of the kernel above begins: o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p, with
-// A and M the largest of A_p = m_p + e_p and of m_p (log2).  A row is shared by up to JOIN_WARPS / rows warps: each takes every
-// so-manieth piece, eight at a time, against maxima of its own, and the row's first warp joins them, always in the same order.
-constexpr int JOIN_WARPS = 16, JOIN_STEP = 8;
+// Joins the pieces of the cut tiles: o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p, with A and M the largest of
+// A_p = m_p + e_p and of m_p (log2).  CTA (x, y) takes the tiles that the CTAs x, x + gridDim.x, .. of the kernel above begin, and of
+// those the rows y, y + 4, ..; its warps share a row's pieces, each against maxima of its own, and the row's first warp joins
+// them, always in the same order.  A few small CTAs: they are in place and waiting before the last CTA above has left.
+constexpr int JOIN_WARPS = 8, JOIN_STEP = 7, JOIN_Y = 4;
 template <int D, bool F32, int NT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) kv_join_kernel(const KvAttnArgs a, const Divider by_g) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAttnArgs a, const Divider by_g, int ctas) {
   constexpr int ROWS = 8 * NT, V = D / 32;
   __shared__ float acc[JOIN_WARPS][D];
   __shared__ float4 sums[JOIN_WARPS];  // A, M, l
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the kernel above has left and is visible
   asm volatile("griddepcontrol.launch_dependents;");
-  const Cut cut = ((const Cut*)a.partial)[blockIdx.x];
-  if (cut.last < 0) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the kernel above has left and is visible
   const int G = a.Hq / a.pool.Hkv;
-  const int rn = (int)(cut.rows_head & 0xffffu), h = (int)(cut.rows_head >> 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int width = rn <= 1 ? 1 : rn <= 2 ? 2 : rn <= 4 ? 4 : rn <= 8 ? 8 : 16;  // warps side by side
-  const int r = warp & (width - 1), part = warp / width, split = JOIN_WARPS / width;
-  const int pieces = cut.last - (int)blockIdx.x + 1;
-  const float* places = a.partial + gridDim.x * (sizeof(Cut) / 4);
-  float A = -INFINITY, M = -INFINITY, l = 0.f;
-  float x[V];
+  const float* places = a.partial + ctas * (sizeof(Cut) / 4);
+  for (int first = blockIdx.x; first < ctas; first += gridDim.x) {
+    const Cut cut = ((const Cut*)a.partial)[first];
+    const int rn = (int)(cut.rows_head & 0xffffu), h = (int)(cut.rows_head >> 16);
+    if (cut.last < 0 || (int)blockIdx.y >= rn) continue;
+    const int mine = (rn - (int)blockIdx.y + JOIN_Y - 1) / JOIN_Y;  // rows of this CTA, at most 4
+    const int width = mine > 2 ? 4 : mine;                          // warps side by side
+    const int k = warp % width, part = warp / width, split = JOIN_WARPS / width;
+    const int r = (int)blockIdx.y + k * JOIN_Y;
+    const int pieces = cut.last - first + 1;
+    float A = -INFINITY, M = -INFINITY, l = 0.f;
+    float x[V];
 #pragma unroll
-  for (int d = 0; d < V; d++) x[d] = 0.f;
-  if (r < rn) {
-    for (int p0 = part; p0 < pieces; p0 += split * JOIN_STEP) {
-      float4 e[JOIN_STEP];
-      float y[JOIN_STEP][V];
+    for (int d = 0; d < V; d++) x[d] = 0.f;
+    if (r < rn) {
+      for (int p0 = part; p0 < pieces; p0 += split * JOIN_STEP) {
+        float4 e[JOIN_STEP];
+        float y[JOIN_STEP][V];
 #pragma unroll
-      for (int i = 0; i < JOIN_STEP; i++) {
-        const int p = p0 + i * split;
-        e[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+        for (int i = 0; i < JOIN_STEP; i++) {
+          const int p = p0 + i * split;
+          e[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
 #pragma unroll
-        for (int d = 0; d < V; d++) y[i][d] = 0.f;
-        if (p < pieces) {  // the first piece is the owner's second place, the others are first places
-          const float* src = places + (long long)(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * place_floats<D, ROWS>();
-          e[i] = *(const float4*)(src + ROWS * D + r * 4);
-          if constexpr (D == 128) {
-            const float4 v = *(const float4*)(src + r * D + lane * 4);
-            y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
-          } else {
-            const float2 v = *(const float2*)(src + r * D + lane * 2);
-            y[i][0] = v.x; y[i][1] = v.y;
+          for (int d = 0; d < V; d++) y[i][d] = 0.f;
+          if (p < pieces) {  // the first piece is the owner's second place, the others are first places
+            const float* src = places + (long long)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * place_floats<D, ROWS>();
+            e[i] = *(const float4*)(src + ROWS * D + r * 4);
+            if constexpr (D == 128) {
+              const float4 v = *(const float4*)(src + r * D + lane * 4);
+              y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
+            } else {
+              const float2 v = *(const float2*)(src + r * D + lane * 2);
+              y[i][0] = v.x; y[i][1] = v.y;
+            }
           }
         }
-      }
-      float A_new = A, M_new = M;
+        float A_new = A, M_new = M;
 #pragma unroll
-      for (int i = 0; i < JOIN_STEP; i++) {
-        A_new = fmaxf(A_new, e[i].x);
-        M_new = fmaxf(M_new, e[i].y);
-      }
-      const float old_o = A == -INFINITY ? 0.f : ex2f(A - A_new), old_l = M == -INFINITY ? 0.f : ex2f(M - M_new);
-      // (0 * NaN is wanted: a NaN row has no maximum)
-      l = M == -INFINITY && l == 0.f ? 0.f : l * old_l;
+        for (int i = 0; i < JOIN_STEP; i++) {
+          A_new = fmaxf(A_new, e[i].x);
+          M_new = fmaxf(M_new, e[i].y);
+        }
+        const float old_o = A == -INFINITY ? 0.f : ex2f(A - A_new), old_l = M == -INFINITY ? 0.f : ex2f(M - M_new);
+        l *= old_l;  // (0 * NaN is wanted: a row of NaN has no maximum)
 #pragma unroll
-      for (int d = 0; d < V; d++) x[d] *= old_o;
-      A = A_new;
-      M = M_new;
+        for (int d = 0; d < V; d++) x[d] *= old_o;
+        A = A_new;
+        M = M_new;
 #pragma unroll
-      for (int i = 0; i < JOIN_STEP; i++) {
-        const bool none = e[i].y == -INFINITY && e[i].z == 0.f;
-        const float wo = none || A == -INFINITY ? 0.f : ex2f(e[i].x - A), wl = none || M == -INFINITY ? 0.f : ex2f(e[i].y - M);
-        l += e[i].z * wl;
+        for (int i = 0; i < JOIN_STEP; i++) {
+          const bool none = e[i].y == -INFINITY && e[i].z == 0.f;
+          const float wo = none || A == -INFINITY ? 0.f : ex2f(e[i].x - A), wl = none || M == -INFINITY ? 0.f : ex2f(e[i].y - M);
+          l += e[i].z * wl;
 #pragma unroll
-        for (int d = 0; d < V; d++) x[d] += y[i][d] * wo;
+          for (int d = 0; d < V; d++) x[d] += y[i][d] * wo;
+        }
       }
     }
-  }
+    __syncthreads();  // (the tile before has been read)
 #pragma unroll
-  for (int d = 0; d < V; d++) acc[warp][lane * V + d] = x[d];
-  if (lane == 0) sums[warp] = make_float4(A, M, l, 0.f);
-  __syncthreads();
-  if (part != 0 || r >= rn) return;
-  for (int k = 1; k < split; k++) {
-    A = fmaxf(A, sums[r + k * width].x);
-    M = fmaxf(M, sums[r + k * width].y);
-  }
-  l = 0.f;
+    for (int d = 0; d < V; d++) acc[warp][lane * V + d] = x[d];
+    if (lane == 0) sums[warp] = make_float4(A, M, l, 0.f);
+    __syncthreads();
+    if (part != 0 || r >= rn) continue;
+    for (int i = 1; i < split; i++) {
+      A = fmaxf(A, sums[k + i * width].x);
+      M = fmaxf(M, sums[k + i * width].y);
+    }
+    l = 0.f;
 #pragma unroll
-  for (int d = 0; d < V; d++) x[d] = 0.f;
-  for (int k = 0; k < split; k++) {
-    const float4 e = sums[r + k * width];
-    const float wo = e.x == -INFINITY ? 0.f : ex2f(e.x - A), wl = e.y == -INFINITY ? 0.f : ex2f(e.y - M);
-    l += e.z * wl;
+    for (int d = 0; d < V; d++) x[d] = 0.f;
+    for (int i = 0; i < split; i++) {
+      const float4 e = sums[k + i * width];
+      const float wo = e.x == -INFINITY ? 0.f : ex2f(e.x - A), wl = e.y == -INFINITY ? 0.f : ex2f(e.y - M);
+      l += e.z * wl;
 #pragma unroll
-    for (int d = 0; d < V; d++) x[d] += acc[r + k * width][lane * V + d] * wo;
-  }
-  const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
-  const int token = by_g(cut.r0 + r), head = h * G + (cut.r0 + r) - token * G;
-  const long long dst = (cut.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + lane * V;
+      for (int d = 0; d < V; d++) x[d] += acc[k + i * width][lane * V + d] * wo;
+    }
+    const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
+    const int token = by_g(cut.r0 + r), head = h * G + (cut.r0 + r) - token * G;
+    const long long dst = (cut.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + lane * V;
 #pragma unroll
-  for (int d = 0; d < V; d += 2) {
-    if constexpr (F32)
-      *(float2*)((float*)a.o.p + dst + d) = make_float2(x[d] * inv, x[d + 1] * inv);
-    else
-      *(uint32_t*)((__nv_bfloat16*)a.o.p + dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+    for (int d = 0; d < V; d += 2) {
+      if constexpr (F32)
+        *(float2*)((float*)a.o.p + dst + d) = make_float2(x[d] * inv, x[d + 1] * inv);
+      else
+        *(uint32_t*)((__nv_bfloat16*)a.o.p + dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+    }
   }
 }
 
@@ -808,7 +814,7 @@ cudaError_t launch(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t str
   if (e != cudaSuccess) return e;
   ++*launches;
   if (plan.ctas) {
-    e = launch_early(kv_join_kernel<D, F32, NT>, dim3((unsigned)plan.ctas), dim3(JOIN_WARPS * 32), 0, stream, a, by_g);
+    e = launch_early(kv_join_kernel<D, F32, NT>, dim3(SMS, JOIN_Y), dim3(JOIN_WARPS * 32), 0, stream, a, by_g, plan.ctas);
     if (e == cudaSuccess) ++*launches;
   }
   return e;
