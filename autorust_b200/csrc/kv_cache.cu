@@ -14,7 +14,7 @@ int check_pool(const ar_kv_pool* p, ar::KvPool* out) {
   int log2 = 4;
   while (log2 < 8 && (1 << log2) != p->page) log2++;
   if (log2 == 8 || p->pages > INT32_MAX || p->Hkv > 65535) return AR_ERR_UNSUPPORTED;
-  if (!aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->k_scale, 4) || !aligned(p->v_scale, 4) || !aligned(p->k_mean, 4))
+  if (!aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->k_scale, 4) || !aligned(p->v_scale, 4) || !aligned(p->k_mean, 16))
     return AR_ERR_ALIGNMENT;
   *out = ar::KvPool{(uint8_t*)p->k, (uint8_t*)p->v, p->k_scale, p->v_scale, p->k_mean, (int)p->pages, (int)p->Hkv, (int)p->D, log2,
                     p->format == AR_KV_E4M3};

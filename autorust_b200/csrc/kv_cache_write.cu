@@ -4,12 +4,16 @@
 //           s = s1, or max(s0, s1) on a page that holds earlier tokens;  code = rn(x * (1 / s)), earlier codes rn(code * (s0 / s))
 //   read    x = code * s (+ mean)
 //
-// Both are bound by memory: (1 + element size) bytes per value.  One CTA owns one page of one head, so that nothing is
+// Both are bound by memory: (1 + element size) bytes per value.  One CTA owns one page of one head at a time, so that nothing is
 // shared between CTAs: the page's tokens are loaded once, 32 values per thread, and stay in registers between the maximum and the
-// codes.  K and V are the two halves of grid.z.
+// codes.  Finding the sequence, its length and its page is a chain of dependent loads, about 2.5 us: in large calls a CTA takes
+// several heads of its page one after the other, and asks for the next head's values before it works on this one's.  K and V
+// are the two halves of grid.z.
 #include <cuda_bf16.h>
 
 #include "kv_cache.cuh"
+
+#include <algorithm>
 
 namespace ar {
 namespace {
@@ -18,16 +22,31 @@ constexpr int PER_THREAD = 32;              // values per thread
 constexpr int VECS = PER_THREAD / 8;        // in vectors of 8
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60: an empty or all-zero page needs no case of its own
 
+// 8 values as they lie in memory.
 template <bool F32>
-__device__ __forceinline__ void load8(const void* base, long long at, float (&x)[8]) {
+struct Raw {
+  uint4 w[F32 ? 2 : 1];
+};
+template <bool F32>
+__device__ __forceinline__ Raw<F32> load8(const void* base, long long at) {
+  Raw<F32> r;
+  const uint4* p = F32 ? (const uint4*)((const float*)base + at) : (const uint4*)((const __nv_bfloat16*)base + at);
+#pragma unroll
+  for (int i = 0; i < (F32 ? 2 : 1); i++) r.w[i] = p[i];
+  return r;
+}
+template <bool F32>
+__device__ __forceinline__ void values8(const Raw<F32>& r, float (&x)[8]) {
   if constexpr (F32) {
-    const float4* p = (const float4*)((const float*)base + at);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      x[4 * i] = __uint_as_float(r.w[i].x);
+      x[4 * i + 1] = __uint_as_float(r.w[i].y);
+      x[4 * i + 2] = __uint_as_float(r.w[i].z);
+      x[4 * i + 3] = __uint_as_float(r.w[i].w);
+    }
   } else {
-    const uint4 w = *(const uint4*)((const __nv_bfloat16*)base + at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       x[2 * i] = __uint_as_float(u[i] << 16);
@@ -84,149 +103,184 @@ __device__ __forceinline__ float scale_of(uint32_t bits, int e4m3) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
-// E values of a page and head, E / 32 threads.
+// What a CTA does: the rows [t0, t1) of a page, packed rows row0 + t.
+struct Span {
+  int page;         // -1: there is none (reported)
+  int t0, t1;
+  long long row0;
+  int padding;      // read: this many of the sequence's rows, from pad_row on, have no token
+  long long pad_row;
+};
+__device__ __forceinline__ Span span_of(const KvPool& pool, const KvBatch& batch) {
+  const KvPlace p = kv_place(batch, blockIdx.x, 1, pool.page_log2, 2);
+  Span s{-1, 0, 0, 0, 0, 0};
+  if (p.tile < 0 || p.n <= 0) return s;
+  const int first = max(p.length - p.n, 0);      // position of the first token
+  const int skipped = max(p.n - p.length, 0);    // padding rows in front of it (negative positions)
+  if (p.tile == 0) s.padding = skipped;
+  s.pad_row = p.row0;
+  const int blk = (first >> pool.page_log2) + p.tile;    // block of the sequence
+  const long long at0 = (long long)blk << pool.page_log2;  // its first token
+  s.t0 = (int)max((long long)first - at0, 0ll);
+  s.t1 = (int)min((long long)first + (p.n - skipped) - at0, 1ll << pool.page_log2);
+  s.row0 = p.row0 + skipped + (at0 - first);
+  if (s.t1 > s.t0) {
+    s.page = kv_page(pool, batch, p.b, blk);
+    if (s.page < 0 && threadIdx.x == 0) kv_report(batch);
+  }
+  return s;
+}
+
+// E values of a page and head, E / 32 threads; heads blockIdx.y, blockIdx.y + gridDim.y, ...
 template <int E, bool F32>
-__global__ void __launch_bounds__(E / PER_THREAD)
+__global__ void __launch_bounds__(E / PER_THREAD, E == 16384 ? 1 : (F32 ? 512 : 768) * PER_THREAD / E)
 kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
   constexpr int THREADS = E / PER_THREAD;
-  const int page_tokens = 1 << pool.page_log2;
+  __shared__ uint32_t tops[2][THREADS / 32];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int d_log2 = pool.D == 128 ? 7 : 6;
-  const KvPlace p = kv_place(batch, blockIdx.x, 1, pool.page_log2, 2);
-  const int first = max(p.length - p.n, 0);            // position of the first token that is written
-  const int skipped = max(p.n - p.length, 0);          // padding rows in front of it (negative positions)
-  const int count = p.n - skipped;
-  if (p.tile < 0 || count <= 0) return;
-  const int blk = (first >> pool.page_log2) + p.tile;  // block of the sequence
-  const long long at0 = (long long)blk << pool.page_log2;                         // its first token
-  const int t0 = (int)max((long long)first - at0, 0ll);                           // rows of the page before the first new token
-  const int t1 = (int)min((long long)first + count - at0, (long long)page_tokens);  // and up to the last
-  if (t1 <= t0) return;
-  const int h = blockIdx.y;
+  const Span span = span_of(pool, batch);
+  if (span.page < 0) return;
   const bool is_v = blockIdx.z != 0;
-  const int page = kv_page(pool, batch, p.b, blk);
-  if (page < 0) {
-    if (threadIdx.x == 0) kv_report(batch);
-    return;
-  }
   const KvRows& rows = is_v ? vr : kr;
-  uint8_t* codes = (is_v ? pool.v : pool.k) + ((long long)page * pool.Hkv + h) * E;
-  float* scale_at = (is_v ? pool.v_scale : pool.k_scale) + (long long)page * pool.Hkv + h;
-  const float s0 = t0 > 0 ? *scale_at : 0.0f;
-  const float* mean = !is_v && pool.k_mean ? pool.k_mean + h * pool.D : nullptr;
-  const long long row0 = p.row0 + skipped + (at0 - first);  // packed row of the page's row 0
-
-  float x[VECS][8];
-  uint32_t top = 0;
+  uint8_t* page_codes = (is_v ? pool.v : pool.k) + (long long)span.page * pool.Hkv * E;
+  float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)span.page * pool.Hkv;
+  Raw<F32> raw[VECS];
+  float next_s0 = 0.f;
+  auto fetch = [&](int h) {
+    if (h >= pool.Hkv) return;
+    if (span.t0 > 0) next_s0 = scales[h];
 #pragma unroll
-  for (int i = 0; i < VECS; i++) {
-    const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
-    if (t >= t0 && t < t1) {
-      load8<F32>(rows.p, (row0 + t) * rows.st + (long long)h * rows.sh + d, x[i]);
-      if (mean) {
+    for (int i = 0; i < VECS; i++) {
+      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
+      if (t >= span.t0 && t < span.t1) raw[i] = load8<F32>(rows.p, (span.row0 + t) * rows.st + (long long)h * rows.sh + d);
+    }
+  };
+  fetch(blockIdx.y);
+  for (int h = blockIdx.y, n = 0; h < pool.Hkv; h += gridDim.y, n ^= 1) {
+    const float* mean = !is_v && pool.k_mean ? pool.k_mean + h * pool.D : nullptr;
+    const float s0 = next_s0;
+    float x[VECS][8];
+    uint32_t top = 0;
 #pragma unroll
-        for (int c = 0; c < 8; c++) x[i][c] -= mean[d + c];
+    for (int i = 0; i < VECS; i++) {
+      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
+      if (t >= span.t0 && t < span.t1) {
+        values8<F32>(raw[i], x[i]);
+        if (mean) {
+          const float4 a = *(const float4*)(mean + d), b = *(const float4*)(mean + d + 4);
+          x[i][0] -= a.x; x[i][1] -= a.y; x[i][2] -= a.z; x[i][3] -= a.w;
+          x[i][4] -= b.x; x[i][5] -= b.y; x[i][6] -= b.z; x[i][7] -= b.w;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++) top = max(top, __float_as_uint(x[i][c]) & 0x7fffffffu);
       }
-#pragma unroll
-      for (int c = 0; c < 8; c++) top = max(top, __float_as_uint(x[i][c]) & 0x7fffffffu);
     }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if constexpr (THREADS > 32) {
-    __shared__ uint32_t tops[THREADS / 32];
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
+    fetch(h + gridDim.y);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (THREADS > 32) {
+      if ((threadIdx.x & 31) == 0) tops[n][threadIdx.x >> 5] = top;
+      __syncthreads();  // (the other half of tops is written before the next one: no second barrier)
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; i++) top = max(top, tops[i]);
-  } else {
-    __syncwarp();
-  }
-  float s = scale_of(top, pool.e4m3);
-  if (t0 > 0 && !(s > s0) && s == s) s = s0;  // (a NaN on either side stays)
-  const bool dead = s != s;
-  const float inverse = 1.0f / s;
-#pragma unroll
-  for (int i = 0; i < VECS; i++) {
-    const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
-    if (t >= t0 && t < t1) {
-      float y[8];
-#pragma unroll
-      for (int c = 0; c < 8; c++) y[c] = x[i][c] * inverse;
-      *(uint2*)(codes + e) = encode8(y, pool.e4m3, dead);
+      for (int i = 0; i < THREADS / 32; i++) top = max(top, tops[n][i]);
+    } else {
+      __syncwarp();
     }
-  }
-  if (t0 > 0 && s > s0) {  // the scale has grown: the earlier codes move to it
-    const float ratio = s0 / s;
-    for (int e = threadIdx.x * 8; e < (t0 << d_log2); e += THREADS * 8) {
-      float y[8];
-      decode8(*(const uint2*)(codes + e), pool.e4m3, y);
+    uint8_t* codes = page_codes + (long long)h * E;
+    float s = scale_of(top, pool.e4m3);
+    if (span.t0 > 0 && !(s > s0) && s == s) s = s0;  // (a NaN on either side stays)
+    const bool dead = s != s;
+    const float inverse = 1.0f / s;
 #pragma unroll
-      for (int c = 0; c < 8; c++) y[c] *= ratio;
-      *(uint2*)(codes + e) = encode8(y, pool.e4m3, false);
+    for (int i = 0; i < VECS; i++) {
+      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
+      if (t >= span.t0 && t < span.t1) {
+        float y[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) y[c] = x[i][c] * inverse;
+        *(uint2*)(codes + e) = encode8(y, pool.e4m3, dead);
+      }
     }
+    if (span.t0 > 0 && s > s0) {  // the scale has grown: the earlier codes move to it
+      const float ratio = s0 / s;
+      for (int e = threadIdx.x * 8; e < (span.t0 << d_log2); e += THREADS * 8) {
+        float y[8];
+        decode8(*(const uint2*)(codes + e), pool.e4m3, y);
+#pragma unroll
+        for (int c = 0; c < 8; c++) y[c] *= ratio;
+        *(uint2*)(codes + e) = encode8(y, pool.e4m3, false);
+      }
+    }
+    if (threadIdx.x == 0) scales[h] = s;
   }
-  if (threadIdx.x == 0) *scale_at = s;
 }
 
 template <int E, bool F32>
 __global__ void __launch_bounds__(E / PER_THREAD)
 kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
   constexpr int THREADS = E / PER_THREAD;
-  const int page_tokens = 1 << pool.page_log2;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int d_log2 = pool.D == 128 ? 7 : 6;
-  const KvPlace p = kv_place(batch, blockIdx.x, 1, pool.page_log2, 2);
-  if (p.tile < 0 || p.n <= 0) return;
-  const int first = max(p.length - p.n, 0);
-  const int skipped = max(p.n - p.length, 0);
-  const int count = p.n - skipped;
-  const int h = blockIdx.y;
+  const Span span = span_of(pool, batch);
   const bool is_v = blockIdx.z != 0;
   const KvRows& rows = is_v ? vr : kr;
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (p.tile == 0) {  // padding rows
-    for (long long e = threadIdx.x * 8; e < ((long long)skipped << d_log2); e += THREADS * 8)
-      store8<F32>(rows.p, (p.row0 + (e >> d_log2)) * rows.st + (long long)h * rows.sh + (e & (pool.D - 1)), zero);
+  if (span.padding > 0) {
+    for (int h = blockIdx.y; h < pool.Hkv; h += gridDim.y)
+      for (long long e = threadIdx.x * 8; e < ((long long)span.padding << d_log2); e += THREADS * 8)
+        store8<F32>(rows.p, (span.pad_row + (e >> d_log2)) * rows.st + (long long)h * rows.sh + (e & (pool.D - 1)), zero);
   }
-  const int blk = (first >> pool.page_log2) + p.tile;
-  const long long at0 = (long long)blk << pool.page_log2;
-  const int t0 = (int)max((long long)first - at0, 0ll);
-  const int t1 = (int)min((long long)first + count - at0, (long long)page_tokens);
-  if (t1 <= t0) return;
-  const int page = kv_page(pool, batch, p.b, blk);
-  if (page < 0 && threadIdx.x == 0) kv_report(batch);
-  const uint8_t* codes = (is_v ? pool.v : pool.k) + ((long long)max(page, 0) * pool.Hkv + h) * E;
-  const float s = (is_v ? pool.v_scale : pool.k_scale)[(long long)max(page, 0) * pool.Hkv + h];
-  const float* mean = !is_v && pool.k_mean ? pool.k_mean + h * pool.D : nullptr;
-  const long long row0 = p.row0 + skipped + (at0 - first);
+  if (span.t1 <= span.t0) return;
+  const uint8_t* page_codes = (is_v ? pool.v : pool.k) + (long long)max(span.page, 0) * pool.Hkv * E;
+  const float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)max(span.page, 0) * pool.Hkv;
   uint2 w[VECS];
+  float next_s = 0.f;
+  auto fetch = [&](int h) {
+    if (h >= pool.Hkv) return;
+    next_s = scales[h];
 #pragma unroll
-  for (int i = 0; i < VECS; i++) {
-    const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
-    if (t >= t0 && t < t1) w[i] = *(const uint2*)(codes + e);
-  }
+    for (int i = 0; i < VECS; i++) {
+      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
+      if (t >= span.t0 && t < span.t1) w[i] = *(const uint2*)(page_codes + (long long)h * E + e);
+    }
+  };
+  fetch(blockIdx.y);
+  for (int h = blockIdx.y; h < pool.Hkv; h += gridDim.y) {
+    const float* mean = !is_v && pool.k_mean && span.page >= 0 ? pool.k_mean + h * pool.D : nullptr;
+    const float s = next_s;
+    uint2 now[VECS];
 #pragma unroll
-  for (int i = 0; i < VECS; i++) {
-    const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
-    if (t >= t0 && t < t1) {
-      float x[8];
-      decode8(w[i], pool.e4m3, x);
+    for (int i = 0; i < VECS; i++) now[i] = w[i];
+    fetch(h + gridDim.y);
 #pragma unroll
-      for (int c = 0; c < 8; c++) x[c] = page < 0 ? 0.f : x[c] * s;
-      if (mean && page >= 0) {
+    for (int i = 0; i < VECS; i++) {
+      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
+      if (t >= span.t0 && t < span.t1) {
+        float x[8];
+        decode8(now[i], pool.e4m3, x);
 #pragma unroll
-        for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[d + c]);  // (not contracted: the definition rounds the product)
+        for (int c = 0; c < 8; c++) x[c] = span.page < 0 ? 0.f : x[c] * s;
+        if (mean) {
+#pragma unroll
+          for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[d + c]);  // (not contracted: the definition rounds the product)
+        }
+        store8<F32>(rows.p, (span.row0 + t) * rows.st + (long long)h * rows.sh + d, x);
       }
-      store8<F32>(rows.p, (row0 + t) * rows.st + (long long)h * rows.sh + d, x);
     }
   }
 }
 
+// CTAs up to which every head of a page gets one of its own: 16 per SM.
+constexpr int SPREAD_CTAS = 16 * 148;
+
 template <bool WRITE, bool F32>
 cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, const KvRows& v, cudaStream_t stream) {
-  const dim3 grid((unsigned)kv_places(batch.B, batch.T, 1, pool.page_log2, 2), (unsigned)pool.Hkv, 2);
-  auto go = [&](auto kern, int E) {
-    kern<<<grid, E / PER_THREAD, 0, stream>>>(pool, batch, k, v);
-    return cudaGetLastError();
-  };
+  const long long places = kv_places(batch.B, batch.T, 1, pool.page_log2, 2);
+  const long long per_cta = std::max(1ll, std::min((long long)pool.Hkv, places * pool.Hkv * 2 / SPREAD_CTAS));  // heads
+  const dim3 grid((unsigned)places, (unsigned)((pool.Hkv + per_cta - 1) / per_cta), 2);
+  auto go = [&](auto kern, int E) { return launch_early(kern, grid, dim3(E / PER_THREAD), 0, stream, pool, batch, k, v); };
 #define AR_KV_E(E) (WRITE ? go(kv_append_kernel<E, F32>, E) : go(kv_read_kernel<E, F32>, E))
   switch (pool.D << pool.page_log2) {
     case 1024: return AR_KV_E(1024);

@@ -273,8 +273,8 @@ int ar_sage_forward_static(int dtype, const void* q, const void* k, const void* 
  * The pool is cut into pages of `page` tokens, and a page of one kv head is the block that shares a scale:
  *   k, v              [pages, Hkv, page, D] codes, dense, 16-byte aligned: int8, or E4M3 bit patterns
  *   k_scale, v_scale  [pages, Hkv] f32; a code stands for code * scale
- *   k_mean            [Hkv, D] f32 or NULL: an offset per kv head and channel that is subtracted from the keys before they
- *                     are quantised and added when they are read back (the smoothing of ar_sage_quantize with a mean
+ *   k_mean            [Hkv, D] f32, 16-byte aligned, or NULL: an offset per kv head and channel that is subtracted
+ *                     from the keys before they are quantised and added when they are read back (the smoothing of ar_sage_quantize with a mean
  *                     that is fixed beforehand; attention does not depend on it: it moves all logits of a row alike)
  * page is 16, 32, 64 or 128; D is 64 or 128. */
 enum ar_kv_format { AR_KV_INT8 = 0, AR_KV_E4M3 = 1 };
