@@ -183,7 +183,7 @@ struct KvAttnPlan {
   int rows, ctas;
   size_t workspace;
 };
-KvAttnPlan kv_attn_plan(const KvPool& pool, int B, int T, int dtype, int Hq, int max_length, int causal);
+KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal);
 cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches);
 
 // Sage prologue (sage_prologue.cu).

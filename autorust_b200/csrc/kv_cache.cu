@@ -100,7 +100,7 @@ size_t ar_kv_cache_attention_workspace_bytes(const ar_kv_pool* pool, const ar_kv
   ar::KvPool p;
   ar::KvBatch s;
   if (check_attention(pool, batch, dtype, Hq, max_length, &p, &s) != AR_OK || s.T == 0) return 0;
-  return ar::kv_attn_plan(p, s.B, s.T, dtype, (int)Hq, (int)max_length, causal).workspace;
+  return ar::kv_attn_plan(p, s, dtype, (int)Hq, (int)max_length, causal).workspace;
 }
 
 int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* q,
@@ -117,7 +117,7 @@ int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int 
   a.max_length = (int)max_length;
   a.causal = causal ? 1 : 0;
   a.partial = (float*)workspace;
-  const ar::KvAttnPlan plan = ar::kv_attn_plan(a.pool, a.batch.B, a.batch.T, dtype, a.Hq, a.max_length, a.causal);
+  const ar::KvAttnPlan plan = ar::kv_attn_plan(a.pool, a.batch, dtype, a.Hq, a.max_length, a.causal);
   if (plan.workspace > 0) {
     if (!workspace || workspace_bytes < plan.workspace) return AR_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return AR_ERR_ALIGNMENT;

@@ -26,6 +26,10 @@ __device__ __forceinline__ long long kv_base(const KvBatch& s, int b, int rows_p
   return (((long long)kv_start(s, b) * rows_per) >> tile_log2) + (long long)slack * b;
 }
 __device__ __forceinline__ KvPlace kv_place(const KvBatch& s, int place, int rows_per, int tile_log2, int slack) {
+  if (!s.starts) {  // one row each: the place says which
+    const int tiles = ((rows_per - 1) >> tile_log2) + 1, b = place / tiles;
+    return KvPlace{b, place - b * tiles, b, 1, max(s.lengths[b], 0)};
+  }
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = s.B;
   while (hi - lo > 1) {
@@ -39,14 +43,15 @@ __device__ __forceinline__ KvPlace kv_place(const KvBatch& s, int place, int row
   KvPlace p;
   p.b = lo;
   p.row0 = kv_start(s, lo);
-  p.n = s.starts ? max(kv_start(s, lo + 1) - p.row0, 0) : 1;
+  p.n = max(kv_start(s, lo + 1) - p.row0, 0);
   p.tile = (int)(place - kv_base(s, lo, rows_per, tile_log2, slack));  // (may be negative in front of starts[0])
   p.length = max(s.lengths[lo], 0);
   return p;
 }
 // Places of such a grid.
-inline long long kv_places(long long B, long long T, long long rows_per, int tile_log2, int slack) {
-  return ((T * rows_per) >> tile_log2) + slack * B;
+inline long long kv_places(const KvBatch& s, int rows_per, int tile_log2, int slack) {
+  if (!s.starts) return (((rows_per - 1) >> tile_log2) + 1) * (long long)s.B;
+  return (((long long)s.T * rows_per) >> tile_log2) + (long long)slack * s.B;
 }
 
 __device__ __forceinline__ void kv_report(const KvBatch& s) {
@@ -77,14 +82,21 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_
 }
 
 // ---- codes ----
-// An E4M3 pattern moved into an f16 (sign, and the 7 other bits one place to the right) is its value times 2^-8, subnormals
-// included: the exponent biases are 7 and 15.
-__device__ __forceinline__ float e4m3_value(uint32_t code) {
-  const uint32_t h = ((code & 0x80u) << 8) | ((code & 0x7fu) << 7);
-  return __half2float(__ushort_as_half((unsigned short)h)) * 256.0f;
-}
-__device__ __forceinline__ float kv_value(uint32_t code, int e4m3) {
-  return e4m3 ? e4m3_value(code) : (float)(int)(int8_t)code;
+// The four codes of w -> f32.
+template <bool E4M3>
+__device__ __forceinline__ void kv_values4(uint32_t w, float (&x)[4]) {
+  if constexpr (E4M3) {
+    uint32_t lo, hi;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&lo)), q = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+  } else {  // code + 128 in the low byte of 2^23
+    const uint32_t u = w ^ 0x80808080u;
+    x[0] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f;
+    x[1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f;
+    x[2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f;
+    x[3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f;
+  }
 }
 // Two values -> two E4M3 codes, round to nearest even (the caller keeps them inside +-448).
 __device__ __forceinline__ uint32_t e4m3_codes(float lo, float hi) {

@@ -808,7 +808,7 @@ cudaError_t launch(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t str
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
   if (e != cudaSuccess) return e;
   const dim3 grid = plan.ctas ? dim3((unsigned)plan.ctas)
-                              : dim3((unsigned)kv_places(a.batch.B, a.batch.T, a.Hq / a.pool.Hkv, NT == 1 ? 3 : 4, 1), (unsigned)a.pool.Hkv);
+                              : dim3((unsigned)kv_places(a.batch, a.Hq / a.pool.Hkv, NT == 1 ? 3 : 4, 1), (unsigned)a.pool.Hkv);
   const Divider by_g = divider((uint32_t)(a.Hq / a.pool.Hkv));
   e = launch_early(kern, grid, dim3(WARPS * 32), S::BYTES, stream, a, by_g, plan.ctas == 0 ? 1 : 0);
   if (e != cudaSuccess) return e;
@@ -826,13 +826,13 @@ cudaError_t launch_nt(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t 
 
 }  // namespace
 
-KvAttnPlan kv_attn_plan(const KvPool& pool, int B, int T, int dtype, int Hq, int max_length, int causal) {
+KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal) {
   (void)dtype;
   (void)causal;
   KvAttnPlan p;
   const int G = Hq / pool.Hkv;
-  p.rows = (long long)T * G <= 8ll * B ? 8 : 16;
-  const long long tiles = kv_places(B, T, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
+  p.rows = (long long)batch.T * G <= 8ll * batch.B ? 8 : 16;
+  const long long tiles = kv_places(batch, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
   p.ctas = SMS * (p.rows == 8 ? Sh<128, 1>::CTAS_PER_SM : Sh<128, 2>::CTAS_PER_SM);
   if (max_length <= WHOLE_KEYS || tiles >= 16 * p.ctas || tiles * ((max_length + GROUP - 1) / GROUP + START_UNITS) > 0xffffffffll) p.ctas = 0;
   p.workspace = (size_t)p.ctas * (sizeof(Cut) + 2 * sizeof(float) * p.rows * (pool.D + 4));

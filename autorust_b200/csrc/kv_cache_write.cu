@@ -69,34 +69,49 @@ __device__ __forceinline__ void store8(void* base, long long at, const float (&x
   }
 }
 
-// Codes of 8 values that are already divided by the scale; `dead` (a NaN scale): zeros, since the codes of a page must stay
-// finite for the products of rows that do not see it.
-__device__ __forceinline__ uint2 encode8(const float (&y)[8], int e4m3, bool dead) {
-  uint32_t w[2] = {0u, 0u};
-  if (!dead) {
+// Codes of 8 values that are already divided by the scale (and so inside +-127 or +-448); `dead` (a NaN scale): zeros, since the
+// codes of a page must stay finite for the products of rows that do not see it.
+template <bool E4M3>
+__device__ __forceinline__ uint2 encode8(const float (&y)[8], bool dead) {
+  uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      uint32_t two;
-      if (e4m3) {
-        two = e4m3_codes(y[i], y[i + 1]);
-      } else {
-        const int a = max(-127, min(127, __float2int_rn(y[i]))), b = max(-127, min(127, __float2int_rn(y[i + 1])));
-        two = (uint32_t)(a & 0xff) | ((uint32_t)(b & 0xff) << 8);
-      }
-      w[i >> 2] |= two << ((i & 2) * 8);
+  for (int i = 0; i < 2; i++) {
+    const float* v = y + 4 * i;
+    if constexpr (E4M3) {
+      w[i] = e4m3_codes(v[0], v[1]) | e4m3_codes(v[2], v[3]) << 16;
+    } else {  // 1.5 * 2^23 + y, rounded to nearest even, has the code in its low byte
+      uint32_t u[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) u[c] = __float_as_uint(__fadd_rn(v[c], 12582912.0f));
+      w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
     }
+    if (dead) w[i] = 0u;
   }
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void decode8(const uint2& w, int e4m3, float (&x)[8]) {
+template <bool E4M3>
+__device__ __forceinline__ void decode8(const uint2& w, float (&x)[8]) {
+  float lo[4], hi[4];
+  kv_values4<E4M3>(w.x, lo);
+  kv_values4<E4M3>(w.y, hi);
 #pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = kv_value(((i < 4 ? w.x : w.y) >> ((i & 3) * 8)) & 0xffu, e4m3);
+  for (int i = 0; i < 4; i++) {
+    x[i] = lo[i];
+    x[4 + i] = hi[i];
+  }
+}
+// max(a, |b|), NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  return d;
 }
 
 // The scale of a largest magnitude given by its bits (infinities and NaN are the largest patterns).
-__device__ __forceinline__ float scale_of(uint32_t bits, int e4m3) {
+template <bool E4M3>
+__device__ __forceinline__ float scale_of(uint32_t bits) {
   if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  if (!e4m3) return fmaxf(__uint_as_float(bits) / 127.0f, SCALE_FLOOR);
+  if constexpr (!E4M3) return fmaxf(__uint_as_float(bits) / 127.0f, SCALE_FLOOR);
   // amax = 1.m * 2^e <= 448 * 2^k = 1.75 * 2^(8 + k); a subnormal amax is far below the floor
   const int e = (int)(bits >> 23) - 127;
   const int k = max(e - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -60);
@@ -132,7 +147,7 @@ __device__ __forceinline__ Span span_of(const KvPool& pool, const KvBatch& batch
 }
 
 // E values of a page and head, E / 32 threads; heads blockIdx.y, blockIdx.y + gridDim.y, ...
-template <int E, bool F32>
+template <int E, bool E4M3, bool F32>
 __global__ void __launch_bounds__(E / PER_THREAD, E == 16384 ? 1 : (F32 ? 512 : 768) * PER_THREAD / E)
 kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
   constexpr int THREADS = E / PER_THREAD;
@@ -162,7 +177,7 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
     const float* mean = !is_v && pool.k_mean ? pool.k_mean + h * pool.D : nullptr;
     const float s0 = next_s0;
     float x[VECS][8];
-    uint32_t top = 0;
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
       const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
@@ -174,11 +189,11 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
           x[i][4] -= b.x; x[i][5] -= b.y; x[i][6] -= b.z; x[i][7] -= b.w;
         }
 #pragma unroll
-        for (int c = 0; c < 8; c++) top = max(top, __float_as_uint(x[i][c]) & 0x7fffffffu);
+        for (int c = 0; c < 8; c++) most = max_abs_nan(most, x[i][c]);
       }
     }
     fetch(h + gridDim.y);
-    top = __reduce_max_sync(0xffffffffu, top);
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // (infinities and NaN are the largest patterns)
     if constexpr (THREADS > 32) {
       if ((threadIdx.x & 31) == 0) tops[n][threadIdx.x >> 5] = top;
       __syncthreads();  // (the other half of tops is written before the next one: no second barrier)
@@ -188,7 +203,7 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
       __syncwarp();
     }
     uint8_t* codes = page_codes + (long long)h * E;
-    float s = scale_of(top, pool.e4m3);
+    float s = scale_of<E4M3>(top);
     if (span.t0 > 0 && !(s > s0) && s == s) s = s0;  // (a NaN on either side stays)
     const bool dead = s != s;
     const float inverse = 1.0f / s;
@@ -198,25 +213,25 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
       if (t >= span.t0 && t < span.t1) {
         float y[8];
 #pragma unroll
-        for (int c = 0; c < 8; c++) y[c] = x[i][c] * inverse;
-        *(uint2*)(codes + e) = encode8(y, pool.e4m3, dead);
+        for (int c = 0; c < 8; c++) y[c] = __fmul_rn(x[i][c], inverse);
+        *(uint2*)(codes + e) = encode8<E4M3>(y, dead);
       }
     }
     if (span.t0 > 0 && s > s0) {  // the scale has grown: the earlier codes move to it
       const float ratio = s0 / s;
       for (int e = threadIdx.x * 8; e < (span.t0 << d_log2); e += THREADS * 8) {
         float y[8];
-        decode8(*(const uint2*)(codes + e), pool.e4m3, y);
+        decode8<E4M3>(*(const uint2*)(codes + e), y);
 #pragma unroll
-        for (int c = 0; c < 8; c++) y[c] *= ratio;
-        *(uint2*)(codes + e) = encode8(y, pool.e4m3, false);
+        for (int c = 0; c < 8; c++) y[c] = __fmul_rn(y[c], ratio);
+        *(uint2*)(codes + e) = encode8<E4M3>(y, false);
       }
     }
     if (threadIdx.x == 0) scales[h] = s;
   }
 }
 
-template <int E, bool F32>
+template <int E, bool E4M3, bool F32>
 __global__ void __launch_bounds__(E / PER_THREAD)
 kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
   constexpr int THREADS = E / PER_THREAD;
@@ -259,7 +274,7 @@ kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const Kv
       const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
       if (t >= span.t0 && t < span.t1) {
         float x[8];
-        decode8(now[i], pool.e4m3, x);
+        decode8<E4M3>(now[i], x);
 #pragma unroll
         for (int c = 0; c < 8; c++) x[c] = span.page < 0 ? 0.f : x[c] * s;
         if (mean) {
@@ -275,13 +290,13 @@ kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const Kv
 // CTAs up to which every head of a page gets one of its own: 16 per SM.
 constexpr int SPREAD_CTAS = 16 * 148;
 
-template <bool WRITE, bool F32>
+template <bool WRITE, bool E4M3, bool F32>
 cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, const KvRows& v, cudaStream_t stream) {
-  const long long places = kv_places(batch.B, batch.T, 1, pool.page_log2, 2);
+  const long long places = kv_places(batch, 1, pool.page_log2, 2);
   const long long per_cta = std::max(1ll, std::min((long long)pool.Hkv, places * pool.Hkv * 2 / SPREAD_CTAS));  // heads
   const dim3 grid((unsigned)places, (unsigned)((pool.Hkv + per_cta - 1) / per_cta), 2);
   auto go = [&](auto kern, int E) { return launch_early(kern, grid, dim3(E / PER_THREAD), 0, stream, pool, batch, k, v); };
-#define AR_KV_E(E) (WRITE ? go(kv_append_kernel<E, F32>, E) : go(kv_read_kernel<E, F32>, E))
+#define AR_KV_E(E) (WRITE ? go(kv_append_kernel<E, E4M3, F32>, E) : go(kv_read_kernel<E, E4M3, F32>, E))
   switch (pool.D << pool.page_log2) {
     case 1024: return AR_KV_E(1024);
     case 2048: return AR_KV_E(2048);
@@ -293,15 +308,22 @@ cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, co
   return cudaErrorInvalidValue;
 }
 
+template <bool WRITE>
+cudaError_t launch_any(const KvPool& pool, const KvBatch& batch, int dtype, const KvRows& k, const KvRows& v, cudaStream_t stream) {
+  const bool f32 = dtype == 0;
+  if (pool.e4m3) return f32 ? launch<WRITE, true, true>(pool, batch, k, v, stream) : launch<WRITE, true, false>(pool, batch, k, v, stream);
+  return f32 ? launch<WRITE, false, true>(pool, batch, k, v, stream) : launch<WRITE, false, false>(pool, batch, k, v, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_kv_append(const KvPool& pool, const KvBatch& batch, int dtype, const KvRows& k, const KvRows& v,
                              cudaStream_t stream) {
-  return dtype == 0 ? launch<true, true>(pool, batch, k, v, stream) : launch<true, false>(pool, batch, k, v, stream);
+  return launch_any<true>(pool, batch, dtype, k, v, stream);
 }
 cudaError_t launch_kv_read(const KvPool& pool, const KvBatch& batch, int dtype, const KvRows& k, const KvRows& v,
                            cudaStream_t stream) {
-  return dtype == 0 ? launch<false, true>(pool, batch, k, v, stream) : launch<false, false>(pool, batch, k, v, stream);
+  return launch_any<false>(pool, batch, dtype, k, v, stream);
 }
 
 }  // namespace ar

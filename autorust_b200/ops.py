@@ -365,7 +365,7 @@ def add_layernorm(x: torch.Tensor, residual: torch.Tensor | None, gamma: torch.T
     return (s_out if s_out is not None else x), y
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KvCache:
     """The pool of an 8-bit key/value cache (ar_kv_pool): k, v [pages, Hkv, page, D] codes -- int8, or uint8 tensors of E4M3
     bit patterns -- and k_scale, v_scale [pages, Hkv] float32, one scale for each page of tokens and kv head.  k_mean
@@ -388,16 +388,17 @@ class KvCache:
         _check_dense("v_scale", self.v_scale, k.shape[:2], torch.float32, k.device)
         if self.k_mean is not None:
             _check_dense("k_mean", self.k_mean, (k.shape[1], k.shape[3]), torch.float32, k.device)
+        # what every call passes on; the fields cannot be replaced, so it stays what it is
+        pages, Hkv, page, D = k.shape
+        pool = _abi.KvPool(k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                           None if self.k_mean is None else self.k_mean.data_ptr(), pages, Hkv, D, page,
+                           _abi.KV_E4M3 if self.fp8 else _abi.KV_INT8)
+        object.__setattr__(self, "_pool", pool)
+        object.__setattr__(self, "_device", k.device)
 
     @property
     def fp8(self) -> bool:
         return self.k.dtype == torch.uint8
-
-    def _pool(self) -> _abi.KvPool:
-        pages, Hkv, page, D = self.k.shape
-        return _abi.KvPool(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                           None if self.k_mean is None else self.k_mean.data_ptr(), pages, Hkv, D, page,
-                           _abi.KV_E4M3 if self.fp8 else _abi.KV_INT8)
 
 
 def kv_cache(pages: int, kv_heads: int, page: int, D: int, fp8: bool = False, k_mean: torch.Tensor | None = None,
@@ -410,24 +411,42 @@ def kv_cache(pages: int, kv_heads: int, page: int, D: int, fp8: bool = False, k_
 
 
 def _kv_batch(cache: KvCache, page_table, lengths, starts, tokens: int) -> _abi.KvBatch:
-    dev = cache.k.device
+    dev = cache._device
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev or page_table.stride(1) != 1:
         raise ValueError("page_table must be a [B, pages] int32 tensor on the cache's device with contiguous rows")
-    B = page_table.shape[0]
-    _check_dense("lengths", lengths, (B,), torch.int32, dev)
+    B, width = page_table.shape
+    if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != dev or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be a contiguous int32 tensor of shape ({B},) on {dev}")
     if starts is not None:
-        _check_dense("starts", starts, (B + 1,), torch.int32, dev)
+        if starts.shape != (B + 1,) or starts.dtype != torch.int32 or starts.device != dev or not starts.is_contiguous():
+            raise ValueError(f"starts must be a contiguous int32 tensor of shape ({B + 1},) on {dev}")
     elif tokens != B:
         raise ValueError(f"without starts every sequence has one token: {tokens} tokens for {B} sequences")
     return _abi.KvBatch(page_table.data_ptr(), lengths.data_ptr(), None if starts is None else starts.data_ptr(),
-                        page_table.stride(0), page_table.shape[1], B, tokens)
+                        page_table.stride(0), width, B, tokens)
+
+
+_Strides2 = ctypes.c_int64 * 2
 
 
 def _kv_rows(name: str, t: torch.Tensor, shape, dtype, device):
     """Strides of a packed [T, H, D] view."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or t.stride(2) != 1:
+    if t.shape != shape or t.dtype != dtype or t.device != device or t.stride(2) != 1:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device} with a contiguous last dimension")
-    return (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+    return _Strides2(t.stride(0), t.stride(1))
+
+
+def _kv_call(what: str, fn, cache: KvCache, stream, *args) -> None:
+    """The call on `stream` (None: the current one of the cache's device), with that device current."""
+    dev = cache._device
+    handle = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(cache._pool, *args, handle)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(cache._pool, *args, handle)
+    if rc != _abi.AR_OK:
+        _abi.check(rc, what)
 
 
 def kv_cache_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -435,17 +454,15 @@ def kv_cache_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, page_table
     """Quantises the call's new tokens into the cache (ar_kv_cache_append).  k, v [T, Hkv, D], float32 or bfloat16 views with
     a contiguous last dimension; sequence b's tokens are the rows starts[b] .. starts[b + 1] (None: one each) and become
     its last ones -- lengths counts them in.  Token t lies on page page_table[b, t // page]."""
-    L = _abi.load()
     if k.dim() != 3:
         raise ValueError("k and v must be [T, Hkv, D]")
-    shape, dtype = (k.shape[0], cache.k.shape[1], cache.k.shape[3]), _dtype_code(k)
-    ks = _kv_rows("k", k, shape, k.dtype, cache.k.device)
-    vs = _kv_rows("v", v, shape, k.dtype, cache.k.device)
-    batch, pool = _kv_batch(cache, page_table, lengths, starts, k.shape[0]), cache._pool()
-    with torch.cuda.device(cache.k.device):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        rc = L.ar_kv_cache_append(pool, batch, dtype, k.data_ptr(), ks, v.data_ptr(), vs, s.cuda_stream)
-    _abi.check(rc, "ar_kv_cache_append")
+    pool, dev = cache._pool, cache._device
+    T = k.shape[0]
+    shape, code = (T, pool.Hkv, pool.D), _dtype_code(k)
+    ks = _kv_rows("k", k, shape, k.dtype, dev)
+    vs = _kv_rows("v", v, shape, k.dtype, dev)
+    batch = _kv_batch(cache, page_table, lengths, starts, T)
+    _kv_call("ar_kv_cache_append", _abi.load().ar_kv_cache_append, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
 
 
 def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None, tokens: int,
@@ -453,16 +470,16 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     """The last starts[b + 1] - starts[b] tokens of every sequence as the values the codes stand for (ar_kv_cache_read):
     (k, v) [tokens, Hkv, D] of `dtype`.  With starts = running sums of lengths that is everything.  out: (k, v) to write into,
     views with a contiguous last dimension; rows that belong to no sequence are left as they were."""
-    L = _abi.load()
-    shape, dev = (int(tokens), cache.k.shape[1], cache.k.shape[3]), cache.k.device
-    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    pool, dev, tokens = cache._pool, cache._device, int(tokens)
+    shape = (tokens, pool.Hkv, pool.D)
+    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
     code = _dtype_code(k)
     ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
-    batch, pool = _kv_batch(cache, page_table, lengths, starts, int(tokens)), cache._pool()
-    with torch.cuda.device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        rc = L.ar_kv_cache_read(pool, batch, code, k.data_ptr(), ks, v.data_ptr(), vs, s.cuda_stream)
-    _abi.check(rc, "ar_kv_cache_read")
+    batch = _kv_batch(cache, page_table, lengths, starts, tokens)
+    _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
+    if stream is not None and out is None:
+        k.record_stream(stream)
+        v.record_stream(stream)
     return k, v
 
 
@@ -477,35 +494,46 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     L = _abi.load()
     if q.dim() != 3:
         raise ValueError("q must be [T, Hq, D]")
+    pool, dev = cache._pool, cache._device
     T, Hq, D = q.shape
-    dev, code = cache.k.device, _dtype_code(q)
-    qs = _kv_rows("q", q, (T, Hq, cache.k.shape[3]), q.dtype, dev)
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    os = _kv_rows("out", out, (T, Hq, D), q.dtype, dev)
-    batch, pool = _kv_batch(cache, page_table, lengths, starts, T), cache._pool()
-    bound = page_table.shape[1] * cache.k.shape[2] if max_length is None else int(max_length)
-    need = int(L.ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, bound, int(causal)))
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    have = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    with torch.cuda.device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        rc = L.ar_kv_cache_attention(pool, batch, code, q.data_ptr(), qs, out.data_ptr(), os, Hq, bound, int(causal),
-                                     workspace.data_ptr() if have else None, have, s.cuda_stream)
-    _abi.check(rc, "ar_kv_cache_attention")
-    if workspace is not None:
-        workspace.record_stream(s)
+    code, causal = _dtype_code(q), int(causal)
+    shape = (T, Hq, pool.D)
+    qs = _kv_rows("q", q, shape, q.dtype, dev)
+    fresh = out is None
+    if fresh:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    os = _kv_rows("out", out, shape, q.dtype, dev)
+    batch = _kv_batch(cache, page_table, lengths, starts, T)
+    bound = batch.table_pages * pool.page if max_length is None else int(max_length)
+    have = 0
+    if workspace is None:
+        have = L.ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, bound, causal)
+        if have:
+            workspace = torch.empty(have, dtype=torch.uint8, device=dev)
+    else:
+        have = workspace.numel() * workspace.element_size()
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous tensor on the cache's device")
+    _kv_call("ar_kv_cache_attention", L.ar_kv_cache_attention, cache, stream, batch, code, q.data_ptr(), qs, out.data_ptr(), os, Hq,
+             bound, causal, workspace.data_ptr() if have else None, have)
+    if stream is not None:  # what another stream than the allocating one uses stays until it has done so
+        if workspace is not None:
+            workspace.record_stream(stream)
+        if fresh:
+            out.record_stream(stream)
     return out
 
 
 def kv_cache_attention_workspace(cache: KvCache, tokens: int, Hq: int, sequences: int, max_length: int,
                                  dtype: torch.dtype = torch.bfloat16, causal: bool = True) -> int:
-    """Bytes of scratch that kv_cache_attention needs for these sizes."""
-    # (the addresses are placeholders: the size depends on the extents only)
-    batch = _abi.KvBatch(16, 16, 16, max_length, max(1, -(-max_length // cache.k.shape[2])), sequences, tokens)
+    """Bytes of scratch that kv_cache_attention needs for these sizes, with starts or (one token each) without."""
+    width = max(1, -(-max_length // cache._pool.page))
     code = _abi.DTYPE_F32 if dtype == torch.float32 else _abi.DTYPE_BF16
-    return int(_abi.load().ar_kv_cache_attention_workspace_bytes(cache._pool(), batch, code, Hq, max_length, int(causal)))
+    need = 0
+    for starts in ([16, None] if tokens == sequences else [16]):
+        batch = _abi.KvBatch(16, 16, starts, width, width, sequences, tokens)  # (placeholders: the sizes decide)
+        need = max(need, _abi.load().ar_kv_cache_attention_workspace_bytes(cache._pool, batch, code, Hq, max_length, int(causal)))
+    return need
 
 
 def last_status(workspace: torch.Tensor | None = None) -> int:
