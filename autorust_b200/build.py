@@ -21,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -36,7 +37,7 @@ NVCC_FLAGS = [
 ]
 
 KERNEL_SOURCES = ["attn_fwd_tc.cu", "attn_fwd_short.cu", "attn_fwd_exact.cu", "attn_train.cu", "attn_train_tc.cu", "sage_prologue.cu", "api.cu",
-                  "sage_static.cu", "encoder_norm.cu", "kv_cache.cu", "kv_cache_write.cu", "kv_cache_attn.cu"]
+                  "sage_static.cu", "encoder_norm.cu", "kv_cache.cu", "kv_cache_write.cu", "kv_cache_attn.cu", "kv_cache_attn_tc.cu"]
 
 
 def _nvcc() -> str:
@@ -60,6 +61,11 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError("build step failed: " + " ".join(cmd))
 
 
+def _run_all(cmds: list[list[str]]) -> None:
+    with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
+        list(pool.map(_run, cmds))
+
+
 def _headers() -> list[Path]:
     return sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h")) + \
         sorted((CSRC / "host").glob("*.h"))
@@ -71,19 +77,16 @@ def build_kernels(force: bool = False) -> Path:
     srcs = [CSRC / s for s in KERNEL_SOURCES]
     if not force and not _newer(out, srcs + _headers()):
         return out
-    objs = []
-    for s in srcs:
-        o = LIB / (s.stem + ".o")
-        if force or _newer(o, [s] + _headers()):
-            _run([_nvcc(), *NVCC_FLAGS, "-c", str(s), "-o", str(o)])
-        objs.append(str(o))
-    _run([_nvcc(), "-shared", "-o", str(out), *objs, "-gencode", "arch=compute_100a,code=sm_100a"])
+    objs = [LIB / (s.stem + ".o") for s in srcs]
+    _run_all([[_nvcc(), *NVCC_FLAGS, "-c", str(s), "-o", str(o)] for s, o in zip(srcs, objs)
+              if force or _newer(o, [s] + _headers())])
+    _run([_nvcc(), "-shared", "-o", str(out), *map(str, objs), "-gencode", "arch=compute_100a,code=sm_100a"])
     return out
 
 
 # Sources whose device code contains bounded waits (api.cu: the test's hold on their tickets): rebuilt with the short budget
 # for the wait-expiry test library.
-WAIT_SOURCES = ["attn_fwd_tc.cu", "attn_fwd_short.cu", "attn_train_tc.cu", "sage_prologue.cu", "api.cu"]
+WAIT_SOURCES = ["attn_fwd_tc.cu", "attn_fwd_short.cu", "attn_train_tc.cu", "sage_prologue.cu", "api.cu", "kv_cache_attn_tc.cu"]
 WAIT_TEST_FLAGS = ["-DAR_WAIT_TEST", "-DAR_WAIT_BUDGET_CYCLES=2000000ll"]
 
 
@@ -96,16 +99,10 @@ def build_wait_test(force: bool = False) -> Path:
     srcs = [CSRC / s for s in KERNEL_SOURCES]
     if not force and not _newer(out, srcs + _headers()):
         return out
-    objs = []
-    for s in srcs:
-        if s.name in WAIT_SOURCES:
-            o = out_dir / (s.stem + ".o")
-            if force or _newer(o, [s] + _headers()):
-                _run([_nvcc(), *NVCC_FLAGS, *WAIT_TEST_FLAGS, "-c", str(s), "-o", str(o)])
-        else:
-            o = LIB / (s.stem + ".o")
-        objs.append(str(o))
-    _run([_nvcc(), "-shared", "-o", str(out), *objs, "-gencode", "arch=compute_100a,code=sm_100a"])
+    objs = [(out_dir if s.name in WAIT_SOURCES else LIB) / (s.stem + ".o") for s in srcs]
+    _run_all([[_nvcc(), *NVCC_FLAGS, *WAIT_TEST_FLAGS, "-c", str(s), "-o", str(o)] for s, o in zip(srcs, objs)
+              if s.name in WAIT_SOURCES and (force or _newer(o, [s] + _headers()))])
+    _run([_nvcc(), "-shared", "-o", str(out), *map(str, objs), "-gencode", "arch=compute_100a,code=sm_100a"])
     return out
 
 

@@ -93,15 +93,17 @@ uint32_t* status_ptr(void* workspace) {
 // The library's word is not: the launch gets a ticket instead, which saves the stream a memset of its own in front of a
 // kernel of 20 microseconds.  A captured call would replay its ticket, so that one clears the word as well.
 std::atomic<uint32_t> g_next_ticket{0};
-bool prepare_status(ar::TcArgs& a, bool callers_word, cudaStream_t stream) {
-  if (!callers_word) {
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) return false;
-    if (capture == cudaStreamCaptureStatusNone) {
-      a.ticket = (g_next_ticket.fetch_add(1) & 0x3fffffffu) + 1u;  // 1 .. 2^30: never 0, never the bit an OR-ed status carries
-      return true;
-    }
+bool take_ticket(uint32_t* status, cudaStream_t stream, uint32_t* ticket) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) return false;
+  if (capture == cudaStreamCaptureStatusNone) {
+    *ticket = (g_next_ticket.fetch_add(1) & 0x3fffffffu) + 1u;  // 1 .. 2^30: never 0, never the bit an OR-ed status carries
+    return true;
   }
+  return cudaMemsetAsync(status, 0, sizeof(uint32_t), stream) == cudaSuccess;
+}
+bool prepare_status(ar::TcArgs& a, bool callers_word, cudaStream_t stream) {
+  if (!callers_word) return take_ticket(a.status, stream, &a.ticket);
   return cudaMemsetAsync(a.status, 0, sizeof(uint32_t), stream) == cudaSuccess;
 }
 uint32_t* sticky_ptr() {
@@ -131,6 +133,12 @@ bool replicas_ok(void* const* replicas, int n, ar::OutReplicas* out) {
 }  // namespace
 
 namespace ar {
+bool launch_ticket(cudaStream_t stream, uint32_t** status, uint32_t* ticket) {
+  *status = library_words();
+  *ticket = 0;
+  return *status && take_ticket(*status, stream, ticket);
+}
+
 bool library_status_words(uint32_t** launch_word, uint32_t** sticky_word) {
   uint32_t* p = library_words();
   if (!p) return false;

@@ -81,6 +81,9 @@ bool attn_tc_has(int mode, int D);
 bool device_ok();
 // Lets other translation units of the library feed the launch counters.
 void count_launches(int mode, int kernels);
+// The library's launch word for a launch with bounded waits that brings no workspace, marked with a ticket of its own, or
+// (in a captured call, whose replays would repeat it) cleared on the stream and without one.
+bool launch_ticket(cudaStream_t stream, uint32_t** status, uint32_t* ticket);
 bool library_status_words(uint32_t** launch_word, uint32_t** sticky_word);
 
 // Layout of the Sage workspace (offsets in bytes from its start; every section 256-byte aligned, the first 256 bytes
@@ -178,13 +181,15 @@ struct KvAttnArgs {
   int dtype, Hq, max_length, causal;
   float* partial;  // workspace; null where the plan needs none
 };
-// How a call is divided: row tiles of `rows` rows, over `ctas` CTAs that take equal shares of all keys (0: one CTA per tile).
+// How a call is divided: row tiles of `rows` rows, over `ctas` CTAs that take equal shares of all keys (0: one CTA per tile);
+// rows = 256: the tensor-core kernel.
 struct KvAttnPlan {
   int rows, ctas;
   size_t workspace;
 };
 KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal);
 cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches);
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t stream);  // kv_cache_attn_tc.cu: many rows, bf16 tensors
 
 // Sage prologue (sage_prologue.cu).
 struct PrologueArgs {

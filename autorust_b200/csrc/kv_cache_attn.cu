@@ -827,11 +827,16 @@ cudaError_t launch_nt(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t 
 }  // namespace
 
 KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal) {
-  (void)dtype;
   (void)causal;
   KvAttnPlan p;
   const int G = Hq / pool.Hkv;
   p.rows = (long long)batch.T * G <= 8ll * batch.B ? 8 : 16;
+  if (dtype != 0 && (long long)batch.T * G >= 96ll * batch.B) {
+    p.rows = 256;
+    p.ctas = 0;
+    p.workspace = 0;
+    return p;
+  }
   const long long tiles = kv_places(batch, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
   p.ctas = SMS * (p.rows == 8 ? Sh<128, 1>::CTAS_PER_SM : Sh<128, 2>::CTAS_PER_SM);
   if (max_length <= WHOLE_KEYS || tiles >= 16 * p.ctas || tiles * ((max_length + GROUP - 1) / GROUP + START_UNITS) > 0xffffffffll) p.ctas = 0;
@@ -841,6 +846,11 @@ KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches) {
   const bool d128 = a.pool.D == 128, f32 = a.dtype == 0;
+  if (plan.rows == 256) {
+    const cudaError_t e = launch_kv_attention_tc(a, stream);
+    if (e == cudaSuccess) ++*launches;
+    return e;
+  }
   if (a.pool.e4m3) {
     if (d128) return f32 ? launch_nt<128, true, true>(a, plan, stream, launches) : launch_nt<128, true, false>(a, plan, stream, launches);
     return f32 ? launch_nt<64, true, true>(a, plan, stream, launches) : launch_nt<64, true, false>(a, plan, stream, launches);

@@ -1,0 +1,540 @@
+// Attention of many rows over the 8-bit paged cache (chunks of a prompt, whole prompts): the products on the tcgen05 tensor
+// cores.  The same mathematics as kv_cache_attn.cu, bf16 tensors only:
+//
+//   x = (q . kcode) * c_row * s_k + log2(s_v / v_ref),   P = 2^(x - m + 8),   O = sum P vcode,   l = sum P * v_ref / s_v,   o = v_ref O / l
+//
+// The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
+// exponential, and the tensor cores see the codes as f16 (exact) and P and q in f16 (q scaled by a power of two per row:
+// exact but for elements 2^-14 below its largest; P rounded to nearest, the row sum keeps the unrounded values).
+//
+// CTA = 2 tiles of 128 rows (tokens x query heads of the group) of one kv head, 512 threads at 128 registers:
+//   warps 0-3, 4-7  softmax of tile 0 and 1: one thread per row = TMEM lane
+//   warps 8-11      producers: codes from global memory to f16 tiles in shared memory, K and V through rings of 2 tiles of
+//                   128 keys.  A 16-byte piece of codes becomes 32 bytes of a row; rows of 128 bytes in boxes of 64 channels,
+//                   the 16-byte chunk c of row r at c ^ (r & 7), as a swizzled TMA load would leave them: K is read K-major, V MN-major.
+//                   The next tile's codes are in registers while the ring is full.
+//   warp  12        issues the MMAs: S_t = Q_t K_j^T, O_t += P_t V_j in the order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
+//   TMEM (512 columns): S_0, S_1 (P overwrites the first half of its S), O_0, O_1.
+// The softmax reads S twice, 32 columns at a time -- maximum, then exponentials -- which keeps it inside 128 registers, so
+// that the producers need no registers of its.
+//
+// What bounds it: a step of two tiles and 128 keys of D = 128 is 2048 clocks of MMA and as many of MUFU exponentials (a quarter of
+// them is taken by a polynomial on the FMA pipe); the operands' reads from shared memory take 1536 of its clocks, the producers'
+// writes 512.
+#include <cuda_bf16.h>
+
+#include "ar_ptx.cuh"
+#include "kv_cache.cuh"
+#include "softmax_math.cuh"
+
+namespace ar {
+namespace {
+using namespace arptx;
+
+#ifdef AR_WAIT_TEST
+__device__ int g_test_skip_cache_tile = -1;
+#endif
+
+constexpr int BM = 128, BN = 128, TILES = 2, ROWS = BM * TILES;
+constexpr int THREADS = 512, W_PROD = 8, W_MMA = 12;
+constexpr int BLOCKS = BN / 16;  // column blocks of one page at least
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NEG = -1e30f;            // where a row's maximum starts; a hidden key is -inf
+constexpr float P_SHIFT = 8.0f, LAG = 6.0f;  // P < 2^14: inside f16, and a weight 2^-22 of the largest still a normal number
+constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60
+constexpr uint32_t POLY_MASK = 0x8888u;  // of 16 pairs of columns, those whose exponentials are a polynomial's
+
+template <int D>
+struct Cfg {
+  static constexpr int STAGES = 2;
+  static constexpr int BOXES = D / 64;
+  static constexpr int BOX = BN * 128;               // bytes: 128 rows of 64 channels
+  static constexpr int TILE = BN * D * 2;            // of Q, K or V
+  static constexpr int SCALE_RING = 4;               // tiles whose scales are kept
+  static constexpr int NUM_BARS = 2 + 4 * STAGES + 2 + 4 + 2;
+  static constexpr int SCALES = (TILES + 2 * STAGES) * TILE;
+  static constexpr int BARS = SCALES + SCALE_RING * 3 * BLOCKS * 4;
+  static constexpr int BYTES = BARS + NUM_BARS * 8 + 16 + 1024;
+  static_assert(BYTES <= 227 * 1024, "shared memory budget");
+  static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, 0, 0, BM, BN);  // f16 x f16 -> f32
+  static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, 0, 1, BM, D);
+  static constexpr int QK_STEPS = D / 16, PV_STEPS = BN / 16;
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Four codes -> two f16x2.  INT8: the byte code + 128 under the exponent of 1024 is 1152 + code.
+template <bool E4M3>
+__device__ __forceinline__ void expand4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+  }
+}
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
+  using C = Cfg<D>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + TILES * C::TILE;
+  uint8_t* sV = sK + ST * C::TILE;
+  float* scales = (float*)(smem + C::SCALES);  // [slot][s_k | log2(s_v / v_ref) | v_ref / s_v][block]
+  uint64_t* bars = (uint64_t*)(smem + C::BARS);
+  uint64_t* q_full = bars;             // [2]
+  uint64_t* k_full = q_full + 2;       // [ST]
+  uint64_t* k_empty = k_full + ST;
+  uint64_t* v_full = k_empty + ST;
+  uint64_t* v_empty = v_full + ST;
+  uint64_t* s_full = v_empty + ST;     // [2]
+  uint64_t* p_part = s_full + 2;       // [tile][half of the keys]
+  uint64_t* o_full = p_part + 4;       // [2]
+  uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const WaitCtx wctx{abort_flag, status, a.batch.sticky, ticket};
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // whatever came before in the stream is done and visible
+
+  const int tid = threadIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int lane = tid & 31;
+  const int G = a.Hq / a.pool.Hkv, Hkv = a.pool.Hkv, h = blockIdx.y;
+  // the last tiles first: under a causal mask they are the heavy ones
+  const KvPlace p = kv_place(a.batch, (int)(gridDim.x - 1 - blockIdx.x), G, 8, 1);
+  const int all_rows = p.n * G;
+  if (p.tile < 0 || (long long)p.tile * ROWS >= all_rows) return;
+  const int r0 = p.tile * ROWS;
+  const long long cap = min((long long)a.batch.table_pages << a.pool.page_log2, (long long)a.max_length);
+  const int total = (int)min((long long)p.length, cap), pos0 = p.length - p.n;
+  auto limit = [&](int row) { return a.causal ? max(min(total, pos0 + row / G + 1), 0) : total; };
+  if (total < p.length && tid == 0) kv_report(a.batch);
+  int nkv[2], low[2];  // key tiles that some row of a row tile sees; keys that all of them see
+#pragma unroll
+  for (int t = 0; t < TILES; t++) {
+    const int first = r0 + t * BM, last = min(first + BM, all_rows) - 1;
+    nkv[t] = first > last ? 0 : (limit(last) + BN - 1) / BN;
+    low[t] = first > last ? 0 : limit(first);
+  }
+  const int nkv_max = max(nkv[0], nkv[1]);
+  const int end = limit(min(r0 + ROWS, all_rows) - 1);
+  const int log2 = a.pool.page_log2;
+  const int* table = a.batch.page_table + (long long)p.b * a.batch.table_stride;
+  auto page_of = [&](int key) {  // -2: past the end, -1: there is none
+    if (key >= end) return -2;
+    const int pg = table[key >> log2];
+    return pg >= 0 && pg < a.pool.pages ? pg : -1;
+  };
+  auto v_scale_of = [&](int pg) {
+    const float s = a.pool.v_scale[(long long)pg * Hkv + h];
+    return s < SCALE_FLOOR ? SCALE_FLOOR : s;  // (a NaN stays)
+  };
+
+  bool lost = false;
+  if (warp == W_MMA) {
+    if (lane == 0) {
+      lost = launch_lost(status, ticket);
+      *abort_flag = lost ? 1u : 0u;
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&q_full[i], 128);
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_part[2 * i], 128);
+        mbar_init(&p_part[2 * i + 1], 128);
+        mbar_init(&o_full[i], 1);
+      }
+      for (int i = 0; i < ST; i++) {
+        mbar_init(&k_full[i], 128);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], 128);
+        mbar_init(&v_empty[i], 1);
+      }
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = *tmem_slot;
+
+  if (warp >= W_PROD && warp < W_MMA) {
+    // ------------------------------------------------------------ producers
+    const int ptid = tid - W_PROD * 32;
+    constexpr int PIECES = D / 16;            // 16-byte pieces of a key's codes
+    constexpr int PER = BN * PIECES / 128;    // of a tile, per thread
+    // thread -> key ptid / PIECES of every 128 / PIECES keys, piece ptid % PIECES
+    constexpr int KEYS = 128 / PIECES;        // keys of one pass: 16 (D = 128) or 32
+    const int key_t = ptid / PIECES, q = ptid % PIECES;
+    const float v_ref_raw = [&] {
+      const int pg = nkv_max > 0 ? page_of(0) : -1;
+      const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
+      return s == s ? s : 1.0f;
+    }();
+    // page numbers: lane l < 8 of every warp holds that of the tile's l-th block of 16 keys, two tiles ahead
+    auto look = [&](int j) { return lane < BLOCKS ? page_of(j * BN + lane * 16) : -2; };
+    int pages = look(0), pages1 = look(1);
+    uint4 kc[PER], vc[PER];
+    auto load = [&](const uint8_t* codes, uint4(&to)[PER], int j, int pages) {
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int key = j * BN + i * KEYS + key_t;
+        const int pg = __shfl_sync(0xffffffffu, pages, (i * KEYS + key_t) >> 4);
+        to[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the end and without a page: codes of value 0
+        if (pg >= 0 && key < end)
+          to[i] = *(const uint4*)(codes + ((((long long)pg * Hkv + h) << log2) + (key & ((1 << log2) - 1))) * D + q * 16);
+      }
+    };
+    // one tile of f16 from the codes in registers
+    auto store = [&](uint8_t* tile, const uint4(&codes)[PER]) {
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int r = i * KEYS + key_t;
+        uint4 x, y;
+        expand4<E4M3>(codes[i].x, x.x, x.y);
+        expand4<E4M3>(codes[i].y, x.z, x.w);
+        expand4<E4M3>(codes[i].z, y.x, y.y);
+        expand4<E4M3>(codes[i].w, y.z, y.w);
+        // chunks 2 * (q & 3) and the next one of box q >> 2; the second box's pieces are written in the other order, so that
+        // the 8 lanes of a row write 8 different chunk places at a time
+        uint8_t* row = tile + (q >> 2) * C::BOX + r * 128;
+        const int c0 = (q & 3) * 2, flip = (q >> 2) & 1;
+        *(uint4*)(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? y : x;
+        *(uint4*)(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? x : y;
+      }
+    };
+    if (nkv_max > 0) {
+      load(a.pool.k, kc, 0, pages);
+      load(a.pool.v, vc, 0, pages);
+    }
+    bool ok = !*abort_flag;
+    for (int j = 0; j < nkv_max && ok; j++) {
+      const int s = j % ST, n = j / ST;
+      const int now = pages;
+      pages = pages1;
+      pages1 = look(j + 2);
+#ifdef AR_WAIT_TEST
+      // Test build only: one tile is never delivered, so that the wait for it runs out.
+      if (j == g_test_skip_cache_tile) break;
+#endif
+      if (n > 0) ok = mbar_wait(&k_empty[s], (n - 1) & 1, wctx, 0x50);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      store(sK + s * C::TILE, kc);
+      if (j + 1 < nkv_max) load(a.pool.k, kc, j + 1, pages);
+      if (ptid < BLOCKS) {  // (lanes 0 .. 7 of the first producer warp, which hold the pages of their blocks)
+        float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS + ptid;
+        float sk = 0.f, lv = -INFINITY, wv = 0.f;  // nothing there: every logit -inf, every weight 0
+        if (now >= 0) {
+          sk = a.pool.k_scale[(long long)now * Hkv + h];
+          const float vs = v_scale_of(now);
+          lv = log2f(vs) - log2f(v_ref_raw);
+          wv = vs == vs ? v_ref_raw / vs : 1.0f;
+        } else if (now == -1) {
+          kv_report(a.batch);
+        }
+        slot[0] = sk;
+        slot[BLOCKS] = lv;
+        slot[2 * BLOCKS] = wv;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&k_full[s]);
+      if (n > 0) ok = mbar_wait(&v_empty[s], (n - 1) & 1, wctx, 0x51);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      store(sV + s * C::TILE, vc);
+      if (j + 1 < nkv_max) load(a.pool.v, vc, j + 1, pages);
+      fence_proxy_async_smem();
+      mbar_arrive(&v_full[s]);
+    }
+  } else if (warp == W_MMA) {
+    // ------------------------------------------------------------ MMA issuer (converged; one elected lane issues)
+    const uint64_t k_proto = make_sdesc_sw128(0, 16, 1024), v_proto = make_sdesc_sw128(0, C::BOX, 1024);
+    const uint32_t k_hi = (uint32_t)(k_proto >> 32), v_hi = (uint32_t)(v_proto >> 32);
+    const uint32_t q_lo0 = (uint32_t)k_proto | (smem_u32(sQ) >> 4);
+    const uint32_t k_lo0 = (uint32_t)k_proto | (smem_u32(sK) >> 4);
+    const uint32_t v_lo0 = (uint32_t)v_proto | (smem_u32(sV) >> 4);
+    auto issue_qk = [&](int t, int s) {
+      const uint32_t qa = q_lo0 + t * (C::TILE >> 4), ka = k_lo0 + s * (C::TILE >> 4);
+      if (!elect_one()) return;
+#pragma unroll
+      for (int i = 0; i < C::QK_STEPS; i++) {  // 16 channels = 32 bytes of a row, four to a box
+        const uint32_t off = ((i >> 2) * C::BOX + (i & 3) * 32) >> 4;
+        mma_ss_lohi<KIND_F16>(tb + t * 128, qa + off, k_hi, ka + off, k_hi, C::IDESC_QK, i > 0);
+      }
+    };
+    auto issue_pv = [&](int t, int s, bool acc, int half) {
+      const uint32_t d = tb + 256 + t * 128, pa = tb + t * 128, va = v_lo0 + s * (C::TILE >> 4);
+      if (!elect_one()) return;
+#pragma unroll
+      for (int i2 = 0; i2 < C::PV_STEPS / 2; i2++) {  // 16 keys = 2048 bytes of each box
+        const int i = half * (C::PV_STEPS / 2) + i2;
+        mma_ts_lohi<KIND_F16>(d, pa + i * 8, va + i * (2048 >> 4), v_hi, C::IDESC_PV, (acc || i > 0) ? 1u : 0u);
+      }
+    };
+    bool ok = true;
+    if (nkv_max > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_full[0], 0, wctx, 0x52));
+    for (int t = 0; t < TILES && ok; t++) {
+      if (nkv[t] == 0) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[t], 0, wctx, 0x53));
+      if (!ok) break;
+      tc_fence_after();
+      issue_qk(t, 0);
+      commit_one(&s_full[t]);
+    }
+    if (ok && nkv_max > 0) commit_one(&k_empty[0]);
+    for (int j = 0; j < nkv_max && ok; j++) {
+      const int s = j % ST, s1 = (j + 1) % ST;
+      ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], (j / ST) & 1, wctx, 0x54));
+      if (!ok) break;
+      if (j + 1 < nkv_max) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_full[s1], ((j + 1) / ST) & 1, wctx, 0x55));
+        if (!ok) break;
+      }
+      for (int t = 0; t < TILES && ok; t++) {
+        if (j >= nkv[t]) continue;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&p_part[2 * t + half], j & 1, wctx, 0x56));
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, s, j > 0, half);
+        }
+        if (!ok) break;
+        if (j + 1 < nkv[t]) {
+          issue_qk(t, s1);
+          commit_one(&s_full[t]);
+        } else {
+          commit_one(&o_full[t]);
+        }
+      }
+      if (!ok) break;
+      commit_one(&v_empty[s]);
+      if (j + 1 < nkv_max) commit_one(&k_empty[s1]);
+    }
+  } else if (warp < W_PROD) {
+    // ------------------------------------------------------------ softmax: thread = row
+    const int t = warp >> 2, r = tid & 127, row = r0 + t * BM + r;
+    const bool in = row < all_rows;
+    const int token = in ? row / G : 0;
+    const int lim = in ? limit(row) : 0;
+    const uint32_t lane_base = (uint32_t)(warp & 3) * 32;
+    const uint32_t tS = tmem_addr(tb, lane_base, t * 128), tO = tmem_addr(tb, lane_base, 256 + t * 128);
+    const int head = h * G + (in ? row - token * G : 0);
+
+    // Q: the row times 2^-e, its largest element below 2
+    float c_row = 0.f;
+    if (nkv[t] > 0) {
+      const uint4* src = (const uint4*)((const __nv_bfloat16*)a.q.p + (p.row0 + (long long)token) * a.q.st + (long long)head * a.q.sh);
+      uint4 w[D / 8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; i++) {
+        w[i] = in ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int x = 0; x < 4; x++) top = max(top, max(u[x] << 16 & 0x7fffffffu, u[x] & 0x7fff0000u));
+      }
+      const int e = min(max((int)(top >> 23) - 127, -100), 126);
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      c_row = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      uint8_t* dst = sQ + t * C::TILE + r * 128;
+#pragma unroll
+      for (int i = 0; i < D / 8; i++) {
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t v[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) v[x] = pack_half2(__uint_as_float(u[x] << 16) * down, __uint_as_float(u[x] & 0xffff0000u) * down);
+        *(uint4*)(dst + (i >> 3) * C::BOX + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full[t]);
+    }
+    float m = NEG, l = 0.f;
+
+    // One step: S of 128 keys -> P.  EDGE: keys from first_out on are not the row's.
+    auto step = [&](auto edge_c, int j) {
+      constexpr bool EDGE = decltype(edge_c)::value;
+      const float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS;
+      const int first_out = lim - j * BN;
+      // maximum
+      float mc = -INFINITY;
+      uint32_t sv[32];
+#pragma unroll
+      for (int qd = 0; qd < 4; qd++) {
+        tmem_ld32(tS + qd * 32, sv);
+        tmem_wait_ld();
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int col = qd * 32 + b * 16 + i + k;
+              x[k] = __uint_as_float(sv[b * 16 + i + k]);
+              if (EDGE && col >= first_out) x[k] = -INFINITY;
+            }
+            top[0] = fmax3(top[0], x[0], x[1]);
+            top[1] = fmax3(top[1], x[2], x[3]);
+          }
+          // (a block without a page: s_k = 0 and log2 -inf, and 0 * -inf above is NaN, which the maximum passes over)
+          mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c_row * slot[qd * 2 + b], slot[BLOCKS + qd * 2 + b]));
+        }
+      }
+      const bool need = mc > m + LAG;
+      if (__any_sync(0xffffffffu, need)) {
+        const float m_new = need ? mc : m;
+        const float alpha = ex2f(m - m_new);
+        m = m_new;
+        l *= alpha;
+        if (j > 0) {  // S(j) has arrived, so PV(j-1) is complete and O may be scaled in place
+          const uint64_t alpha2 = pack_f32x2(alpha, alpha);
+#pragma unroll 1
+          for (int cch = 0; cch < D / 32; cch++) {
+            tmem_ld32(tO + cch * 32, sv);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x, y;
+              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), alpha2), x, y);
+              sv[i] = __float_as_uint(x);
+              sv[i + 1] = __float_as_uint(y);
+            }
+            tmem_st32(tO + cch * 32, sv);
+          }
+        }
+      }
+      // exponentials
+      const float ref = m - P_SHIFT;
+#pragma unroll
+      for (int qd = 0; qd < 4; qd++) {
+        tmem_ld32(tS + qd * 32, sv);
+        tmem_wait_ld();
+        uint32_t pk[16];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const float c = c_row * slot[qd * 2 + b], add = slot[BLOCKS + qd * 2 + b] - ref;
+          const uint64_t c2 = pack_f32x2(c, c), add2 = pack_f32x2(add, add);
+          uint64_t sum = pack_f32x2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int at = b * 16 + 2 * i;
+            uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2);
+            float p0, p1;
+            if constexpr (EDGE) {
+              float x, y;
+              unpack_f32x2(x2, x, y);
+              p0 = qd * 32 + at >= first_out ? 0.f : ex2f(x);
+              p1 = qd * 32 + at + 1 >= first_out ? 0.f : ex2f(y);
+            } else if ((POLY_MASK >> (b * 8 + i)) & 1u) {
+              exp2_poly_x2(x2, p0, p1);
+            } else {
+              exp2_mufu_x2(x2, p0, p1);
+            }
+            sum = add_f32x2(sum, pack_f32x2(p0, p1));
+            pk[b * 8 + i] = pack_half2(p0, p1);
+          }
+          float s0, s1;
+          unpack_f32x2(sum, s0, s1);
+          l = fmaf(s0 + s1, slot[2 * BLOCKS + qd * 2 + b], l);
+        }
+        if (qd == 2) {  // the first half of P has landed: its products run under the rest
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&p_part[2 * t]);
+        }
+        tmem_st16(tS + qd * 16, pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_part[2 * t + 1]);
+    };
+
+    bool ok = true;
+    for (int j = 0; j < nkv[t]; j++) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, wctx, 0x57));
+      if (!ok) break;
+      tc_fence_after();
+      if (j * BN + BN > low[t])
+        step(std::true_type{}, j);
+      else
+        step(std::false_type{}, j);
+    }
+    if (ok && nkv[t] > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, wctx, 0x58));
+      tc_fence_after();
+    }
+    if (ok) {
+      // v_ref once more: the scale of the sequence's first page
+      float inv = 0.f;
+      if (nkv[t] > 0 && l != 0.f) {
+        const int pg = page_of(0);
+        const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
+        inv = (s == s ? s : 1.0f) / l;
+      }
+      uint4* dst = (uint4*)((__nv_bfloat16*)a.o.p + (p.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh);
+#pragma unroll
+      for (int cch = 0; cch < D / 32; cch++) {
+        uint32_t ov[32];
+        if (nkv[t] > 0) {
+          tmem_ld32(tO + cch * 32, ov);
+          tmem_wait_ld();
+        }
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);  // a row tile that sees no key
+            if (nkv[t] > 0) {
+              w.x = pack_bf16x2(__uint_as_float(ov[8 * i]) * inv, __uint_as_float(ov[8 * i + 1]) * inv);
+              w.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv);
+              w.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv);
+              w.w = pack_bf16x2(__uint_as_float(ov[8 * i + 6]) * inv, __uint_as_float(ov[8 * i + 7]) * inv);
+            }
+            dst[cch * 4 + i] = w;
+          }
+        }
+      }
+    }
+  }
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == W_MMA) tmem_dealloc(tb, 512);
+}
+
+template <int D, bool E4M3>
+cudaError_t launch(const KvAttnArgs& a, cudaStream_t stream) {
+  auto kern = kv_attn_tc_kernel<D, E4M3>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES);
+  if (e != cudaSuccess) return e;
+  uint32_t *status = nullptr, ticket = 0;
+  if (!launch_ticket(stream, &status, &ticket)) return cudaErrorUnknown;
+  const dim3 grid((unsigned)kv_places(a.batch, a.Hq / a.pool.Hkv, 8, 1), (unsigned)a.pool.Hkv);
+  return launch_early(kern, grid, dim3(THREADS), Cfg<D>::BYTES, stream, a, status, ticket);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t stream) {
+  if (a.pool.e4m3) return a.pool.D == 128 ? launch<128, true>(a, stream) : launch<64, true>(a, stream);
+  return a.pool.D == 128 ? launch<128, false>(a, stream) : launch<64, false>(a, stream);
+}
+
+}  // namespace ar
+
+#ifdef AR_WAIT_TEST
+// Test build only: which tile of keys the producers leave out, -1 for none.
+extern "C" int ar_test_skip_cache_tile(int j) {
+  return (int)cudaMemcpyToSymbol(ar::g_test_skip_cache_tile, &j, sizeof(int));
+}
+#endif

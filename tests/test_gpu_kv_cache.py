@@ -243,6 +243,26 @@ def test_long_sequences_are_cut_and_joined(ops, fp8, f32, D, page, Hkv, Hq):
     s.check_attention(lengths, [2, 2, 2], Hq, causal=False)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 32), (128, 128), (64, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_rows(ops, fp8, D, page, causal):
+    """Calls that the tensor-core kernel takes: row tiles of 128 and 256 and their edges, key tiles of 128 and theirs, rows
+    without keys, sequences of one row beside them, groups that do not divide a tile."""
+    lengths, new = [300, 129, 256, 257, 5, 640, 90, 0], [300, 128, 255, 1, 5, 100, 130, 3]
+    s = Setup(ops, D + page + 7, lengths, Hkv=2, D=D, page=page, fp8=fp8, mean=True)
+    s.append(lengths, lengths)
+    for Hq in (2, 6, 8):
+        s.check_attention(lengths, new, Hq, causal)
+
+
+def test_many_rows_on_a_long_sequence(ops):
+    s = Setup(ops, 17, [4000, 1000], Hkv=1, D=128, page=64)
+    s.append([4000, 1000], [4000, 1000])
+    s.check_attention([4000, 1000], [70, 33], 4)
+    s.check_attention([4000, 1000], [70, 33], 4, causal=False)
+
+
 def test_rows_of_no_sequence_are_left(ops):
     import torch
     s = Setup(ops, 21, [40, 9], Hkv=1, D=64)
@@ -264,8 +284,11 @@ def test_unused_rows_and_pages_do_not_matter(ops, fp8, f32):
     s = Setup(ops, 31, lengths, Hkv=2, D=128, page=64, fp8=fp8, f32=f32)
     s.append(lengths, lengths)
     q, _ = s.rows(3, 8)
+    many, _ = s.rows(90, 8)
     where = (s.dtable, s.ints(lengths))
+    wide = (many, *where, s.ints([0, 20, 89, 90]))
     first = s.ops.kv_cache_attention(s.cache, q, *where)
+    first_wide = s.ops.kv_cache_attention(s.cache, *wide)
     used = torch.zeros(s.cache.k.shape[0], s.page, dtype=torch.bool, device="cuda")
     for b, n in enumerate(lengths):
         for t in range(n):
@@ -274,6 +297,7 @@ def test_unused_rows_and_pages_do_not_matter(ops, fp8, f32):
         codes.masked_fill_(~used[:, None, :, None], 0x7f if fp8 else -128)
         scales.masked_fill_(~used.any(dim=1)[:, None], float("nan"))
     assert torch.equal(first, s.ops.kv_cache_attention(s.cache, q, *where))
+    assert torch.equal(first_wide, s.ops.kv_cache_attention(s.cache, *wide))
 
 
 @pytest.mark.parametrize("f32", [False, True])
@@ -289,16 +313,17 @@ def test_scales_that_differ_by_orders_of_magnitude(ops, f32, fp8):
         v[j * page:(j + 1) * page] *= 2.0 ** e
     v[3 * page:4 * page] = 0.0
     v = torch.from_numpy(v).cuda().to(k.dtype)
-    q, qf = s.rows(8, 4, 2.0)
+    q, qf = s.rows(40, 4, 2.0)
     where = (s.dtable, s.ints([L]), s.ints([0, L]))
     s.ops.kv_cache_append(s.cache, k, v, *where)
     s.plain.append(kf, v.float().cpu().numpy(), s.table, [L], [0, L])
     s.check_pool()
     # causal rows up to the end of each page: what a row sees differs by 2^40 from what the next one does
     for last in (16, 32, 33, 48, 64, 80, 95, 96, 160):
-        got = s.ops.kv_cache_attention(s.cache, q, s.dtable, s.ints([last]), s.ints([0, 8]))
-        want = s.expect(qf, [last], np.array([0, 8]), True)
-        assert_attention_close(got.double().cpu().numpy(), *want, f32)
+        for n in (8, 40):
+            got = s.ops.kv_cache_attention(s.cache, q[:n], s.dtable, s.ints([last]), s.ints([0, n]))
+            want = s.expect(qf[:n], [last], np.array([0, n]), True)
+            assert_attention_close(got.double().cpu().numpy(), *want, f32)
 
 
 @pytest.mark.parametrize("f32", [False, True])
@@ -308,9 +333,10 @@ def test_large_and_tiny_queries(ops, f32):
     s = Setup(ops, 51, lengths, Hkv=1, D=128, page=32, f32=f32)
     s.append(lengths, lengths)
     for scale in (300.0, 1e-30, 0.0):
-        got, qf, starts = s.attend(lengths, [5], 4, q_scale=scale)
-        want = s.expect(qf, lengths, starts, True)
-        assert_attention_close(got.double().cpu().numpy(), *want, f32)
+        for n in (5, 30):
+            got, qf, starts = s.attend(lengths, [n], 4, q_scale=scale)
+            want = s.expect(qf, lengths, starts, True)
+            assert_attention_close(got.double().cpu().numpy(), *want, f32)
 
 
 def test_pages_shared_by_sequences_that_only_read_them(ops):
@@ -356,6 +382,14 @@ def test_bad_pages_are_skipped_and_reported(ops):
         want = attention(qf[:1].astype(np.float64), kk[keep], vv[keep], np.array([63]), True)
         assert_attention_close(o[:1].double().cpu().numpy(), *want, False)
         assert torch.equal(o[1:], s.ops.kv_cache_attention(s.cache, q, s.dtable, where[1])[1:])
+        # the same in a call of many rows
+        many, mf = s.rows(100, 4)
+        o = s.ops.kv_cache_attention(s.cache, many, *where, s.ints([0, 60, 100]))
+        assert ops.last_status(None) == _abi.AR_ERR_PAGE and ops.last_status(None) == 0
+        pos = np.arange(4, 64)
+        seen = np.where(pos < 16, pos, np.where(pos < 32, 15, pos - 16))
+        want = attention(mf[:60].astype(np.float64), kk[keep], vv[keep], seen, True)
+        assert_attention_close(o[:60].double().cpu().numpy(), *want, False)
         # writing: nothing of that page's tokens, the others are written
         before = [x.clone() for x in (s.cache.k, s.cache.v)]
         new, _ = s.rows(16, 2)
