@@ -7,25 +7,27 @@
 // exponential, and the tensor cores see the codes as f16 (exact) and P and q in f16 (q scaled by a power of two per row:
 // exact but for elements 2^-14 below its largest; P rounded to nearest, the row sum keeps the unrounded values).
 //
-// CTA = 2 tiles of 128 rows (tokens x query heads of the group) of one kv head, 512 threads at 128 registers:
-//   warps 0-3, 4-7  softmax of tile 0 and 1: one thread per row = TMEM lane
-//   warps 8-11      producers: codes from global memory to f16 tiles in shared memory, K and V through rings of 2 tiles of
-//                   128 keys.  A 16-byte piece of codes becomes 32 bytes of a row; rows of 128 bytes in boxes of 64 channels,
-//                   the 16-byte chunk c of row r at c ^ (r & 7), as a swizzled TMA load would leave them: K is read K-major, V MN-major.
-//                   The next tile's codes are in registers while the ring is full.
-//   warp  12        issues the MMAs: S_t = Q_t K_j^T, O_t += P_t V_j in the order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
-//   TMEM (512 columns): S_0, S_1 (P overwrites the first half of its S), O_0, O_1.
-// The softmax reads S twice, 32 columns at a time -- maximum, then exponentials -- which keeps it inside 128 registers, so
-// that the producers need no registers of its.
+// CTA = 2 tiles of 128 rows (tokens x query heads of the group) of one kv head, five warpgroups:
+//   0, 1  softmax of tile 0 and 1: one thread per row = TMEM lane
+//   2, 3  producers of K and of V: codes from global memory to f16 tiles in shared memory, rings of 2 tiles of 128 keys.  A
+//         16-byte piece of codes becomes 32 bytes of a row; rows of 128 bytes in boxes of 64 channels, the 16-byte chunk c of
+//         row r at c ^ (r & 7), as a swizzled TMA load would leave them: K is read K-major, V MN-major.  The next tile's codes
+//         are in registers while the ring is full.
+//   4     warp 0 issues the MMAs: S_t = Q_t K_j^T, O_t += P_t V_j in the order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
+//   TMEM (512 columns): S_0, S_1 (P overwrites the second half of its S), O_0, O_1.
+// The softmax takes S 64 columns at a time -- the maximum of all, then the exponentials, the upper 64 first: those it still
+// holds -- which leaves registers for the producers (setmaxnreg: 136, 80 and 48 of the 96 per thread at launch).
 //
-// What bounds it: a step of two tiles and 128 keys of D = 128 is 2048 clocks of MMA and as many of MUFU exponentials (a quarter of
-// them is taken by a polynomial on the FMA pipe); the operands' reads from shared memory take 1536 of its clocks, the producers'
-// writes 512.
+// What bounds it: a step of two tiles and 128 keys of D = 128 is 2048 clocks of MMA and as many of MUFU exponentials; the
+// operands' reads from shared memory take 1536 of its clocks, the producers' writes 512; the schedulers issue about 1900
+// instructions each.  (A quarter of the exponentials as polynomials, as in the bf16 forward, would cost issue slots that the
+// producers need.)
 #include <cuda_bf16.h>
 
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
-#include "softmax_math.cuh"
+
+#include <type_traits>
 
 namespace ar {
 namespace {
@@ -36,13 +38,14 @@ __device__ int g_test_skip_cache_tile = -1;
 #endif
 
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = BM * TILES;
-constexpr int THREADS = 512, W_PROD = 8, W_MMA = 12;
+constexpr int THREADS = 640, W_PROD = 8, W_MMA = 16;
+constexpr int SOFTMAX_REGS = 136, PRODUCER_REGS = 80, MMA_REGS = 48, LAUNCH_REGS = 96;
+static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * MMA_REGS <= LAUNCH_REGS * THREADS, "register pool of the CTA");
 constexpr int BLOCKS = BN / 16;  // column blocks of one page at least
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -1e30f;            // where a row's maximum starts; a hidden key is -inf
 constexpr float P_SHIFT = 8.0f, LAG = 6.0f;  // P < 2^14: inside f16, and a weight 2^-22 of the largest still a normal number
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60
-constexpr uint32_t POLY_MASK = 0x8888u;  // of 16 pairs of columns, those whose exponentials are a polynomial's
 
 template <int D>
 struct Cfg {
@@ -169,76 +172,84 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   const uint32_t tb = *tmem_slot;
 
   if (warp >= W_PROD && warp < W_MMA) {
-    // ------------------------------------------------------------ producers
-    const int ptid = tid - W_PROD * 32;
-    constexpr int PIECES = D / 16;            // 16-byte pieces of a key's codes
-    constexpr int PER = BN * PIECES / 128;    // of a tile, per thread
-    // thread -> key ptid / PIECES of every 128 / PIECES keys, piece ptid % PIECES
-    constexpr int KEYS = 128 / PIECES;        // keys of one pass: 16 (D = 128) or 32
+    // ------------------------------------------------------------ producers: the first warpgroup K, the second V
+    setmaxnreg_dec<PRODUCER_REGS>();
+    const bool is_v = warp >= W_PROD + 4;
+    const int ptid = tid & 127;
+    constexpr int PIECES = D / 16;          // 16-byte pieces of a key's codes
+    constexpr int PER = BN * PIECES / 128;  // of a tile, per thread
+    constexpr int KEYS = 128 / PIECES;      // keys of one pass: 16 (D = 128) or 32; thread: key key_t of them, piece q
     const int key_t = ptid / PIECES, q = ptid % PIECES;
-    const float v_ref_raw = [&] {
-      const int pg = nkv_max > 0 ? page_of(0) : -1;
+    const int in_page = (1 << log2) - 1;
+    const long long page_bytes = ((long long)Hkv << log2) * D;
+    const uint8_t* codes = (is_v ? a.pool.v : a.pool.k) + ((long long)h << log2) * D + (key_t & 15) * D + q * 16;
+    float v_ref = 1.0f;
+    if (nkv_max > 0) {
+      const int pg = page_of(0);
       const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
-      return s == s ? s : 1.0f;
-    }();
+      v_ref = s == s ? s : 1.0f;
+    }
     // page numbers: lane l < 8 of every warp holds that of the tile's l-th block of 16 keys, two tiles ahead
     auto look = [&](int j) { return lane < BLOCKS ? page_of(j * BN + lane * 16) : -2; };
     int pages = look(0), pages1 = look(1);
-    uint4 kc[PER], vc[PER];
-    auto load = [&](const uint8_t* codes, uint4(&to)[PER], int j, int pages) {
+    uint4 held[PER];
+    auto load = [&](int j, int pages) {
+      const bool whole = __all_sync(0xffffffffu, pages >= 0 || lane >= BLOCKS) && j * BN + BN <= end;
 #pragma unroll
       for (int i = 0; i < PER; i++) {
-        const int key = j * BN + i * KEYS + key_t;
-        const int pg = __shfl_sync(0xffffffffu, pages, (i * KEYS + key_t) >> 4);
-        to[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the end and without a page: codes of value 0
-        if (pg >= 0 && key < end)
-          to[i] = *(const uint4*)(codes + ((((long long)pg * Hkv + h) << log2) + (key & ((1 << log2) - 1))) * D + q * 16);
+        const int blk = (i * KEYS + key_t) >> 4;
+        const int pg = __shfl_sync(0xffffffffu, pages, blk);
+        const uint8_t* src = codes + (long long)pg * page_bytes + ((j * BN + blk * 16) & in_page) * D;
+        if (whole) {
+          held[i] = *(const uint4*)src;
+        } else {  // keys past the end and without a page: codes of value 0
+          held[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (pg >= 0 && j * BN + i * KEYS + key_t < end) held[i] = *(const uint4*)src;
+        }
       }
     };
-    // one tile of f16 from the codes in registers
-    auto store = [&](uint8_t* tile, const uint4(&codes)[PER]) {
+    // Chunks 2 * (q & 3) and the next one of box q >> 2; the second box's pieces are written in the other order, so that the 8
+    // lanes of a row write 8 different chunk places at a time.
+    const int flip = (q >> 2) & 1;
+    const uint32_t row_at = (q >> 2) * C::BOX + key_t * 128;
+    const uint32_t at0 = row_at + ((((q & 3) * 2 + flip) ^ (key_t & 7)) << 4), at1 = row_at + ((((q & 3) * 2 + 1 - flip) ^ (key_t & 7)) << 4);
+    auto store = [&](uint8_t* tile) {
 #pragma unroll
       for (int i = 0; i < PER; i++) {
-        const int r = i * KEYS + key_t;
+        const uint4 w = held[i];
         uint4 x, y;
-        expand4<E4M3>(codes[i].x, x.x, x.y);
-        expand4<E4M3>(codes[i].y, x.z, x.w);
-        expand4<E4M3>(codes[i].z, y.x, y.y);
-        expand4<E4M3>(codes[i].w, y.z, y.w);
-        // chunks 2 * (q & 3) and the next one of box q >> 2; the second box's pieces are written in the other order, so that
-        // the 8 lanes of a row write 8 different chunk places at a time
-        uint8_t* row = tile + (q >> 2) * C::BOX + r * 128;
-        const int c0 = (q & 3) * 2, flip = (q >> 2) & 1;
-        *(uint4*)(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? y : x;
-        *(uint4*)(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? x : y;
+        expand4<E4M3>(flip ? w.z : w.x, x.x, x.y);
+        expand4<E4M3>(flip ? w.w : w.y, x.z, x.w);
+        expand4<E4M3>(flip ? w.x : w.z, y.x, y.y);
+        expand4<E4M3>(flip ? w.y : w.w, y.z, y.w);
+        *(uint4*)(tile + at0 + i * KEYS * 128) = x;
+        *(uint4*)(tile + at1 + i * KEYS * 128) = y;
       }
     };
-    if (nkv_max > 0) {
-      load(a.pool.k, kc, 0, pages);
-      load(a.pool.v, vc, 0, pages);
-    }
+    if (nkv_max > 0) load(0, pages);
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    uint8_t* ring = is_v ? sV : sK;
     bool ok = !*abort_flag;
-    for (int j = 0; j < nkv_max && ok; j++) {
+    for (int j = 0; j < nkv_max; j++) {
       const int s = j % ST, n = j / ST;
       const int now = pages;
       pages = pages1;
       pages1 = look(j + 2);
 #ifdef AR_WAIT_TEST
       // Test build only: one tile is never delivered, so that the wait for it runs out.
-      if (j == g_test_skip_cache_tile) break;
+      if (j == g_test_skip_cache_tile && !is_v) break;
 #endif
-      if (n > 0) ok = mbar_wait(&k_empty[s], (n - 1) & 1, wctx, 0x50);
+      if (n > 0) ok = mbar_wait(&empty[s], (n - 1) & 1, wctx, is_v ? 0x51 : 0x50);
       if (!__all_sync(0xffffffffu, ok)) break;
-      store(sK + s * C::TILE, kc);
-      if (j + 1 < nkv_max) load(a.pool.k, kc, j + 1, pages);
-      if (ptid < BLOCKS) {  // (lanes 0 .. 7 of the first producer warp, which hold the pages of their blocks)
+      store(ring + s * C::TILE);
+      if (!is_v && ptid < BLOCKS) {  // (lanes 0 .. 7 of the first warp, which hold the pages of their blocks)
         float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS + ptid;
         float sk = 0.f, lv = -INFINITY, wv = 0.f;  // nothing there: every logit -inf, every weight 0
         if (now >= 0) {
           sk = a.pool.k_scale[(long long)now * Hkv + h];
           const float vs = v_scale_of(now);
-          lv = log2f(vs) - log2f(v_ref_raw);
-          wv = vs == vs ? v_ref_raw / vs : 1.0f;
+          lv = log2f(vs) - log2f(v_ref);
+          wv = vs == vs ? v_ref / vs : 1.0f;
         } else if (now == -1) {
           kv_report(a.batch);
         }
@@ -247,15 +258,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         slot[2 * BLOCKS] = wv;
       }
       fence_proxy_async_smem();
-      mbar_arrive(&k_full[s]);
-      if (n > 0) ok = mbar_wait(&v_empty[s], (n - 1) & 1, wctx, 0x51);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      store(sV + s * C::TILE, vc);
-      if (j + 1 < nkv_max) load(a.pool.v, vc, j + 1, pages);
-      fence_proxy_async_smem();
-      mbar_arrive(&v_full[s]);
+      mbar_arrive(&full[s]);
+      if (j + 1 < nkv_max) load(j + 1, pages);
     }
-  } else if (warp == W_MMA) {
+  } else if (warp >= W_MMA) {
+    setmaxnreg_dec<MMA_REGS>();
+    if (warp == W_MMA) {
     // ------------------------------------------------------------ MMA issuer (converged; one elected lane issues)
     const uint64_t k_proto = make_sdesc_sw128(0, 16, 1024), v_proto = make_sdesc_sw128(0, C::BOX, 1024);
     const uint32_t k_hi = (uint32_t)(k_proto >> 32), v_hi = (uint32_t)(v_proto >> 32);
@@ -276,8 +284,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       if (!elect_one()) return;
 #pragma unroll
       for (int i2 = 0; i2 < C::PV_STEPS / 2; i2++) {  // 16 keys = 2048 bytes of each box
-        const int i = half * (C::PV_STEPS / 2) + i2;
-        mma_ts_lohi<KIND_F16>(d, pa + i * 8, va + i * (2048 >> 4), v_hi, C::IDESC_PV, (acc || i > 0) ? 1u : 0u);
+        const int i = (1 - half) * (C::PV_STEPS / 2) + i2;  // the upper half of the keys comes first, also in TMEM
+        mma_ts_lohi<KIND_F16>(d, pa + 64 + half * 32 + i2 * 8, va + i * (2048 >> 4), v_hi, C::IDESC_PV, (acc || half > 0 || i2 > 0) ? 1u : 0u);
       }
     };
     bool ok = true;
@@ -320,8 +328,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       commit_one(&v_empty[s]);
       if (j + 1 < nkv_max) commit_one(&k_empty[s1]);
     }
-  } else if (warp < W_PROD) {
+    }
+  } else {
     // ------------------------------------------------------------ softmax: thread = row
+    setmaxnreg_inc<SOFTMAX_REGS>();
     const int t = warp >> 2, r = tid & 127, row = r0 + t * BM + r;
     const bool in = row < all_rows;
     const int token = in ? row / G : 0;
@@ -365,13 +375,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       constexpr bool EDGE = decltype(edge_c)::value;
       const float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS;
       const int first_out = lim - j * BN;
-      // maximum
+      uint32_t sa[32], sb[32];
       float mc = -INFINITY;
-      uint32_t sv[32];
-#pragma unroll
-      for (int qd = 0; qd < 4; qd++) {
-        tmem_ld32(tS + qd * 32, sv);
-        tmem_wait_ld();
+      auto maximum = [&](const uint32_t(&sv)[32], int qd) {  // of columns 32 * qd ..
+        const float2 c = *(const float2*)(slot + qd * 2), add = *(const float2*)(slot + BLOCKS + qd * 2);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
           float top[2] = {-INFINITY, -INFINITY};
@@ -380,17 +387,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
             float x[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const int col = qd * 32 + b * 16 + i + k;
               x[k] = __uint_as_float(sv[b * 16 + i + k]);
-              if (EDGE && col >= first_out) x[k] = -INFINITY;
+              if (EDGE && qd * 32 + b * 16 + i + k >= first_out) x[k] = -INFINITY;
             }
             top[0] = fmax3(top[0], x[0], x[1]);
             top[1] = fmax3(top[1], x[2], x[3]);
           }
-          // (a block without a page: s_k = 0 and log2 -inf, and 0 * -inf above is NaN, which the maximum passes over)
-          mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c_row * slot[qd * 2 + b], slot[BLOCKS + qd * 2 + b]));
+          // (a block without a page: s_k = 0 and log2 -inf; where all of it is hidden as well, 0 * -inf is NaN, which the
+          // maximum passes over)
+          mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c_row * (b ? c.y : c.x), b ? add.y : add.x));
         }
-      }
+      };
+      tmem_ld32(tS, sa);
+      tmem_ld32(tS + 32, sb);
+      tmem_wait_ld32(sa);
+      tmem_wait_ld32(sb);
+      maximum(sa, 0);
+      tmem_ld32(tS + 64, sa);
+      maximum(sb, 1);
+      tmem_ld32(tS + 96, sb);
+      tmem_wait_ld32(sa);
+      tmem_wait_ld32(sb);
+      maximum(sa, 2);
+      maximum(sb, 3);
       const bool need = mc > m + LAG;
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? mc : m;
@@ -400,61 +419,62 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         if (j > 0) {  // S(j) has arrived, so PV(j-1) is complete and O may be scaled in place
           const uint64_t alpha2 = pack_f32x2(alpha, alpha);
 #pragma unroll 1
-          for (int cch = 0; cch < D / 32; cch++) {
-            tmem_ld32(tO + cch * 32, sv);
+          for (int cch = 0; cch < D / 16; cch++) {
+            uint32_t ov[16];
+            tmem_ld16(tO + cch * 16, ov);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+            for (int i = 0; i < 16; i += 2) {
               float x, y;
-              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), alpha2), x, y);
-              sv[i] = __float_as_uint(x);
-              sv[i + 1] = __float_as_uint(y);
+              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1])), alpha2), x, y);
+              ov[i] = __float_as_uint(x);
+              ov[i + 1] = __float_as_uint(y);
             }
-            tmem_st32(tO + cch * 32, sv);
+            tmem_st16(tO + cch * 16, ov);
           }
         }
       }
-      // exponentials
       const float ref = m - P_SHIFT;
-#pragma unroll
-      for (int qd = 0; qd < 4; qd++) {
-        tmem_ld32(tS + qd * 32, sv);
-        tmem_wait_ld();
+      auto weights = [&](const uint32_t(&sv)[32], int qd, uint32_t to) {
+        const float2 c = *(const float2*)(slot + qd * 2), add = *(const float2*)(slot + BLOCKS + qd * 2),
+                     w = *(const float2*)(slot + 2 * BLOCKS + qd * 2);
         uint32_t pk[16];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-          const float c = c_row * slot[qd * 2 + b], add = slot[BLOCKS + qd * 2 + b] - ref;
-          const uint64_t c2 = pack_f32x2(c, c), add2 = pack_f32x2(add, add);
+          const float cb = c_row * (b ? c.y : c.x), ab = (b ? add.y : add.x) - ref;
+          const uint64_t c2 = pack_f32x2(cb, cb), add2 = pack_f32x2(ab, ab);
           uint64_t sum = pack_f32x2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const int at = b * 16 + 2 * i;
-            uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2);
-            float p0, p1;
+            float x, y;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2), x, y);
+            float p0 = ex2f(x), p1 = ex2f(y);
             if constexpr (EDGE) {
-              float x, y;
-              unpack_f32x2(x2, x, y);
-              p0 = qd * 32 + at >= first_out ? 0.f : ex2f(x);
-              p1 = qd * 32 + at + 1 >= first_out ? 0.f : ex2f(y);
-            } else if ((POLY_MASK >> (b * 8 + i)) & 1u) {
-              exp2_poly_x2(x2, p0, p1);
-            } else {
-              exp2_mufu_x2(x2, p0, p1);
+              if (qd * 32 + at >= first_out) p0 = 0.f;
+              if (qd * 32 + at + 1 >= first_out) p1 = 0.f;
             }
             sum = add_f32x2(sum, pack_f32x2(p0, p1));
             pk[b * 8 + i] = pack_half2(p0, p1);
           }
           float s0, s1;
           unpack_f32x2(sum, s0, s1);
-          l = fmaf(s0 + s1, slot[2 * BLOCKS + qd * 2 + b], l);
+          l = fmaf(s0 + s1, b ? w.y : w.x, l);
         }
-        if (qd == 2) {  // the first half of P has landed: its products run under the rest
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&p_part[2 * t]);
-        }
-        tmem_st16(tS + qd * 16, pk);
-      }
+        tmem_st16(to, pk);
+      };
+      // P: keys 64 .. 127 at columns 64 .. 95 (their scores are in registers), keys 0 .. 63 at 96 .. 127
+      weights(sa, 2, tS + 64);
+      tmem_ld32(tS, sa);
+      weights(sb, 3, tS + 80);
+      tmem_ld32(tS + 32, sb);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_part[2 * t]);  // the first half's products run under the rest
+      tmem_wait_ld32(sa);
+      tmem_wait_ld32(sb);
+      weights(sa, 0, tS + 96);
+      weights(sb, 1, tS + 112);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_part[2 * t + 1]);
