@@ -16,16 +16,16 @@
 //   4     warp 0 issues the MMAs: S_t = Q_t K_j^T, O_t += P_t V_j in the order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
 //   TMEM (512 columns): S_0, S_1 (P overwrites the second half of its S), O_0, O_1.
 // The softmax takes S 64 columns at a time -- the maximum of all, then the exponentials, the upper 64 first: those it still
-// holds -- which leaves registers for the producers (setmaxnreg: 136, 80 and 48 of the 96 per thread at launch).
+// holds -- which leaves registers for the producers (setmaxnreg: 144, 64 and 64 of the 96 per thread at launch).
 //
 // What bounds it: a step of two tiles and 128 keys of D = 128 is 2048 clocks of MMA and as many of MUFU exponentials; the
-// operands' reads from shared memory take 1536 of its clocks, the producers' writes 512; the schedulers issue about 1900
-// instructions each.  (A quarter of the exponentials as polynomials, as in the bf16 forward, would cost issue slots that the
-// producers need.)
+// operands' reads from shared memory take 1536 of its clocks, the producers' writes 512.  (A quarter of the exponentials as
+// polynomials, as in the bf16 forward, changed the time by 1 %.)
 #include <cuda_bf16.h>
 
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
+#include "softmax_math.cuh"
 
 #include <type_traits>
 
@@ -39,7 +39,7 @@ __device__ int g_test_skip_cache_tile = -1;
 
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = BM * TILES;
 constexpr int THREADS = 640, W_PROD = 8, W_MMA = 16;
-constexpr int SOFTMAX_REGS = 136, PRODUCER_REGS = 80, MMA_REGS = 48, LAUNCH_REGS = 96;
+constexpr int SOFTMAX_REGS = 144, PRODUCER_REGS = 64, MMA_REGS = 64, LAUNCH_REGS = 96;
 static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * MMA_REGS <= LAUNCH_REGS * THREADS, "register pool of the CTA");
 constexpr int BLOCKS = BN / 16;  // column blocks of one page at least
 constexpr float LOG2E = 1.4426950408889634f;
@@ -195,15 +195,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     uint4 held[PER];
     auto load = [&](int j, int pages) {
       const bool whole = __all_sync(0xffffffffu, pages >= 0 || lane >= BLOCKS) && j * BN + BN <= end;
+      if (whole && log2 == 7) {  // one page
+        const uint8_t* src = codes + (long long)__shfl_sync(0xffffffffu, pages, 0) * page_bytes + (key_t & ~15) * D;
 #pragma unroll
-      for (int i = 0; i < PER; i++) {
-        const int blk = (i * KEYS + key_t) >> 4;
-        const int pg = __shfl_sync(0xffffffffu, pages, blk);
-        const uint8_t* src = codes + (long long)pg * page_bytes + ((j * BN + blk * 16) & in_page) * D;
-        if (whole) {
-          held[i] = *(const uint4*)src;
-        } else {  // keys past the end and without a page: codes of value 0
-          held[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < PER; i++) held[i] = *(const uint4*)(src + i * KEYS * D);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          const int blk = (i * KEYS + key_t) >> 4;
+          const int pg = __shfl_sync(0xffffffffu, pages, blk);
+          const uint8_t* src = codes + (long long)pg * page_bytes + ((j * BN + blk * 16) & in_page) * D;
+          held[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the end and without a page: codes of value 0
           if (pg >= 0 && j * BN + i * KEYS + key_t < end) held[i] = *(const uint4*)src;
         }
       }
@@ -447,9 +449,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const int at = b * 16 + 2 * i;
-            float x, y;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2), x, y);
-            float p0 = ex2f(x), p1 = ex2f(y);
+            const uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2);
+            float p0, p1;
+            exp2_mufu_x2(x2, p0, p1);
             if constexpr (EDGE) {
               if (qd * 32 + at >= first_out) p0 = 0.f;
               if (qd * 32 + at + 1 >= first_out) p1 = 0.f;
