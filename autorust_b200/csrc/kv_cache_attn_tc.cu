@@ -13,14 +13,14 @@
 //         16-byte piece of codes becomes 32 bytes of a row; rows of 128 bytes in boxes of 64 channels, the 16-byte chunk c of
 //         row r at c ^ (r & 7), as a swizzled TMA load would leave them: K is read K-major, V MN-major.  The next tile's codes
 //         are in registers while the ring is full.
-//   4     warp 0 issues the MMAs: S_t = Q_t K_j^T, O_t += P_t V_j in the order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
-//   TMEM (512 columns): S_0, S_1 (P overwrites the second half of its S), O_0, O_1.
-// The softmax takes S 64 columns at a time -- the maximum of all, then the exponentials, the upper 64 first: those it still
-// holds -- which leaves registers for the producers (setmaxnreg: 144, 64 and 64 of the 96 per thread at launch).
+//   4     warp 0 issues the MMAs
+//   TMEM (512 columns): S_0, S_1, O_0, O_1.  S_t is two buffers of 64 keys: while the softmax works on one, the other is computed,
+// so that no row waits for the way from its weights over PV and QK to the next scores.  P (f16) overwrites the first half of its
+// scores.  Step i of tile t: P_t(i) done -> O_t += P_t(i) V(i), then S_t(i + 2) = Q_t K(i + 2) into the same buffer.
+// A row's O may be rescaled only when no PV of its tile is under way: the softmax waits for the last one then, which is rare.
 //
-// What bounds it: a step of two tiles and 128 keys of D = 128 is 2048 clocks of MMA and as many of MUFU exponentials; the
-// operands' reads from shared memory take 1536 of its clocks, the producers' writes 512.  (A quarter of the exponentials as
-// polynomials, as in the bf16 forward, changed the time by 1 %.)
+// Measured, 2 x 1024 rows x 4 heads against 16384 keys, D = 128: S in one buffer of 128 keys 643 us, every unit below 40 % -- the rows
+// waited.  (A quarter of the exponentials as polynomials, as in the bf16 forward, changed that by 1 %.)
 #include <cuda_bf16.h>
 
 #include "ar_ptx.cuh"
@@ -35,9 +35,10 @@ using namespace arptx;
 
 #ifdef AR_WAIT_TEST
 __device__ int g_test_skip_cache_tile = -1;
+__device__ int g_test_late_ns[2] = {0, 0};
 #endif
 
-constexpr int BM = 128, BN = 128, TILES = 2, ROWS = BM * TILES;
+constexpr int BM = 128, BN = 128, HALF = 64, TILES = 2, ROWS = BM * TILES;
 constexpr int THREADS = 640, W_PROD = 8, W_MMA = 16;
 constexpr int SOFTMAX_REGS = 144, PRODUCER_REGS = 64, MMA_REGS = 64, LAUNCH_REGS = 96;
 static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * MMA_REGS <= LAUNCH_REGS * THREADS, "register pool of the CTA");
@@ -54,14 +55,14 @@ struct Cfg {
   static constexpr int BOX = BN * 128;               // bytes: 128 rows of 64 channels
   static constexpr int TILE = BN * D * 2;            // of Q, K or V
   static constexpr int SCALE_RING = 4;               // tiles whose scales are kept
-  static constexpr int NUM_BARS = 2 + 4 * STAGES + 2 + 4 + 2;
+  static constexpr int NUM_BARS = 2 + 4 * STAGES + 4 + 4 + 2;
   static constexpr int SCALES = (TILES + 2 * STAGES) * TILE;
   static constexpr int BARS = SCALES + SCALE_RING * 3 * BLOCKS * 4;
   static constexpr int BYTES = BARS + NUM_BARS * 8 + 16 + 1024;
   static_assert(BYTES <= 227 * 1024, "shared memory budget");
-  static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, 0, 0, BM, BN);  // f16 x f16 -> f32
+  static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, 0, 0, BM, HALF);  // f16 x f16 -> f32
   static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, 0, 1, BM, D);
-  static constexpr int QK_STEPS = D / 16, PV_STEPS = BN / 16;
+  static constexpr int QK_STEPS = D / 16, PV_STEPS = HALF / 16;
 };
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -98,10 +99,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   uint64_t* k_empty = k_full + ST;
   uint64_t* v_full = k_empty + ST;
   uint64_t* v_empty = v_full + ST;
-  uint64_t* s_full = v_empty + ST;     // [2]
-  uint64_t* p_part = s_full + 2;       // [tile][half of the keys]
-  uint64_t* o_full = p_part + 4;       // [2]
-  uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+  uint64_t* s_full = v_empty + ST;     // [tile][buffer]
+  uint64_t* p_full = s_full + 4;       // [tile][buffer]
+  uint64_t* pv_done = p_full + 4;      // [2]
+  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   const WaitCtx wctx{abort_flag, status, a.batch.sticky, ticket};
 
@@ -121,14 +122,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   const int total = (int)min((long long)p.length, cap), pos0 = p.length - p.n;
   auto limit = [&](int row) { return a.causal ? max(min(total, pos0 + row / G + 1), 0) : total; };
   if (total < p.length && tid == 0) kv_report(a.batch);
-  int nkv[2], low[2];  // key tiles that some row of a row tile sees; keys that all of them see
+  int nh[2], low[2];  // halves of key tiles that some row of a row tile sees; keys that all of them see
 #pragma unroll
   for (int t = 0; t < TILES; t++) {
     const int first = r0 + t * BM, last = min(first + BM, all_rows) - 1;
-    nkv[t] = first > last ? 0 : (limit(last) + BN - 1) / BN;
+    nh[t] = first > last ? 0 : (limit(last) + HALF - 1) / HALF;
     low[t] = first > last ? 0 : limit(first);
   }
-  const int nkv_max = max(nkv[0], nkv[1]);
+  const int nh_max = max(nh[0], nh[1]), nkv_max = (nh_max + 1) / 2;
   const int end = limit(min(r0 + ROWS, all_rows) - 1);
   const int log2 = a.pool.page_log2;
   const int* table = a.batch.page_table + (long long)p.b * a.batch.table_stride;
@@ -149,10 +150,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       *abort_flag = lost ? 1u : 0u;
       for (int i = 0; i < 2; i++) {
         mbar_init(&q_full[i], 128);
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_part[2 * i], 128);
-        mbar_init(&p_part[2 * i + 1], 128);
-        mbar_init(&o_full[i], 1);
+        mbar_init(&s_full[2 * i], 1);
+        mbar_init(&s_full[2 * i + 1], 1);
+        mbar_init(&p_full[2 * i], 128);
+        mbar_init(&p_full[2 * i + 1], 128);
+        mbar_init(&pv_done[i], 1);
       }
       for (int i = 0; i < ST; i++) {
         mbar_init(&k_full[i], 128);
@@ -240,6 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #ifdef AR_WAIT_TEST
       // Test build only: one tile is never delivered, so that the wait for it runs out.
       if (j == g_test_skip_cache_tile && !is_v) break;
+      if (g_test_late_ns[is_v] > 0) __nanosleep(g_test_late_ns[is_v]);  // or every one comes late
 #endif
       if (n > 0) ok = mbar_wait(&empty[s], (n - 1) & 1, wctx, is_v ? 0x51 : 0x50);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -272,63 +275,63 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const uint32_t q_lo0 = (uint32_t)k_proto | (smem_u32(sQ) >> 4);
     const uint32_t k_lo0 = (uint32_t)k_proto | (smem_u32(sK) >> 4);
     const uint32_t v_lo0 = (uint32_t)v_proto | (smem_u32(sV) >> 4);
-    auto issue_qk = [&](int t, int s) {
-      const uint32_t qa = q_lo0 + t * (C::TILE >> 4), ka = k_lo0 + s * (C::TILE >> 4);
+    auto issue_qk = [&](int t, int i) {  // S_t(i): 64 keys of tile i / 2, eight row groups of 1024 bytes into each box
+      const uint32_t qa = q_lo0 + t * (C::TILE >> 4), ka = k_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
       if (!elect_one()) return;
 #pragma unroll
-      for (int i = 0; i < C::QK_STEPS; i++) {  // 16 channels = 32 bytes of a row, four to a box
-        const uint32_t off = ((i >> 2) * C::BOX + (i & 3) * 32) >> 4;
-        mma_ss_lohi<KIND_F16>(tb + t * 128, qa + off, k_hi, ka + off, k_hi, C::IDESC_QK, i > 0);
+      for (int x = 0; x < C::QK_STEPS; x++) {  // 16 channels = 32 bytes of a row, four to a box
+        const uint32_t off = ((x >> 2) * C::BOX + (x & 3) * 32) >> 4;
+        mma_ss_lohi<KIND_F16>(tb + t * 128 + (i & 1) * HALF, qa + off, k_hi, ka + off, k_hi, C::IDESC_QK, x > 0);
       }
     };
-    auto issue_pv = [&](int t, int s, bool acc, int half) {
-      const uint32_t d = tb + 256 + t * 128, pa = tb + t * 128, va = v_lo0 + s * (C::TILE >> 4);
+    auto issue_pv = [&](int t, int i) {
+      const uint32_t d = tb + 256 + t * 128, pa = tb + t * 128 + (i & 1) * HALF;
+      const uint32_t va = v_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
       if (!elect_one()) return;
 #pragma unroll
-      for (int i2 = 0; i2 < C::PV_STEPS / 2; i2++) {  // 16 keys = 2048 bytes of each box
-        const int i = (1 - half) * (C::PV_STEPS / 2) + i2;  // the upper half of the keys comes first, also in TMEM
-        mma_ts_lohi<KIND_F16>(d, pa + 64 + half * 32 + i2 * 8, va + i * (2048 >> 4), v_hi, C::IDESC_PV, (acc || half > 0 || i2 > 0) ? 1u : 0u);
-      }
+      for (int x = 0; x < C::PV_STEPS; x++)  // 16 keys = 2048 bytes of each box
+        mma_ts_lohi<KIND_F16>(d, pa + x * 8, va + x * (2048 >> 4), v_hi, C::IDESC_PV, (i > 0 || x > 0) ? 1u : 0u);
     };
     bool ok = true;
-    if (nkv_max > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_full[0], 0, wctx, 0x52));
+    if (nh_max > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_full[0], 0, wctx, 0x52));
     for (int t = 0; t < TILES && ok; t++) {
-      if (nkv[t] == 0) continue;
+      if (nh[t] == 0) continue;
       ok = __all_sync(0xffffffffu, mbar_wait(&q_full[t], 0, wctx, 0x53));
       if (!ok) break;
       tc_fence_after();
-      issue_qk(t, 0);
-      commit_one(&s_full[t]);
+      for (int i = 0; i < min(nh[t], 2); i++) {
+        issue_qk(t, i);
+        commit_one(&s_full[2 * t + i]);
+      }
     }
-    if (ok && nkv_max > 0) commit_one(&k_empty[0]);
-    for (int j = 0; j < nkv_max && ok; j++) {
-      const int s = j % ST, s1 = (j + 1) % ST;
-      ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], (j / ST) & 1, wctx, 0x54));
-      if (!ok) break;
-      if (j + 1 < nkv_max) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_full[s1], ((j + 1) / ST) & 1, wctx, 0x55));
+    if (ok && nh_max > 0) commit_one(&k_empty[0]);
+    for (int i = 0; i < nh_max && ok; i++) {
+      const int j = i >> 1, buf = i & 1;
+      if (buf == 0) {  // a new tile of V, and of K for the step after next
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % ST], (j / ST) & 1, wctx, 0x54));
         if (!ok) break;
+        if (j + 1 < nkv_max) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&k_full[(j + 1) % ST], ((j + 1) / ST) & 1, wctx, 0x55));
+          if (!ok) break;
+        }
       }
       for (int t = 0; t < TILES && ok; t++) {
-        if (j >= nkv[t]) continue;
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&p_part[2 * t + half], j & 1, wctx, 0x56));
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, s, j > 0, half);
-        }
+        if (i >= nh[t]) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(&p_full[2 * t + buf], j & 1, wctx, 0x56));
         if (!ok) break;
-        if (j + 1 < nkv[t]) {
-          issue_qk(t, s1);
-          commit_one(&s_full[t]);
-        } else {
-          commit_one(&o_full[t]);
+        tc_fence_after();
+        issue_pv(t, i);
+        commit_one(&pv_done[t]);
+        if (i + 2 < nh[t]) {
+          issue_qk(t, i + 2);
+          commit_one(&s_full[2 * t + buf]);
         }
       }
       if (!ok) break;
-      commit_one(&v_empty[s]);
-      if (j + 1 < nkv_max) commit_one(&k_empty[s1]);
+      if (buf == 1) {
+        commit_one(&v_empty[j % ST]);
+        if (j + 1 < nkv_max) commit_one(&k_empty[(j + 1) % ST]);
+      }
     }
     }
   } else {
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 
     // Q: the row times 2^-e, its largest element below 2
     float c_row = 0.f;
-    if (nkv[t] > 0) {
+    if (nh[t] > 0) {
       const uint4* src = (const uint4*)((const __nv_bfloat16*)a.q.p + (p.row0 + (long long)token) * a.q.st + (long long)head * a.q.sh);
       uint4 w[D / 8];
       uint32_t top = 0;
@@ -372,53 +375,48 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     }
     float m = NEG, l = 0.f;
 
-    // One step: S of 128 keys -> P.  EDGE: keys from first_out on are not the row's.
-    auto step = [&](auto edge_c, int j) {
+    // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's.  False: a wait has run out.
+    auto step = [&](auto edge_c, int i) {
       constexpr bool EDGE = decltype(edge_c)::value;
-      const float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS;
-      const int first_out = lim - j * BN;
-      uint32_t sa[32], sb[32];
+      const float* slot = scales + ((i >> 1) % C::SCALE_RING) * 3 * BLOCKS + (i & 1) * (BLOCKS / 2);
+      const int first_out = lim - i * HALF;
+      const uint32_t ts = tS + (i & 1) * HALF;
+      uint32_t sv[2][32];
+      tmem_ld32(ts, sv[0]);
+      tmem_ld32(ts + 32, sv[1]);
+      const float4 sc = *(const float4*)slot, sa = *(const float4*)(slot + BLOCKS), sw = *(const float4*)(slot + 2 * BLOCKS);
+      const float c[4] = {c_row * sc.x, c_row * sc.y, c_row * sc.z, c_row * sc.w}, add[4] = {sa.x, sa.y, sa.z, sa.w};
+      const float weight[4] = {sw.x, sw.y, sw.z, sw.w};
+      tmem_wait_ld32(sv[0]);
+      tmem_wait_ld32(sv[1]);
       float mc = -INFINITY;
-      auto maximum = [&](const uint32_t(&sv)[32], int qd) {  // of columns 32 * qd ..
-        const float2 c = *(const float2*)(slot + qd * 2), add = *(const float2*)(slot + BLOCKS + qd * 2);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-          float top[2] = {-INFINITY, -INFINITY};
+      for (int b = 0; b < 4; b++) {
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float x[4];
+        for (int x = 0; x < 16; x += 4) {
+          float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              x[k] = __uint_as_float(sv[b * 16 + i + k]);
-              if (EDGE && qd * 32 + b * 16 + i + k >= first_out) x[k] = -INFINITY;
-            }
-            top[0] = fmax3(top[0], x[0], x[1]);
-            top[1] = fmax3(top[1], x[2], x[3]);
+          for (int k = 0; k < 4; k++) {
+            v[k] = __uint_as_float(sv[b >> 1][(b & 1) * 16 + x + k]);
+            if (EDGE && b * 16 + x + k >= first_out) v[k] = -INFINITY;
           }
-          // (a block without a page: s_k = 0 and log2 -inf; where all of it is hidden as well, 0 * -inf is NaN, which the
-          // maximum passes over)
-          mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c_row * (b ? c.y : c.x), b ? add.y : add.x));
+          top[0] = fmax3(top[0], v[0], v[1]);
+          top[1] = fmax3(top[1], v[2], v[3]);
         }
-      };
-      tmem_ld32(tS, sa);
-      tmem_ld32(tS + 32, sb);
-      tmem_wait_ld32(sa);
-      tmem_wait_ld32(sb);
-      maximum(sa, 0);
-      tmem_ld32(tS + 64, sa);
-      maximum(sb, 1);
-      tmem_ld32(tS + 96, sb);
-      tmem_wait_ld32(sa);
-      tmem_wait_ld32(sb);
-      maximum(sa, 2);
-      maximum(sb, 3);
+        // (a block without a page: s_k = 0 and log2 -inf; where all of it is hidden as well, 0 * -inf is NaN, which the
+        // maximum passes over)
+        mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c[b], add[b]));
+      }
       const bool need = mc > m + LAG;
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? mc : m;
         const float alpha = ex2f(m - m_new);
         m = m_new;
         l *= alpha;
-        if (j > 0) {  // S(j) has arrived, so PV(j-1) is complete and O may be scaled in place
+        if (i > 0) {  // (PV(i - 2) is done, S(i) came after it)
+          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (i - 1) & 1, wctx, 0x59))) return false;
+          tc_fence_after();
           const uint64_t alpha2 = pack_f32x2(alpha, alpha);
 #pragma unroll 1
           for (int cch = 0; cch < D / 16; cch++) {
@@ -426,80 +424,68 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
             tmem_ld16(tO + cch * 16, ov);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float x, y;
-              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1])), alpha2), x, y);
-              ov[i] = __float_as_uint(x);
-              ov[i + 1] = __float_as_uint(y);
+            for (int x = 0; x < 16; x += 2) {
+              float y, z;
+              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(ov[x]), __uint_as_float(ov[x + 1])), alpha2), y, z);
+              ov[x] = __float_as_uint(y);
+              ov[x + 1] = __float_as_uint(z);
             }
             tmem_st16(tO + cch * 16, ov);
           }
         }
       }
       const float ref = m - P_SHIFT;
-      auto weights = [&](const uint32_t(&sv)[32], int qd, uint32_t to) {
-        const float2 c = *(const float2*)(slot + qd * 2), add = *(const float2*)(slot + BLOCKS + qd * 2),
-                     w = *(const float2*)(slot + 2 * BLOCKS + qd * 2);
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
         uint32_t pk[16];
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const float cb = c_row * (b ? c.y : c.x), ab = (b ? add.y : add.x) - ref;
-          const uint64_t c2 = pack_f32x2(cb, cb), add2 = pack_f32x2(ab, ab);
+        for (int b2 = 0; b2 < 2; b2++) {
+          const int b = hf * 2 + b2;
+          const float ab = add[b] - ref;
+          const uint64_t c2 = pack_f32x2(c[b], c[b]), add2 = pack_f32x2(ab, ab);
           uint64_t sum = pack_f32x2(0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int at = b * 16 + 2 * i;
-            const uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), c2, add2);
+          for (int k = 0; k < 8; k++) {
+            const int at = b2 * 16 + 2 * k;
             float p0, p1;
-            exp2_mufu_x2(x2, p0, p1);
+            exp2_mufu_x2(fma_f32x2(pack_f32x2(__uint_as_float(sv[hf][at]), __uint_as_float(sv[hf][at + 1])), c2, add2), p0, p1);
             if constexpr (EDGE) {
-              if (qd * 32 + at >= first_out) p0 = 0.f;
-              if (qd * 32 + at + 1 >= first_out) p1 = 0.f;
+              if (hf * 32 + at >= first_out) p0 = 0.f;
+              if (hf * 32 + at + 1 >= first_out) p1 = 0.f;
             }
             sum = add_f32x2(sum, pack_f32x2(p0, p1));
-            pk[b * 8 + i] = pack_half2(p0, p1);
+            pk[b2 * 8 + k] = pack_half2(p0, p1);
           }
           float s0, s1;
           unpack_f32x2(sum, s0, s1);
-          l = fmaf(s0 + s1, b ? w.y : w.x, l);
+          l = fmaf(s0 + s1, weight[b], l);
         }
-        tmem_st16(to, pk);
-      };
-      // P: keys 64 .. 127 at columns 64 .. 95 (their scores are in registers), keys 0 .. 63 at 96 .. 127
-      weights(sa, 2, tS + 64);
-      tmem_ld32(tS, sa);
-      weights(sb, 3, tS + 80);
-      tmem_ld32(tS + 32, sb);
+        tmem_st16(ts + hf * 16, pk);
+      }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_part[2 * t]);  // the first half's products run under the rest
-      tmem_wait_ld32(sa);
-      tmem_wait_ld32(sb);
-      weights(sa, 0, tS + 96);
-      weights(sb, 1, tS + 112);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_part[2 * t + 1]);
+      mbar_arrive(&p_full[2 * t + (i & 1)]);
+      return true;
     };
 
     bool ok = true;
-    for (int j = 0; j < nkv[t]; j++) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, wctx, 0x57));
+    for (int i = 0; i < nh[t]; i++) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (i & 1)], (i >> 1) & 1, wctx, 0x57));
       if (!ok) break;
       tc_fence_after();
-      if (j * BN + BN > low[t])
-        step(std::true_type{}, j);
-      else
-        step(std::false_type{}, j);
+      ok = i * HALF + HALF > low[t] ? step(std::true_type{}, i) : step(std::false_type{}, i);
+      if (!ok) break;
     }
-    if (ok && nkv[t] > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, wctx, 0x58));
+    if (ok && nh[t] > 0) {
+      // S(i) tells that PV(i - 2) is done: after the last step two may be under way, and a parity tells one phase from the next only
+      if (nh[t] > 1) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (nh[t] - 2) & 1, wctx, 0x58));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (nh[t] - 1) & 1, wctx, 0x58));
       tc_fence_after();
     }
     if (ok) {
       // v_ref once more: the scale of the sequence's first page
       float inv = 0.f;
-      if (nkv[t] > 0 && l != 0.f) {
+      if (nh[t] > 0 && l != 0.f) {
         const int pg = page_of(0);
         const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
         inv = (s == s ? s : 1.0f) / l;
@@ -508,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
       for (int cch = 0; cch < D / 32; cch++) {
         uint32_t ov[32];
-        if (nkv[t] > 0) {
+        if (nh[t] > 0) {
           tmem_ld32(tO + cch * 32, ov);
           tmem_wait_ld();
         }
@@ -516,7 +502,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             uint4 w = make_uint4(0u, 0u, 0u, 0u);  // a row tile that sees no key
-            if (nkv[t] > 0) {
+            if (nh[t] > 0) {
               w.x = pack_bf16x2(__uint_as_float(ov[8 * i]) * inv, __uint_as_float(ov[8 * i + 1]) * inv);
               w.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv);
               w.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv);
@@ -555,8 +541,12 @@ cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t stream) {
 }  // namespace ar
 
 #ifdef AR_WAIT_TEST
-// Test build only: which tile of keys the producers leave out, -1 for none.
+// Test build only: which tile of keys the producers leave out, -1 for none; by how many nanoseconds those of K and V come late.
 extern "C" int ar_test_skip_cache_tile(int j) {
   return (int)cudaMemcpyToSymbol(ar::g_test_skip_cache_tile, &j, sizeof(int));
+}
+extern "C" int ar_test_late_cache_tiles(int k_ns, int v_ns) {
+  const int ns[2] = {k_ns, v_ns};
+  return (int)cudaMemcpyToSymbol(ar::g_test_late_ns, ns, sizeof(ns));
 }
 #endif
