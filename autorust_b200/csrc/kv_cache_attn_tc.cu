@@ -13,7 +13,8 @@
 //         16-byte piece of codes becomes 32 bytes of a row; rows of 128 bytes in boxes of 64 channels, the 16-byte chunk c of
 //         row r at c ^ (r & 7), as a swizzled TMA load would leave them: K is read K-major, V MN-major.  The next tile's codes
 //         are in registers while the ring is full.
-//   4     warp 0 issues the MMAs
+//   4     warps 0 and 1 issue the MMAs of tile 0 and 1: a wait that is over at once, a commit and the way to the next MMA take an
+//         issuer some 400 clocks a step, under which the other's MMAs run (one issuer for both: 637 us of the case below)
 //   TMEM (512 columns): S_0, S_1, O_0, O_1.  S_t is two buffers of 64 keys: while the softmax works on one, the other is computed,
 // so that no row waits for the way from its weights over PV and QK to the next scores.  P (f16) overwrites the first half of its
 // scores.  Step i of tile t: P_t(i) done -> O_t += P_t(i) V(i), then S_t(i + 2) = Q_t K(i + 2) into the same buffer.
@@ -83,6 +84,13 @@ __device__ __forceinline__ void expand4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   }
 }
 
+// One arrival for the whole warp: 32 lanes that arrive one by one take the barrier's word in turn, 128 of them several hundred
+// clocks (the handshakes of a step alone: 245 us of the case below).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if (elect_one()) mbar_arrive(bar);
+}
+
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
   using C = Cfg<D>;
@@ -114,7 +122,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   const int lane = tid & 31;
   const int G = a.Hq / a.pool.Hkv, Hkv = a.pool.Hkv, h = blockIdx.y;
   // the last tiles first: under a causal mask they are the heavy ones
-  const KvPlace p = kv_place(a.batch, (int)(gridDim.x - 1 - blockIdx.x), G, 8, 1);
+  KvPlace p = kv_place(a.batch, (int)(gridDim.x - 1 - blockIdx.x), G, 8, 1);
+  // Read from memory, but the same for all threads: told to the compiler, which otherwise takes what follows for divergent and wraps
+  // every tcgen05 instruction in an election of its own.
+  p.b = __shfl_sync(0xffffffffu, p.b, 0);
+  p.tile = __shfl_sync(0xffffffffu, p.tile, 0);
+  p.row0 = __shfl_sync(0xffffffffu, p.row0, 0);
+  p.n = __shfl_sync(0xffffffffu, p.n, 0);
+  p.length = __shfl_sync(0xffffffffu, p.length, 0);
   const int all_rows = p.n * G;
   if (p.tile < 0 || (long long)p.tile * ROWS >= all_rows) return;
   const int r0 = p.tile * ROWS;
@@ -149,18 +164,18 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       lost = launch_lost(status, ticket);
       *abort_flag = lost ? 1u : 0u;
       for (int i = 0; i < 2; i++) {
-        mbar_init(&q_full[i], 128);
+        mbar_init(&q_full[i], 4);
         mbar_init(&s_full[2 * i], 1);
         mbar_init(&s_full[2 * i + 1], 1);
-        mbar_init(&p_full[2 * i], 128);
-        mbar_init(&p_full[2 * i + 1], 128);
+        mbar_init(&p_full[2 * i], 4);
+        mbar_init(&p_full[2 * i + 1], 4);
         mbar_init(&pv_done[i], 1);
       }
       for (int i = 0; i < ST; i++) {
-        mbar_init(&k_full[i], 128);
-        mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], 128);
-        mbar_init(&v_empty[i], 1);
+        mbar_init(&k_full[i], 4);
+        mbar_init(&k_empty[i], TILES);
+        mbar_init(&v_full[i], 4);
+        mbar_init(&v_empty[i], TILES);
       }
       fence_mbar_init();
     }
@@ -263,76 +278,74 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         slot[2 * BLOCKS] = wv;
       }
       fence_proxy_async_smem();
-      mbar_arrive(&full[s]);
+      warp_arrive(&full[s]);
       if (j + 1 < nkv_max) load(j + 1, pages);
     }
   } else if (warp >= W_MMA) {
     setmaxnreg_dec<MMA_REGS>();
-    if (warp == W_MMA) {
-    // ------------------------------------------------------------ MMA issuer (converged; one elected lane issues)
-    const uint64_t k_proto = make_sdesc_sw128(0, 16, 1024), v_proto = make_sdesc_sw128(0, C::BOX, 1024);
-    const uint32_t k_hi = (uint32_t)(k_proto >> 32), v_hi = (uint32_t)(v_proto >> 32);
-    const uint32_t q_lo0 = (uint32_t)k_proto | (smem_u32(sQ) >> 4);
-    const uint32_t k_lo0 = (uint32_t)k_proto | (smem_u32(sK) >> 4);
-    const uint32_t v_lo0 = (uint32_t)v_proto | (smem_u32(sV) >> 4);
-    auto issue_qk = [&](int t, int i) {  // S_t(i): 64 keys of tile i / 2, eight row groups of 1024 bytes into each box
-      const uint32_t qa = q_lo0 + t * (C::TILE >> 4), ka = k_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
-      if (!elect_one()) return;
+    if (warp < W_MMA + TILES) {
+      // ---------------------------------------------------------- MMA issuers (converged; one elected lane issues)
+      const int t = warp - W_MMA, mine = t ? nh[1] : nh[0];
+      const uint64_t k_proto = make_sdesc_sw128(0, 16, 1024), v_proto = make_sdesc_sw128(0, C::BOX, 1024);
+      const uint32_t k_hi = (uint32_t)(k_proto >> 32), v_hi = (uint32_t)(v_proto >> 32);
+      const uint32_t q_lo = ((uint32_t)k_proto | (smem_u32(sQ) >> 4)) + t * (C::TILE >> 4);
+      const uint32_t k_lo0 = (uint32_t)k_proto | (smem_u32(sK) >> 4);
+      const uint32_t v_lo0 = (uint32_t)v_proto | (smem_u32(sV) >> 4);
+      const uint32_t ts = tb + t * 128, to = tb + 256 + t * 128;
+      // half i of the keys lies eight row groups of 1024 bytes into each box of tile i / 2
+      auto issue_qk = [&](int i) {
+        const uint32_t ka = k_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
+        if (!elect_one()) return;
 #pragma unroll
-      for (int x = 0; x < C::QK_STEPS; x++) {  // 16 channels = 32 bytes of a row, four to a box
-        const uint32_t off = ((x >> 2) * C::BOX + (x & 3) * 32) >> 4;
-        mma_ss_lohi<KIND_F16>(tb + t * 128 + (i & 1) * HALF, qa + off, k_hi, ka + off, k_hi, C::IDESC_QK, x > 0);
-      }
-    };
-    auto issue_pv = [&](int t, int i) {
-      const uint32_t d = tb + 256 + t * 128, pa = tb + t * 128 + (i & 1) * HALF;
-      const uint32_t va = v_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
-      if (!elect_one()) return;
+        for (int x = 0; x < C::QK_STEPS; x++) {  // 16 channels = 32 bytes of a row, four to a box
+          const uint32_t off = ((x >> 2) * C::BOX + (x & 3) * 32) >> 4;
+          mma_ss_lohi<KIND_F16>(ts + (i & 1) * HALF, q_lo + off, k_hi, ka + off, k_hi, C::IDESC_QK, x > 0);
+        }
+      };
+      auto issue_pv = [&](int i) {
+        const uint32_t va = v_lo0 + ((i >> 1) % ST) * (C::TILE >> 4) + (i & 1) * (HALF * 128 >> 4);
+        if (!elect_one()) return;
 #pragma unroll
-      for (int x = 0; x < C::PV_STEPS; x++)  // 16 keys = 2048 bytes of each box
-        mma_ts_lohi<KIND_F16>(d, pa + x * 8, va + x * (2048 >> 4), v_hi, C::IDESC_PV, (i > 0 || x > 0) ? 1u : 0u);
-    };
-    bool ok = true;
-    if (nh_max > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_full[0], 0, wctx, 0x52));
-    for (int t = 0; t < TILES && ok; t++) {
-      if (nh[t] == 0) continue;
-      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[t], 0, wctx, 0x53));
-      if (!ok) break;
-      tc_fence_after();
-      for (int i = 0; i < min(nh[t], 2); i++) {
-        issue_qk(t, i);
-        commit_one(&s_full[2 * t + i]);
+        for (int x = 0; x < C::PV_STEPS; x++)  // 16 keys = 2048 bytes of each box
+          mma_ts_lohi<KIND_F16>(to, ts + (i & 1) * HALF + x * 8, va + x * (2048 >> 4), v_hi, C::IDESC_PV, (i > 0 || x > 0) ? 1u : 0u);
+      };
+      auto tile_in = [&](uint64_t* full, int j, uint32_t site) { return __all_sync(0xffffffffu, mbar_wait(&full[j % ST], (j / ST) & 1, wctx, site)); };
+      bool ok = true;
+      if (nh_max > 0) ok = tile_in(k_full, 0, 0x52);
+      if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[t], 0, wctx, 0x53));
+      if (ok) {
+        tc_fence_after();
+        for (int i = 0; i < min(mine, 2); i++) {
+          issue_qk(i);
+          commit_one(&s_full[2 * t + i]);
+        }
+        if (nh_max > 0) commit_one(&k_empty[0]);
       }
-    }
-    if (ok && nh_max > 0) commit_one(&k_empty[0]);
-    for (int i = 0; i < nh_max && ok; i++) {
-      const int j = i >> 1, buf = i & 1;
-      if (buf == 0) {  // a new tile of V, and of K for the step after next
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % ST], (j / ST) & 1, wctx, 0x54));
-        if (!ok) break;
-        if (j + 1 < nkv_max) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&k_full[(j + 1) % ST], ((j + 1) / ST) & 1, wctx, 0x55));
+      // (a row tile that sees fewer keys than the other passes on what it does not use)
+      for (int i = 0; i < nh_max && ok; i++) {
+        const int j = i >> 1, buf = i & 1;
+        if (buf == 0) {  // a new tile of V, and of K for the step after next
+          ok = tile_in(v_full, j, 0x54);
+          if (j + 1 < nkv_max) ok = ok && tile_in(k_full, j + 1, 0x55);
           if (!ok) break;
         }
-      }
-      for (int t = 0; t < TILES && ok; t++) {
-        if (i >= nh[t]) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(&p_full[2 * t + buf], j & 1, wctx, 0x56));
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(t, i);
-        commit_one(&pv_done[t]);
-        if (i + 2 < nh[t]) {
-          issue_qk(t, i + 2);
-          commit_one(&s_full[2 * t + buf]);
+        if (i < mine) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&p_full[2 * t + buf], j & 1, wctx, 0x56));
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i);
+          if (i + 2 < mine) {
+            issue_qk(i + 2);
+            commit_one(&s_full[2 * t + buf]);
+          } else {
+            commit_one(&pv_done[t]);
+          }
+        }
+        if (buf == 1) {
+          commit_one(&v_empty[j % ST]);
+          if (j + 1 < nkv_max) commit_one(&k_empty[(j + 1) % ST]);
         }
       }
-      if (!ok) break;
-      if (buf == 1) {
-        commit_one(&v_empty[j % ST]);
-        if (j + 1 < nkv_max) commit_one(&k_empty[(j + 1) % ST]);
-      }
-    }
     }
   } else {
     // ------------------------------------------------------------ softmax: thread = row
@@ -371,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         *(uint4*)(dst + (i >> 3) * C::BOX + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
       }
       fence_proxy_async_smem();
-      mbar_arrive(&q_full[t]);
+      warp_arrive(&q_full[t]);
     }
     float m = NEG, l = 0.f;
 
@@ -414,8 +427,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         const float alpha = ex2f(m - m_new);
         m = m_new;
         l *= alpha;
-        if (i > 0) {  // (PV(i - 2) is done, S(i) came after it)
-          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (i - 1) & 1, wctx, 0x59))) return false;
+        if (i > 0) {  // PV(i - 1) is done when S(i + 1), issued after it, is there; behind the last scores it reports itself
+          const bool last = i + 1 == nh[t];
+          uint64_t* bar = last ? &pv_done[t] : &s_full[2 * t + ((i + 1) & 1)];
+          if (!__all_sync(0xffffffffu, mbar_wait(bar, last ? 0 : ((i + 1) >> 1) & 1, wctx, 0x59))) return false;
           tc_fence_after();
           const uint64_t alpha2 = pack_f32x2(alpha, alpha);
 #pragma unroll 1
@@ -464,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[2 * t + (i & 1)]);
+      warp_arrive(&p_full[2 * t + (i & 1)]);
       return true;
     };
 
@@ -477,9 +492,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       if (!ok) break;
     }
     if (ok && nh[t] > 0) {
-      // S(i) tells that PV(i - 2) is done: after the last step two may be under way, and a parity tells one phase from the next only
-      if (nh[t] > 1) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (nh[t] - 2) & 1, wctx, 0x58));
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (nh[t] - 1) & 1, wctx, 0x58));
+      // the last two PV report: both may be under way, and a parity tells one phase from the next only
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], 0, wctx, 0x58));
+      if (nh[t] > 1) ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_done[t], 1, wctx, 0x58));
       tc_fence_after();
     }
     if (ok) {
