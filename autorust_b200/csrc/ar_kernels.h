@@ -181,15 +181,16 @@ struct KvAttnArgs {
   int dtype, Hq, max_length, causal;
   float* partial;  // workspace; null where the plan needs none
 };
-// How a call is divided: row tiles of `rows` rows, over `ctas` CTAs that take equal shares of all keys (0: one CTA per tile);
-// rows = 256: the tensor-core kernel.
+// How a call is divided: row tiles of `rows` rows, over `ctas` CTAs that take equal shares of all keys (0: one CTA per tile).
+// rows = 256: the tensor-core kernel, with the keys of a row tile in `parts`.
 struct KvAttnPlan {
-  int rows, ctas;
+  int rows, ctas, parts;
   size_t workspace;
 };
 KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal);
 cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches);
-cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t stream);  // kv_cache_attn_tc.cu: many rows, bf16 tensors
+// kv_cache_attn_tc.cu: many rows, bf16 tensors; the keys in `parts` (at most 16).
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int parts, cudaStream_t stream, int* launches);
 
 // Sage prologue (sage_prologue.cu).
 struct PrologueArgs {

@@ -29,6 +29,7 @@
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace ar {
@@ -826,16 +827,39 @@ cudaError_t launch_nt(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t 
 
 }  // namespace
 
+// The kernels' times in microseconds, estimated from the call's sizes, decide between this one and the tensor cores' and on the
+// latter's parts.  Fitted to measured calls (1 to 64 sequences, 4 to 1024 rows x 1 to 16 heads, 64 to 16384 keys): this
+// kernel takes 1.45 ns (D = 64: 1.1) per row tile and group of keys over the whole GPU, the other a 128-key step of 256 rows in
+// 2.3 us (1.9) on one SM and 6 us for a CTA's beginning and end; partial results pass memory twice.  8 rows x 4 heads of one
+// sequence against 4096 keys: 17 us here, 72 there; 64 rows of 16 sequences against 2048: 231 and 62; 128 rows of 4
+// sequences against 16384: 749 here, 324 there in one part, 189 in four.
 KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int Hq, int max_length, int causal) {
   (void)causal;
   KvAttnPlan p;
   const int G = Hq / pool.Hkv;
-  p.rows = (long long)batch.T * G <= 8ll * batch.B ? 8 : 16;
-  if (dtype != 0 && (long long)batch.T * G >= 96ll * batch.B) {
-    p.rows = 256;
-    p.ctas = 0;
-    p.workspace = 0;
-    return p;
+  const long long mean_rows = ((long long)batch.T * G + batch.B - 1) / batch.B;
+  p.rows = mean_rows <= 8 ? 8 : 16;
+  p.parts = 1;
+  if (dtype != 0 && mean_rows > 16) {
+    const double per_group = pool.D == 128 ? 1.45e-3 : 1.1e-3, per_step = pool.D == 128 ? 2.3 : 1.9;
+    const double pairs = (double)batch.B * pool.Hkv;
+    const double here = (max_length <= WHOLE_KEYS ? 6.0 : 14.0) +
+                        pairs * ((mean_rows + 15) / 16) * ((max_length + GROUP - 1) / GROUP + START_UNITS) * per_group;
+    const long long steps = (max_length + 127) / 128, ctas = batch.B * (long long)pool.Hkv * ((mean_rows + 255) / 256);
+    auto bytes = [&](long long parts) { return parts > 1 ? sizeof(float) * (size_t)parts * batch.T * Hq * (pool.D + 4) : 0; };
+    auto there = [&](long long parts) {
+      return 5.0 + (double)((ctas * parts + SMS - 1) / SMS) * (6.0 + per_step * (double)((steps + parts - 1) / parts)) +
+             (parts > 1 ? 6.0 + 2.0 * (double)bytes(parts) / 4e6 : 0.0);
+    };
+    long long parts = std::max(1ll, std::min(std::min((long long)SMS / ctas, 16ll), steps / 4));
+    if (there(1) < there(parts)) parts = 1;
+    if (there(parts) < here) {
+      p.rows = 256;
+      p.ctas = 0;
+      p.parts = (int)parts;
+      p.workspace = bytes(parts);
+      return p;
+    }
   }
   const long long tiles = kv_places(batch, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
   p.ctas = SMS * (p.rows == 8 ? Sh<128, 1>::CTAS_PER_SM : Sh<128, 2>::CTAS_PER_SM);
@@ -846,11 +870,7 @@ KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, const KvAttnPlan& plan, cudaStream_t stream, int* launches) {
   const bool d128 = a.pool.D == 128, f32 = a.dtype == 0;
-  if (plan.rows == 256) {
-    const cudaError_t e = launch_kv_attention_tc(a, stream);
-    if (e == cudaSuccess) ++*launches;
-    return e;
-  }
+  if (plan.rows == 256) return launch_kv_attention_tc(a, plan.parts, stream, launches);
   if (a.pool.e4m3) {
     if (d128) return f32 ? launch_nt<128, true, true>(a, plan, stream, launches) : launch_nt<128, true, false>(a, plan, stream, launches);
     return f32 ? launch_nt<64, true, true>(a, plan, stream, launches) : launch_nt<64, true, false>(a, plan, stream, launches);

@@ -91,7 +91,9 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if (elect_one()) mbar_arrive(bar);
 }
 
-template <int D, bool E4M3>
+// SPLIT: the keys are divided over gridDim.z CTAs, which leave partial results for kv_join_rows_kernel: one row of D + 4 values per
+// part, packed row and head -- the accumulated values, then m + log2 v_ref, m, l.
+template <int D, bool E4M3, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
   using C = Cfg<D>;
   constexpr int ST = C::STAGES;
@@ -137,15 +139,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   const int total = (int)min((long long)p.length, cap), pos0 = p.length - p.n;
   auto limit = [&](int row) { return a.causal ? max(min(total, pos0 + row / G + 1), 0) : total; };
   if (total < p.length && tid == 0) kv_report(a.batch);
-  int nh[2], low[2];  // halves of key tiles that some row of a row tile sees; keys that all of them see
+  int end = limit(min(r0 + ROWS, all_rows) - 1), kb = 0;  // this CTA's keys: [kb, end)
+  if constexpr (SPLIT) {
+    const int tiles = (end + BN - 1) / BN;
+    kb = (int)((long long)tiles * blockIdx.z / gridDim.z) * BN;
+    end = min(end, (int)((long long)tiles * (blockIdx.z + 1) / gridDim.z) * BN);
+  }
+  int nh[2], low[2];  // halves of key tiles that some row of a row tile sees here; keys that all of them see
 #pragma unroll
   for (int t = 0; t < TILES; t++) {
     const int first = r0 + t * BM, last = min(first + BM, all_rows) - 1;
-    nh[t] = first > last ? 0 : (limit(last) + HALF - 1) / HALF;
+    nh[t] = first > last ? 0 : (max(min(limit(last), end) - kb, 0) + HALF - 1) / HALF;
     low[t] = first > last ? 0 : limit(first);
   }
   const int nh_max = max(nh[0], nh[1]), nkv_max = (nh_max + 1) / 2;
-  const int end = limit(min(r0 + ROWS, all_rows) - 1);
   const int log2 = a.pool.page_log2;
   const int* table = a.batch.page_table + (long long)p.b * a.batch.table_stride;
   auto page_of = [&](int key) {  // -2: past the end, -1: there is none
@@ -202,16 +209,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const uint8_t* codes = (is_v ? a.pool.v : a.pool.k) + ((long long)h << log2) * D + (key_t & 15) * D + q * 16;
     float v_ref = 1.0f;
     if (nkv_max > 0) {
-      const int pg = page_of(0);
+      const int pg = page_of(kb);
       const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
       v_ref = s == s ? s : 1.0f;
     }
     // page numbers: lane l < 8 of every warp holds that of the tile's l-th block of 16 keys, two tiles ahead
-    auto look = [&](int j) { return lane < BLOCKS ? page_of(j * BN + lane * 16) : -2; };
+    auto look = [&](int j) { return lane < BLOCKS ? page_of(kb + j * BN + lane * 16) : -2; };
     int pages = look(0), pages1 = look(1);
     uint4 held[PER];
     auto load = [&](int j, int pages) {
-      const bool whole = __all_sync(0xffffffffu, pages >= 0 || lane >= BLOCKS) && j * BN + BN <= end;
+      const bool whole = __all_sync(0xffffffffu, pages >= 0 || lane >= BLOCKS) && kb + j * BN + BN <= end;
       if (whole && log2 == 7) {  // one page
         const uint8_t* src = codes + (long long)__shfl_sync(0xffffffffu, pages, 0) * page_bytes + (key_t & ~15) * D;
 #pragma unroll
@@ -223,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           const int pg = __shfl_sync(0xffffffffu, pages, blk);
           const uint8_t* src = codes + (long long)pg * page_bytes + ((j * BN + blk * 16) & in_page) * D;
           held[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the end and without a page: codes of value 0
-          if (pg >= 0 && j * BN + i * KEYS + key_t < end) held[i] = *(const uint4*)src;
+          if (pg >= 0 && kb + j * BN + i * KEYS + key_t < end) held[i] = *(const uint4*)src;
         }
       }
     };
@@ -353,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const int t = warp >> 2, r = tid & 127, row = r0 + t * BM + r;
     const bool in = row < all_rows;
     const int token = in ? row / G : 0;
-    const int lim = in ? limit(row) : 0;
+    const int lim = (in ? limit(row) : 0) - kb;
     const uint32_t lane_base = (uint32_t)(warp & 3) * 32;
     const uint32_t tS = tmem_addr(tb, lane_base, t * 128), tO = tmem_addr(tb, lane_base, 256 + t * 128);
     const int head = h * G + (in ? row - token * G : 0);
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (i & 1)], (i >> 1) & 1, wctx, 0x57));
       if (!ok) break;
       tc_fence_after();
-      ok = i * HALF + HALF > low[t] ? step(std::true_type{}, i) : step(std::false_type{}, i);
+      ok = kb + i * HALF + HALF > low[t] || kb + i * HALF + HALF > end ? step(std::true_type{}, i) : step(std::false_type{}, i);
       if (!ok) break;
     }
     if (ok && nh[t] > 0) {
@@ -498,14 +505,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tc_fence_after();
     }
     if (ok) {
-      // v_ref once more: the scale of the sequence's first page
-      float inv = 0.f;
-      if (nh[t] > 0 && l != 0.f) {
-        const int pg = page_of(0);
+      // v_ref once more: the scale of this CTA's first page
+      float v_ref = 1.0f;
+      if (nh[t] > 0) {
+        const int pg = page_of(kb);
         const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
-        inv = (s == s ? s : 1.0f) / l;
+        v_ref = s == s ? s : 1.0f;
       }
-      uint4* dst = (uint4*)((__nv_bfloat16*)a.o.p + (p.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh);
+      const float inv = SPLIT ? 1.0f : nh[t] > 0 && l != 0.f ? v_ref / l : 0.f;
+      __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (p.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh;
+      float* part = a.partial + (((long long)blockIdx.z * a.batch.T + p.row0 + token) * a.Hq + head) * (D + 4);
 #pragma unroll
       for (int cch = 0; cch < D / 32; cch++) {
         uint32_t ov[32];
@@ -515,18 +524,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         }
         if (in) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);  // a row tile that sees no key
-            if (nh[t] > 0) {
-              w.x = pack_bf16x2(__uint_as_float(ov[8 * i]) * inv, __uint_as_float(ov[8 * i + 1]) * inv);
-              w.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv);
-              w.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv);
-              w.w = pack_bf16x2(__uint_as_float(ov[8 * i + 6]) * inv, __uint_as_float(ov[8 * i + 7]) * inv);
-            }
-            dst[cch * 4 + i] = w;
+          for (int i = 0; i < 8; i++) {
+            float4 w = make_float4(0.f, 0.f, 0.f, 0.f);  // a row tile that sees no key
+            if (nh[t] > 0)
+              w = make_float4(__uint_as_float(ov[4 * i]) * inv, __uint_as_float(ov[4 * i + 1]) * inv, __uint_as_float(ov[4 * i + 2]) * inv,
+                              __uint_as_float(ov[4 * i + 3]) * inv);
+            if constexpr (SPLIT)
+              *(float4*)(part + cch * 32 + i * 4) = w;
+            else
+              *(uint2*)(dst + cch * 32 + i * 4) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
           }
         }
       }
+      if (SPLIT && in) *(float4*)(part + D) = make_float4(m + log2f(v_ref), m, l, 0.f);
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -535,22 +545,75 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   if (warp == W_MMA) tmem_dealloc(tb, 512);
 }
 
+// o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p over the parts of a row, in order; A_p = m_p + log2 v_ref_p.  One warp per
+// packed row and head.
+constexpr int MOST_PARTS = 16;
+template <int D>
+__global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, int parts) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)a.batch.T * a.Hq, at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= rows) return;
+  const int row = (int)(at / a.Hq), head = (int)(at - (long long)row * a.Hq);
+  const KvPlace p = kv_place(a.batch, row, 1, 0, 0);
+  if (row < p.row0 || row >= p.row0 + p.n) return;  // a row of no sequence
+  constexpr int V = D / 32;
+  float4 e[MOST_PARTS];
+  float A = NEG, M = NEG;
+#pragma unroll
+  for (int i = 0; i < MOST_PARTS; i++) {
+    e[i] = make_float4(NEG, NEG, 0.f, 0.f);
+    if (i < parts) e[i] = *(const float4*)(a.partial + (i * rows + at) * (D + 4) + D);
+    A = fmaxf(A, e[i].x);
+    M = fmaxf(M, e[i].y);
+  }
+  float x[V], l = 0.f;
+#pragma unroll
+  for (int d = 0; d < V; d++) x[d] = 0.f;
+#pragma unroll
+  for (int i = 0; i < MOST_PARTS; i++) {
+    if (i < parts) {
+      const float* src = a.partial + (i * rows + at) * (D + 4) + lane * V;
+      const float wo = ex2f(e[i].x - A), wl = ex2f(e[i].y - M);
+      l = fmaf(e[i].z, wl, l);
+#pragma unroll
+      for (int d = 0; d < V; d += 2) {
+        const float2 y = *(const float2*)(src + d);
+        x[d] = fmaf(y.x, wo, x[d]);
+        x[d + 1] = fmaf(y.y, wo, x[d + 1]);
+      }
+    }
+  }
+  const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
+  __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (long long)row * a.o.st + (long long)head * a.o.sh + lane * V;
+#pragma unroll
+  for (int d = 0; d < V; d += 2) *(uint32_t*)(dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+}
+
 template <int D, bool E4M3>
-cudaError_t launch(const KvAttnArgs& a, cudaStream_t stream) {
-  auto kern = kv_attn_tc_kernel<D, E4M3>;
+cudaError_t launch(const KvAttnArgs& a, int parts, cudaStream_t stream, int* launches) {
+  auto kern = parts > 1 ? kv_attn_tc_kernel<D, E4M3, true> : kv_attn_tc_kernel<D, E4M3, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES);
   if (e != cudaSuccess) return e;
   uint32_t *status = nullptr, ticket = 0;
   if (!launch_ticket(stream, &status, &ticket)) return cudaErrorUnknown;
-  const dim3 grid((unsigned)kv_places(a.batch, a.Hq / a.pool.Hkv, 8, 1), (unsigned)a.pool.Hkv);
-  return launch_early(kern, grid, dim3(THREADS), Cfg<D>::BYTES, stream, a, status, ticket);
+  const dim3 grid((unsigned)kv_places(a.batch, a.Hq / a.pool.Hkv, 8, 1), (unsigned)a.pool.Hkv, (unsigned)parts);
+  e = launch_early(kern, grid, dim3(THREADS), Cfg<D>::BYTES, stream, a, status, ticket);
+  if (e != cudaSuccess) return e;
+  ++*launches;
+  if (parts > 1) {
+    e = launch_early(kv_join_rows_kernel<D>, dim3((unsigned)(((long long)a.batch.T * a.Hq + 7) / 8)), dim3(256), 0, stream, a, parts);
+    if (e == cudaSuccess) ++*launches;
+  }
+  return e;
 }
 
 }  // namespace
 
-cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t stream) {
-  if (a.pool.e4m3) return a.pool.D == 128 ? launch<128, true>(a, stream) : launch<64, true>(a, stream);
-  return a.pool.D == 128 ? launch<128, false>(a, stream) : launch<64, false>(a, stream);
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int parts, cudaStream_t stream, int* launches) {
+  if (a.pool.e4m3) return a.pool.D == 128 ? launch<128, true>(a, parts, stream, launches) : launch<64, true>(a, parts, stream, launches);
+  return a.pool.D == 128 ? launch<128, false>(a, parts, stream, launches) : launch<64, false>(a, parts, stream, launches);
 }
 
 }  // namespace ar

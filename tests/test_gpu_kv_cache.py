@@ -256,11 +256,23 @@ def test_many_rows(ops, fp8, D, page, causal):
         s.check_attention(lengths, new, Hq, causal)
 
 
-def test_many_rows_on_a_long_sequence(ops):
-    s = Setup(ops, 17, [4000, 1000], Hkv=1, D=128, page=64)
-    s.append([4000, 1000], [4000, 1000])
-    s.check_attention([4000, 1000], [70, 33], 4)
-    s.check_attention([4000, 1000], [70, 33], 4, causal=False)
+@pytest.mark.parametrize("fp8,D,page", [(False, 128, 64), (True, 128, 16), (False, 64, 128), (True, 64, 32)])
+def test_many_rows_on_long_sequences(ops, fp8, D, page):
+    """Few row tiles: the keys are divided over CTAs and joined.  Sequences shorter than the parts are many, idle ones, a row
+    that belongs to none."""
+    lengths, new = [4000, 1000, 100, 0], [170, 133, 90, 2]
+    s = Setup(ops, 17 + page, lengths, Hkv=1, D=D, page=page, fp8=fp8)
+    s.append(lengths, lengths)
+    parts, rest = divmod(ops.kv_cache_attention_workspace(s.cache, 395, 4, 4, 4000), 395 * 4 * (D + 4) * 4)
+    assert parts > 1 and rest == 0  # (a row of results for each)
+    for causal in (True, False):
+        s.check_attention(lengths, new, 4, causal, max_length=4000)
+    out = s.torch.full((397, 4, D), 7.0, dtype=s.torch.bfloat16, device="cuda")
+    q, qf = s.rows(397, 4)
+    s.ops.kv_cache_attention(s.cache, q, s.dtable, s.ints(lengths), s.ints([1, 171, 304, 394, 396]), out=out, max_length=4000)
+    want = s.expect(qf[1:396], lengths, np.array([0, 170, 303, 393, 395]), True)
+    assert_attention_close(out[1:396].double().cpu().numpy(), *want, False)
+    assert (out[:1] == 7).all() and (out[396:] == 7).all()
 
 
 def test_rows_of_no_sequence_are_left(ops):
