@@ -412,7 +412,8 @@ def kv_cache(pages: int, kv_heads: int, page: int, D: int, fp8: bool = False, k_
 
 def _kv_batch(cache: KvCache, page_table, lengths, starts, tokens: int) -> _abi.KvBatch:
     dev = cache._device
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev or page_table.stride(1) != 1:
+    strides = page_table.stride()
+    if len(strides) != 2 or page_table.dtype != torch.int32 or page_table.device != dev or strides[1] != 1:
         raise ValueError("page_table must be a [B, pages] int32 tensor on the cache's device with contiguous rows")
     B, width = page_table.shape
     if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != dev or not lengths.is_contiguous():
@@ -423,23 +424,26 @@ def _kv_batch(cache: KvCache, page_table, lengths, starts, tokens: int) -> _abi.
     elif tokens != B:
         raise ValueError(f"without starts every sequence has one token: {tokens} tokens for {B} sequences")
     return _abi.KvBatch(page_table.data_ptr(), lengths.data_ptr(), None if starts is None else starts.data_ptr(),
-                        page_table.stride(0), width, B, tokens)
+                        strides[0], width, B, tokens)
 
 
 _Strides2 = ctypes.c_int64 * 2
+# The handle of torch's current stream on a device, without the Stream object around it (2 us of a call of 15).
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _kv_rows(name: str, t: torch.Tensor, shape, dtype, device):
     """Strides of a packed [T, H, D] view."""
-    if t.shape != shape or t.dtype != dtype or t.device != device or t.stride(2) != 1:
+    strides = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.device != device or strides[2] != 1:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device} with a contiguous last dimension")
-    return _Strides2(t.stride(0), t.stride(1))
+    return _Strides2(strides[0], strides[1])
 
 
 def _kv_call(what: str, fn, cache: KvCache, stream, *args) -> None:
     """The call on `stream` (None: the current one of the cache's device), with that device current."""
     dev = cache._device
-    handle = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
+    handle = stream.cuda_stream if stream is not None else _current_stream(dev.index)
     if torch.cuda.current_device() == dev.index:
         rc = fn(cache._pool, *args, handle)
     else:
@@ -472,14 +476,13 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     views with a contiguous last dimension; rows that belong to no sequence are left as they were."""
     pool, dev, tokens = cache._pool, cache._device, int(tokens)
     shape = (tokens, pool.Hkv, pool.D)
-    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+    k, v = out if out is not None else torch.empty((2, *shape), dtype=dtype, device=dev).unbind()
     code = _dtype_code(k)
     ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, tokens)
     _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
     if stream is not None and out is None:
-        k.record_stream(stream)
-        v.record_stream(stream)
+        k.record_stream(stream)  # (of the memory that both lie in)
     return k, v
 
 
