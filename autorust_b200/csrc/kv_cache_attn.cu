@@ -47,7 +47,6 @@ constexpr int START_UNITS = 9;
 constexpr float P_SHIFT = 12.0f, LAG = 2.0f;
 constexpr int E_LIMIT = 100;    // largest |e - e_ref|
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60, the least scale a page is given
-constexpr int WHOLE_KEYS = 512;  // up to this length a row tile's keys are not cut
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -843,7 +842,7 @@ KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int
   if (dtype != 0 && mean_rows > 16) {
     const double per_group = pool.D == 128 ? 1.45e-3 : 1.1e-3, per_step = pool.D == 128 ? 2.3 : 1.9;
     const double pairs = (double)batch.B * pool.Hkv;
-    const double here = (max_length <= WHOLE_KEYS ? 6.0 : 14.0) +
+    const double here = (max_length <= 512 ? 6.0 : 14.0) +
                         pairs * ((mean_rows + 15) / 16) * ((max_length + GROUP - 1) / GROUP + START_UNITS) * per_group;
     const long long steps = (max_length + 127) / 128, ctas = batch.B * (long long)pool.Hkv * ((mean_rows + 255) / 256);
     auto bytes = [&](long long parts) { return parts > 1 ? sizeof(float) * (size_t)parts * batch.T * Hq * (pool.D + 4) : 0; };
@@ -861,9 +860,18 @@ KvAttnPlan kv_attn_plan(const KvPool& pool, const KvBatch& batch, int dtype, int
       return p;
     }
   }
-  const long long tiles = kv_places(batch, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
+  const long long tiles = batch.B * (long long)pool.Hkv * ((mean_rows + p.rows - 1) / p.rows), groups = (max_length + GROUP - 1) / GROUP;
+  const long long most_tiles = kv_places(batch, G, p.rows == 8 ? 3 : 4, 1) * pool.Hkv;
   p.ctas = SMS * (p.rows == 8 ? Sh<128, 1>::CTAS_PER_SM : Sh<128, 2>::CTAS_PER_SM);
-  if (max_length <= WHOLE_KEYS || tiles >= 16 * p.ctas || tiles * ((max_length + GROUP - 1) / GROUP + START_UNITS) > 0xffffffffll) p.ctas = 0;
+  // Cut or whole, again by estimated times: a step of a whole tile's four warps takes 1.05 us (D = 64: 0.85; f32 tensors and
+  // 16 rows a quarter more), the codes pass at 4.6 TB/s; shares pass them at 6.0 and cost 10.5 us and 35 ns a tile for
+  // being found and joined.  One sequence, 32 / 8 heads, D = 128: 7.7 us whole and 10.7 cut at 512 keys, 36 and 12.6 at
+  // 4096; 32 sequences: 20 and 28 at 1024, 58 and 60 at 4096.
+  const double step = (pool.D == 128 ? 1.05 : 0.85) * (dtype == 0 ? 1.25 : 1.0) * (p.rows == 8 ? 1.0 : 1.25);
+  const double megabytes = 2.0 * pool.D * GROUP * (double)groups * (double)tiles / 1e6;
+  const double whole = 4.0 + std::max((double)((tiles + p.ctas - 1) / p.ctas) * (double)((groups + WARPS - 1) / WARPS) * step, megabytes / 4.6 + 3.0);
+  const double cut = 10.5 + megabytes / 6.0 + 0.035 * (double)tiles;
+  if (whole <= cut || most_tiles * (groups + START_UNITS) > 0xffffffffll) p.ctas = 0;  // (units are 32-bit numbers)
   p.workspace = (size_t)p.ctas * (sizeof(Cut) + 2 * sizeof(float) * p.rows * (pool.D + 4));
   return p;
 }
