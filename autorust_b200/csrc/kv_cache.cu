@@ -30,16 +30,20 @@ int check_batch(const ar_kv_batch* s, const ar::KvPool& pool, ar::KvBatch* out) 
   *out = ar::KvBatch{s->page_table, s->lengths, s->starts, s->table_stride, (int)s->table_pages, (int)s->B, (int)s->T, nullptr};
   return AR_OK;
 }
-// A packed tensor that is read (or, `written`, whose rows must not lie on one another).
-int check_rows(const void* p, const int64_t* strides, int dtype, bool written, ar::KvRows* out) {
+// A packed [T, H, D] tensor that is read (or, `written`, whose rows must not lie on one another).  The stride of an extent of
+// one is not used and may be anything.
+int check_rows(const void* p, const int64_t* strides, int64_t T, int64_t H, int dtype, bool written, ar::KvRows* out) {
   if (!p || !strides) return AR_ERR_NULL;
-  const int64_t size = dtype == AR_DTYPE_F32 ? 4 : 2;
+  const int64_t size = dtype == AR_DTYPE_F32 ? 4 : 2, extent[2] = {T, H};
+  int64_t used[2];
   for (int i = 0; i < 2; i++) {
-    if (strides[i] < 0 || (written && strides[i] == 0)) return AR_ERR_SHAPE;
-    if (strides[i] * size % 16 != 0) return AR_ERR_ALIGNMENT;
+    used[i] = extent[i] == 1 ? 0 : strides[i];
+    if (extent[i] == 1) continue;
+    if (used[i] < 0 || (written && used[i] == 0)) return AR_ERR_SHAPE;
+    if (used[i] * size % 16 != 0) return AR_ERR_ALIGNMENT;
   }
   if (!aligned(p, 16)) return AR_ERR_ALIGNMENT;
-  *out = ar::KvRows{const_cast<void*>(p), strides[0], strides[1]};
+  *out = ar::KvRows{const_cast<void*>(p), used[0], used[1]};
   return AR_OK;
 }
 bool known(int dtype) { return dtype == AR_DTYPE_F32 || dtype == AR_DTYPE_BF16; }
@@ -58,10 +62,10 @@ int move(bool write, const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype
   int rc = check_pool(pool, &p);
   if (rc == AR_OK) rc = check_batch(batch, p, &s);
   if (rc == AR_OK && !known(dtype)) rc = AR_ERR_UNSUPPORTED;
-  if (rc == AR_OK) rc = check_rows(k, k_strides, dtype, !write, &kr);
-  if (rc == AR_OK) rc = check_rows(v, v_strides, dtype, !write, &vr);
+  if (rc != AR_OK || s.T == 0) return rc;
+  rc = check_rows(k, k_strides, s.T, p.Hkv, dtype, !write, &kr);
+  if (rc == AR_OK) rc = check_rows(v, v_strides, s.T, p.Hkv, dtype, !write, &vr);
   if (rc != AR_OK) return rc;
-  if (s.T == 0) return AR_OK;
   rc = ready(&s);
   if (rc != AR_OK) return rc;
   const cudaStream_t stream = (cudaStream_t)cu_stream;
@@ -108,10 +112,10 @@ int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int 
                           int causal, void* workspace, size_t workspace_bytes, void* cu_stream) {
   ar::KvAttnArgs a;
   int rc = check_attention(pool, batch, dtype, Hq, max_length, &a.pool, &a.batch);
-  if (rc == AR_OK) rc = check_rows(q, q_strides, dtype, false, &a.q);
-  if (rc == AR_OK) rc = check_rows(o, o_strides, dtype, true, &a.o);
+  if (rc != AR_OK || a.batch.T == 0) return rc;
+  rc = check_rows(q, q_strides, a.batch.T, Hq, dtype, false, &a.q);
+  if (rc == AR_OK) rc = check_rows(o, o_strides, a.batch.T, Hq, dtype, true, &a.o);
   if (rc != AR_OK) return rc;
-  if (a.batch.T == 0) return AR_OK;
   a.dtype = dtype;
   a.Hq = (int)Hq;
   a.max_length = (int)max_length;

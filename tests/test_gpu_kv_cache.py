@@ -513,3 +513,81 @@ def test_same_call_same_bits(ops):
     first = s.ops.kv_cache_attention(s.cache, q, *where)
     for _ in range(5):
         assert torch.equal(first, s.ops.kv_cache_attention(s.cache, q, *where))
+
+
+def test_many_rows_captured(ops):
+    """The tensor-core kernel, whole and in parts, captured between an append and a read and replayed on other tokens."""
+    import torch
+    for lengths, new, heads in (([500, 300], [200, 130], 8), ([3000, 200], [300, 150], 4)):
+        s = Setup(ops, 97, lengths, Hkv=2, D=64, page=32)
+        s.append([x - n for x, n in zip(lengths, new)], [x - n for x, n in zip(lengths, new)])
+        T = sum(new)
+        starts, where = s.batch(lengths, new)
+        k, v, q = s.rows(T, 2)[0].clone(), s.rows(T, 2)[0].clone(), s.rows(T, heads)[0].clone()
+        need = s.ops.kv_cache_attention_workspace(s.cache, T, heads, 2, max(lengths))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+
+        def step():
+            s.ops.kv_cache_append(s.cache, k, v, *where)
+            o = s.ops.kv_cache_attention(s.cache, q, *where, max_length=max(lengths), workspace=ws)
+            return o, s.ops.kv_cache_read(s.cache, *where, T)
+
+        step()
+        graph = torch.cuda.CUDAGraph()
+        saved = [x.clone() for x in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale)]
+        with torch.cuda.graph(graph):
+            o, (rk, rv) = step()
+        for _ in range(3):
+            for x, H in ((k, 2), (v, 2), (q, heads)):
+                x.copy_(s.rows(T, H)[0])
+            for x, y in zip((s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale), saved):
+                x.copy_(y)
+            graph.replay()
+            got = [x.clone() for x in (o, rk, rv)]
+            for x, y in zip((s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale), saved):
+                x.copy_(y)
+            eager, (ek, ev) = step()
+            for x, y in zip(got, (eager, ek, ev)):
+                assert torch.equal(x, y)
+        assert ops.last_status(None) == 0
+
+
+def test_a_pool_beyond_32_bit_offsets(ops):
+    """Pages whose codes lie more than 2^32 bytes into the pool, and rows of packed tensors that do so too."""
+    import torch
+    Hkv, page, D = 8, 128, 128
+    pages = (5 << 30) // (Hkv * page * D)
+    cache = ops.kv_cache(pages, Hkv, page, D)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = ints([[pages - 1, 0, pages - 2], [pages // 2, pages - 3, 1]])
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = [300, 129]
+    T, wide = sum(n), 5_100_000  # elements between the rows: the last one lies 4.4 GB behind the first
+    big = torch.empty((T - 1) * wide + 2 * Hkv * D, dtype=torch.bfloat16, device="cuda")
+    k, v = (torch.as_strided(big, (T, Hkv, D), (wide, D, 1), i * Hkv * D) for i in range(2))
+    rows = torch.randn(2, T, Hkv, D, device="cuda", generator=g).to(torch.bfloat16)
+    k.copy_(rows[0]); v.copy_(rows[1])
+    where = (table, ints(n), ints([0, n[0], T]))
+    ops.kv_cache_append(cache, k, v, *where)
+    small = ops.kv_cache(8, Hkv, page, D)
+    near = (ints([[5, 0, 2], [3, 7, 1]]), *where[1:])
+    ops.kv_cache_append(small, rows[0], rows[1], *near)
+    for far, close in zip(ops.kv_cache_read(cache, *where, T), ops.kv_cache_read(small, *near, T)):
+        assert torch.equal(far, close)
+    for m in (1, 40):
+        q = torch.randn(2 * m, 16, D, device="cuda", generator=g).to(torch.bfloat16)
+        out = torch.as_strided(big, (2 * m, 16, D), (wide * (T // (2 * m)) // 8 * 8 if m == 1 else wide, D, 1))
+        few = ints([0, m, 2 * m])
+        want = ops.kv_cache_attention(small, q, near[0], near[1], few)
+        assert torch.equal(ops.kv_cache_attention(cache, q, table, near[1], few, out=out), want)
+    assert ops.last_status(None) == 0
+
+
+def test_empty_calls(ops):
+    import torch
+    s = Setup(ops, 99, [10], Hkv=1, D=64)
+    none = torch.empty(0, 1, 64, dtype=torch.bfloat16, device="cuda")
+    where = (s.dtable, s.ints([10]), s.ints([0, 0]))
+    s.ops.kv_cache_append(s.cache, none, none, *where)
+    assert s.ops.kv_cache_read(s.cache, *where, 0)[0].shape == (0, 1, 64)
+    assert s.ops.kv_cache_attention(s.cache, none, *where).shape == (0, 1, 64)

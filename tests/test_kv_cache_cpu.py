@@ -77,6 +77,18 @@ def test_refusals_of_single_calls(attn_lib):
 
 def test_no_rows_is_no_work(attn_lib):
     assert calls(attn_lib, pool(), batch(T=0)) == [_abi.AR_OK] * 3
+    assert calls(attn_lib, pool(), batch(T=0), x=None, y=None) == [_abi.AR_OK] * 3  # (an empty tensor has no address)
+    assert calls(attn_lib, pool(), batch(T=0), dtype=7) == [_abi.AR_ERR_UNSUPPORTED] * 3
+
+
+def test_the_stride_of_a_single_row_or_head_is_not_looked_at(attn_lib):
+    import torch
+    ok = _abi.AR_ERR_NO_DEVICE if not torch.cuda.is_available() else None
+    one = batch(B=1, T=1, starts=None)
+    for sx in ((3, 128), (0, 128), (-7, 128)):
+        if ok is not None:
+            assert calls(attn_lib, pool(), one, sx=sx, sy=sx) == [ok] * 3
+    assert calls(attn_lib, pool(), one, sx=(256, 3)) == [_abi.AR_ERR_ALIGNMENT] * 3
 
 
 def test_no_device_is_an_error(attn_lib):
