@@ -146,47 +146,54 @@ __device__ __forceinline__ Span span_of(const KvPool& pool, const KvBatch& batch
   return s;
 }
 
-// E values of a page and head, E / 32 threads; heads blockIdx.y, blockIdx.y + gridDim.y, ...
-template <int E, bool E4M3, bool F32>
+// E = page * D values of a page and head, E / 32 threads; heads blockIdx.y, blockIdx.y + gridDim.y, ...  A thread has the same 8 channels
+// of every TOKENS-th token.
+template <int E, int D, bool E4M3, bool F32>
 __global__ void __launch_bounds__(E / PER_THREAD, E == 16384 ? 1 : (F32 ? 512 : 768) * PER_THREAD / E)
 kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
-  constexpr int THREADS = E / PER_THREAD;
+  constexpr int THREADS = E / PER_THREAD, TOKENS = THREADS * 8 / D;
   __shared__ uint32_t tops[2][THREADS / 32];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int d_log2 = pool.D == 128 ? 7 : 6;
   const Span span = span_of(pool, batch);
   if (span.page < 0) return;
   const bool is_v = blockIdx.z != 0;
-  const KvRows& rows = is_v ? vr : kr;
-  uint8_t* page_codes = (is_v ? pool.v : pool.k) + (long long)span.page * pool.Hkv * E;
+  const KvRows rows{is_v ? vr.p : kr.p, is_v ? vr.st : kr.st, is_v ? vr.sh : kr.sh};
+  const int t = threadIdx.x * 8 / D, d = threadIdx.x * 8 % D;
+  const long long first_row = (span.row0 + t) * rows.st + d, step = TOKENS * rows.st;
+  bool in[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; i++) in[i] = t + i * TOKENS >= span.t0 && t + i * TOKENS < span.t1;
+  uint8_t* codes = (is_v ? pool.v : pool.k) + (long long)span.page * pool.Hkv * E;
   float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)span.page * pool.Hkv;
+  const float* means = is_v ? nullptr : pool.k_mean;
   Raw<F32> raw[VECS];
   float next_s0 = 0.f;
   auto fetch = [&](int h) {
     if (h >= pool.Hkv) return;
     if (span.t0 > 0) next_s0 = scales[h];
+    const long long at = first_row + (long long)h * rows.sh;
 #pragma unroll
-    for (int i = 0; i < VECS; i++) {
-      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
-      if (t >= span.t0 && t < span.t1) raw[i] = load8<F32>(rows.p, (span.row0 + t) * rows.st + (long long)h * rows.sh + d);
-    }
+    for (int i = 0; i < VECS; i++)
+      if (in[i]) raw[i] = load8<F32>(rows.p, at + i * step);
   };
   fetch(blockIdx.y);
   for (int h = blockIdx.y, n = 0; h < pool.Hkv; h += gridDim.y, n ^= 1) {
-    const float* mean = !is_v && pool.k_mean ? pool.k_mean + h * pool.D : nullptr;
     const float s0 = next_s0;
     float x[VECS][8];
     float most = 0.f;
+    float4 ma, mb;
+    if (means) {
+      ma = *(const float4*)(means + h * D + d);
+      mb = *(const float4*)(means + h * D + d + 4);
+    }
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
-      if (t >= span.t0 && t < span.t1) {
+      if (in[i]) {
         values8<F32>(raw[i], x[i]);
-        if (mean) {
-          const float4 a = *(const float4*)(mean + d), b = *(const float4*)(mean + d + 4);
-          x[i][0] -= a.x; x[i][1] -= a.y; x[i][2] -= a.z; x[i][3] -= a.w;
-          x[i][4] -= b.x; x[i][5] -= b.y; x[i][6] -= b.z; x[i][7] -= b.w;
+        if (means) {
+          x[i][0] -= ma.x; x[i][1] -= ma.y; x[i][2] -= ma.z; x[i][3] -= ma.w;
+          x[i][4] -= mb.x; x[i][5] -= mb.y; x[i][6] -= mb.z; x[i][7] -= mb.w;
         }
 #pragma unroll
         for (int c = 0; c < 8; c++) most = max_abs_nan(most, x[i][c]);
@@ -202,93 +209,108 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
     } else {
       __syncwarp();
     }
-    uint8_t* codes = page_codes + (long long)h * E;
+    uint8_t* to = codes + (long long)h * E + threadIdx.x * 8;
     float s = scale_of<E4M3>(top);
     if (span.t0 > 0 && !(s > s0) && s == s) s = s0;  // (a NaN on either side stays)
     const bool dead = s != s;
     const float inverse = 1.0f / s;
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
-      if (t >= span.t0 && t < span.t1) {
+      if (in[i]) {
         float y[8];
 #pragma unroll
         for (int c = 0; c < 8; c++) y[c] = __fmul_rn(x[i][c], inverse);
-        *(uint2*)(codes + e) = encode8<E4M3>(y, dead);
+        *(uint2*)(to + i * THREADS * 8) = encode8<E4M3>(y, dead);
       }
     }
     if (span.t0 > 0 && s > s0) {  // the scale has grown: the earlier codes move to it
       const float ratio = s0 / s;
-      for (int e = threadIdx.x * 8; e < (span.t0 << d_log2); e += THREADS * 8) {
+#pragma unroll 1
+      for (int i = 0; i < VECS; i++) {
+        if (t + i * TOKENS >= span.t0) break;
         float y[8];
-        decode8<E4M3>(*(const uint2*)(codes + e), y);
+        decode8<E4M3>(*(const uint2*)(to + i * THREADS * 8), y);
 #pragma unroll
         for (int c = 0; c < 8; c++) y[c] = __fmul_rn(y[c], ratio);
-        *(uint2*)(codes + e) = encode8<E4M3>(y, false);
+        *(uint2*)(to + i * THREADS * 8) = encode8<E4M3>(y, false);
       }
     }
     if (threadIdx.x == 0) scales[h] = s;
   }
 }
 
-template <int E, bool E4M3, bool F32>
+template <int E, int D, bool E4M3, bool F32>
 __global__ void __launch_bounds__(E / PER_THREAD)
 kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
-  constexpr int THREADS = E / PER_THREAD;
+  constexpr int THREADS = E / PER_THREAD, TOKENS = THREADS * 8 / D;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int d_log2 = pool.D == 128 ? 7 : 6;
   const Span span = span_of(pool, batch);
   const bool is_v = blockIdx.z != 0;
-  const KvRows& rows = is_v ? vr : kr;
+  const KvRows rows{is_v ? vr.p : kr.p, is_v ? vr.st : kr.st, is_v ? vr.sh : kr.sh};
+  const int t = threadIdx.x * 8 / D, d = threadIdx.x * 8 % D;
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (span.padding > 0) {
     for (int h = blockIdx.y; h < pool.Hkv; h += gridDim.y)
-      for (long long e = threadIdx.x * 8; e < ((long long)span.padding << d_log2); e += THREADS * 8)
-        store8<F32>(rows.p, (span.pad_row + (e >> d_log2)) * rows.st + (long long)h * rows.sh + (e & (pool.D - 1)), zero);
+      for (int r = t; r < span.padding; r += TOKENS) store8<F32>(rows.p, (span.pad_row + r) * rows.st + (long long)h * rows.sh + d, zero);
   }
   if (span.t1 <= span.t0) return;
-  const uint8_t* page_codes = (is_v ? pool.v : pool.k) + (long long)max(span.page, 0) * pool.Hkv * E;
-  const float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)max(span.page, 0) * pool.Hkv;
+  const long long first_row = (span.row0 + t) * rows.st + d, step = TOKENS * rows.st;
+  bool in[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; i++) in[i] = t + i * TOKENS >= span.t0 && t + i * TOKENS < span.t1;
+  if (span.page < 0) {  // reported
+    for (int h = blockIdx.y; h < pool.Hkv; h += gridDim.y)
+#pragma unroll
+      for (int i = 0; i < VECS; i++)
+        if (in[i]) store8<F32>(rows.p, first_row + i * step + (long long)h * rows.sh, zero);
+    return;
+  }
+  const uint8_t* codes = (is_v ? pool.v : pool.k) + (long long)span.page * pool.Hkv * E + threadIdx.x * 8;
+  const float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)span.page * pool.Hkv;
+  const float* means = is_v ? nullptr : pool.k_mean;
   uint2 w[VECS];
   float next_s = 0.f;
   auto fetch = [&](int h) {
     if (h >= pool.Hkv) return;
     next_s = scales[h];
 #pragma unroll
-    for (int i = 0; i < VECS; i++) {
-      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2;
-      if (t >= span.t0 && t < span.t1) w[i] = *(const uint2*)(page_codes + (long long)h * E + e);
-    }
+    for (int i = 0; i < VECS; i++)
+      if (in[i]) w[i] = *(const uint2*)(codes + (long long)h * E + i * THREADS * 8);
   };
   fetch(blockIdx.y);
   for (int h = blockIdx.y; h < pool.Hkv; h += gridDim.y) {
-    const float* mean = !is_v && pool.k_mean && span.page >= 0 ? pool.k_mean + h * pool.D : nullptr;
     const float s = next_s;
+    float mean[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (means) {
+      const float4 a = *(const float4*)(means + h * D + d), b = *(const float4*)(means + h * D + d + 4);
+      mean[0] = a.x; mean[1] = a.y; mean[2] = a.z; mean[3] = a.w;
+      mean[4] = b.x; mean[5] = b.y; mean[6] = b.z; mean[7] = b.w;
+    }
     uint2 now[VECS];
 #pragma unroll
     for (int i = 0; i < VECS; i++) now[i] = w[i];
     fetch(h + gridDim.y);
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-      const int e = (i * THREADS + threadIdx.x) * 8, t = e >> d_log2, d = e & (pool.D - 1);
-      if (t >= span.t0 && t < span.t1) {
+      if (in[i]) {
         float x[8];
         decode8<E4M3>(now[i], x);
 #pragma unroll
-        for (int c = 0; c < 8; c++) x[c] = span.page < 0 ? 0.f : x[c] * s;
-        if (mean) {
+        for (int c = 0; c < 8; c++) x[c] *= s;
+        if (means) {
 #pragma unroll
-          for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[d + c]);  // (not contracted: the definition rounds the product)
+          for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[c]);  // (not contracted: the definition rounds the product)
         }
-        store8<F32>(rows.p, (span.row0 + t) * rows.st + (long long)h * rows.sh + d, x);
+        store8<F32>(rows.p, first_row + i * step + (long long)h * rows.sh, x);
       }
     }
   }
 }
 
-// CTAs up to which every head of a page gets one of its own: 16 per SM.
-constexpr int SPREAD_CTAS = 16 * 148;
+// CTAs up to which every head of a page gets one of its own: 8 per SM (32768 tokens written and read back: 62 + 56 us with 32, 50 + 46
+// with 16, 49 + 44 with 8, 50 + 43 with 4).
+constexpr int SPREAD_CTAS = 8 * 148;
 
 template <bool WRITE, bool E4M3, bool F32>
 cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, const KvRows& v, cudaStream_t stream) {
@@ -296,13 +318,21 @@ cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, co
   const long long per_cta = std::max(1ll, std::min((long long)pool.Hkv, places * pool.Hkv * 2 / SPREAD_CTAS));  // heads
   const dim3 grid((unsigned)places, (unsigned)((pool.Hkv + per_cta - 1) / per_cta), 2);
   auto go = [&](auto kern, int E) { return launch_early(kern, grid, dim3(E / PER_THREAD), 0, stream, pool, batch, k, v); };
-#define AR_KV_E(E) (WRITE ? go(kv_append_kernel<E, E4M3, F32>, E) : go(kv_read_kernel<E, E4M3, F32>, E))
-  switch (pool.D << pool.page_log2) {
-    case 1024: return AR_KV_E(1024);
-    case 2048: return AR_KV_E(2048);
-    case 4096: return AR_KV_E(4096);
-    case 8192: return AR_KV_E(8192);
-    case 16384: return AR_KV_E(16384);
+#define AR_KV_E(E, D) (WRITE ? go(kv_append_kernel<E, D, E4M3, F32>, E) : go(kv_read_kernel<E, D, E4M3, F32>, E))
+  if (pool.D == 128) {
+    switch (pool.page_log2) {
+      case 4: return AR_KV_E(2048, 128);
+      case 5: return AR_KV_E(4096, 128);
+      case 6: return AR_KV_E(8192, 128);
+      case 7: return AR_KV_E(16384, 128);
+    }
+  } else {
+    switch (pool.page_log2) {
+      case 4: return AR_KV_E(1024, 64);
+      case 5: return AR_KV_E(2048, 64);
+      case 6: return AR_KV_E(4096, 64);
+      case 7: return AR_KV_E(8192, 64);
+    }
   }
 #undef AR_KV_E
   return cudaErrorInvalidValue;
