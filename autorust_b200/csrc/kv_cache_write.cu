@@ -11,6 +11,7 @@
 // are the two halves of grid.z.
 #include <cuda_bf16.h>
 
+#include "ar_ptx.cuh"
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -80,10 +81,11 @@ __device__ __forceinline__ uint2 encode8(const float (&y)[8], bool dead) {
     if constexpr (E4M3) {
       w[i] = e4m3_codes(v[0], v[1]) | e4m3_codes(v[2], v[3]) << 16;
     } else {  // 1.5 * 2^23 + y, rounded to nearest even, has the code in its low byte
-      uint32_t u[4];
+      float u[4];
 #pragma unroll
-      for (int c = 0; c < 4; c++) u[c] = __float_as_uint(__fadd_rn(v[c], 12582912.0f));
-      w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+      for (int c = 0; c < 4; c++) u[c] = __fadd_rn(v[c], 12582912.0f);
+      w[i] = __byte_perm(__byte_perm(__float_as_uint(u[0]), __float_as_uint(u[1]), 0x0040),
+                         __byte_perm(__float_as_uint(u[2]), __float_as_uint(u[3]), 0x0040), 0x5410);
     }
     if (dead) w[i] = 0u;
   }
@@ -100,11 +102,18 @@ __device__ __forceinline__ void decode8(const uint2& w, float (&x)[8]) {
     x[4 + i] = hi[i];
   }
 }
-// max(a, |b|), NaN if either is.
-__device__ __forceinline__ float max_abs_nan(float a, float b) {
+// max(|a|, |b|, |c|), NaN if one is.
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+// Two values at a time.  (Sums of these products are taken one by one: a packed product and a packed sum behind it become one
+// multiply-add, which rounds once where the definition rounds twice.)
+__device__ __forceinline__ void scale8(const float (&x)[8], float by, float (&y)[8]) {
+  const uint64_t by2 = arptx::pack_f32x2(by, by);
+#pragma unroll
+  for (int c = 0; c < 8; c += 2) arptx::unpack_f32x2(arptx::mul_f32x2(arptx::pack_f32x2(x[c], x[c + 1]), by2), y[c], y[c + 1]);
 }
 
 // The scale of a largest magnitude given by its bits (infinities and NaN are the largest patterns).
@@ -192,11 +201,14 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
       if (in[i]) {
         values8<F32>(raw[i], x[i]);
         if (means) {
-          x[i][0] -= ma.x; x[i][1] -= ma.y; x[i][2] -= ma.z; x[i][3] -= ma.w;
-          x[i][4] -= mb.x; x[i][5] -= mb.y; x[i][6] -= mb.z; x[i][7] -= mb.w;
+          const float off[8] = {-ma.x, -ma.y, -ma.z, -ma.w, -mb.x, -mb.y, -mb.z, -mb.w};
+#pragma unroll
+          for (int c = 0; c < 8; c += 2)
+            arptx::unpack_f32x2(arptx::add_f32x2(arptx::pack_f32x2(x[i][c], x[i][c + 1]), arptx::pack_f32x2(off[c], off[c + 1])), x[i][c],
+                                x[i][c + 1]);
         }
 #pragma unroll
-        for (int c = 0; c < 8; c++) most = max_abs_nan(most, x[i][c]);
+        for (int c = 0; c < 8; c += 2) most = max_abs_nan(most, x[i][c], x[i][c + 1]);
       }
     }
     fetch(h + gridDim.y);
@@ -204,8 +216,7 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
     if constexpr (THREADS > 32) {
       if ((threadIdx.x & 31) == 0) tops[n][threadIdx.x >> 5] = top;
       __syncthreads();  // (the other half of tops is written before the next one: no second barrier)
-#pragma unroll
-      for (int i = 0; i < THREADS / 32; i++) top = max(top, tops[n][i]);
+      top = __reduce_max_sync(0xffffffffu, tops[n][threadIdx.x & (THREADS / 32 - 1)]);
     } else {
       __syncwarp();
     }
@@ -218,8 +229,7 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
     for (int i = 0; i < VECS; i++) {
       if (in[i]) {
         float y[8];
-#pragma unroll
-        for (int c = 0; c < 8; c++) y[c] = __fmul_rn(x[i][c], inverse);
+        scale8(x[i], inverse, y);
         *(uint2*)(to + i * THREADS * 8) = encode8<E4M3>(y, dead);
       }
     }
@@ -230,8 +240,7 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
         if (t + i * TOKENS >= span.t0) break;
         float y[8];
         decode8<E4M3>(*(const uint2*)(to + i * THREADS * 8), y);
-#pragma unroll
-        for (int c = 0; c < 8; c++) y[c] = __fmul_rn(y[c], ratio);
+        scale8(y, ratio, y);
         *(uint2*)(to + i * THREADS * 8) = encode8<E4M3>(y, false);
       }
     }
@@ -296,11 +305,10 @@ kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const Kv
       if (in[i]) {
         float x[8];
         decode8<E4M3>(now[i], x);
-#pragma unroll
-        for (int c = 0; c < 8; c++) x[c] *= s;
+        scale8(x, s, x);
         if (means) {
 #pragma unroll
-          for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[c]);  // (not contracted: the definition rounds the product)
+          for (int c = 0; c < 8; c++) x[c] = __fadd_rn(x[c], mean[c]);
         }
         store8<F32>(rows.p, first_row + i * step + (long long)h * rows.sh, x);
       }
