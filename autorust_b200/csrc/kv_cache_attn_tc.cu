@@ -20,12 +20,16 @@
 // scores.  Step i of tile t: P_t(i) done -> O_t += P_t(i) V(i), then S_t(i + 2) = Q_t K(i + 2) into the same buffer.
 // A row's O may be rescaled only when no PV of its tile is under way: the softmax waits for the last one then, which is rare.
 //
-// Measured, 2 x 1024 rows x 4 heads against 16384 keys, D = 128: S in one buffer of 128 keys 643 us, every unit below 40 % -- the rows
-// waited.  (A quarter of the exponentials as polynomials, as in the bf16 forward, changed that by 1 %.)
+// Measured, 2 x 1024 rows x 4 heads against 16384 keys, D = 128: 576 us, 924 TFLOP/s.  S in one buffer of 128 keys took 643 us with one
+// issuer and 674 with two.  With the softmax and the producers switched off (a scratch build) the MMAs and their hand-overs
+// alone take 555: a step's 48 MMAs 85 clocks each, against 32 to 64 of arithmetic.  A buffer's round -- PV and QK of both tiles
+// 1400 clocks, the way to the softmax 300, the softmax 1700, the way back 300 -- is what a step waits for; TMEM has room for two
+// buffers per tile and no more.
 #include <cuda_bf16.h>
 
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
+#include "softmax_math.cuh"
 #include "softmax_math.cuh"
 
 #include <type_traits>
@@ -48,6 +52,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -1e30f;            // where a row's maximum starts; a hidden key is -inf
 constexpr float P_SHIFT = 8.0f, LAG = 6.0f;  // P < 2^14: inside f16, and a weight 2^-22 of the largest still a normal number
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60
+// Of 8 pairs of columns, those whose exponentials are the polynomial's (1.1e-4, below P's rounding to f16): the two tiles'
+// softmax steps mostly fall together and share the MUFU (none 600 us of the case above, a quarter 576, three eighths 578, half 593).
+constexpr uint32_t POLY_MASK = 0x88u;
 
 template <int D>
 struct Cfg {
@@ -470,7 +477,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           for (int k = 0; k < 8; k++) {
             const int at = b2 * 16 + 2 * k;
             float p0, p1;
-            exp2_mufu_x2(fma_f32x2(pack_f32x2(__uint_as_float(sv[hf][at]), __uint_as_float(sv[hf][at + 1])), c2, add2), p0, p1);
+            const uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sv[hf][at]), __uint_as_float(sv[hf][at + 1])), c2, add2);
+            if (!EDGE && ((POLY_MASK >> k) & 1u))
+              exp2_poly_x2(x2, p0, p1);
+            else
+              exp2_mufu_x2(x2, p0, p1);
             if constexpr (EDGE) {
               if (hf * 32 + at >= first_out) p0 = 0.f;
               if (hf * 32 + at + 1 >= first_out) p1 = 0.f;
