@@ -30,7 +30,6 @@
 #include "ar_ptx.cuh"
 #include "kv_cache.cuh"
 #include "softmax_math.cuh"
-#include "softmax_math.cuh"
 
 #include <type_traits>
 
