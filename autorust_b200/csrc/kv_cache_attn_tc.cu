@@ -39,7 +39,7 @@ using namespace arptx;
 
 #ifdef AR_WAIT_TEST
 __device__ int g_test_skip_cache_tile = -1;
-__device__ int g_test_late_ns[2] = {0, 0};
+__device__ int g_test_late_ns[3] = {0, 0, 0};
 #endif
 
 constexpr int BM = 128, BN = 128, HALF = 64, TILES = 2, ROWS = BM * TILES;
@@ -62,7 +62,7 @@ struct Cfg {
   static constexpr int BOX = BN * 128;               // bytes: 128 rows of 64 channels
   static constexpr int TILE = BN * D * 2;            // of Q, K or V
   static constexpr int SCALE_RING = 4;               // tiles whose scales are kept
-  static constexpr int NUM_BARS = 2 + 4 * STAGES + 4 + 4 + 2;
+  static constexpr int NUM_BARS = 2 + 4 * STAGES + 4 + 4 + 4;
   static constexpr int SCALES = (TILES + 2 * STAGES) * TILE;
   static constexpr int BARS = SCALES + SCALE_RING * 3 * BLOCKS * 4;
   static constexpr int BYTES = BARS + NUM_BARS * 8 + 16 + 1024;
@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   uint64_t* v_empty = v_full + ST;
   uint64_t* s_full = v_empty + ST;     // [tile][buffer]
   uint64_t* p_full = s_full + 4;       // [tile][buffer]
-  uint64_t* pv_done = p_full + 4;      // [2]
-  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
+  uint64_t* pv_done = p_full + 4;      // [tile][buffer], each for one PV: the last of its buffer
+  uint32_t* tmem_slot = (uint32_t*)(pv_done + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   const WaitCtx wctx{abort_flag, status, a.batch.sticky, ticket};
 
@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         mbar_init(&s_full[2 * i + 1], 1);
         mbar_init(&p_full[2 * i], 4);
         mbar_init(&p_full[2 * i + 1], 4);
-        mbar_init(&pv_done[i], 1);
+        mbar_init(&pv_done[2 * i], 1);
+        mbar_init(&pv_done[2 * i + 1], 1);
       }
       for (int i = 0; i < ST; i++) {
         mbar_init(&k_full[i], 4);
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
             issue_qk(i + 2);
             commit_one(&s_full[2 * t + buf]);
           } else {
-            commit_one(&pv_done[t]);
+            commit_one(&pv_done[2 * t + buf]);
           }
         }
         if (buf == 1) {
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         l *= alpha;
         if (i > 0) {  // PV(i - 1) is done when S(i + 1), issued after it, is there; behind the last scores it reports itself
           const bool last = i + 1 == nh[t];
-          uint64_t* bar = last ? &pv_done[t] : &s_full[2 * t + ((i + 1) & 1)];
+          uint64_t* bar = (last ? pv_done : s_full) + 2 * t + ((i + 1) & 1);
           if (!__all_sync(0xffffffffu, mbar_wait(bar, last ? 0 : ((i + 1) >> 1) & 1, wctx, 0x59))) return false;
           tc_fence_after();
           const uint64_t alpha2 = pack_f32x2(alpha, alpha);
@@ -504,14 +505,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     for (int i = 0; i < nh[t]; i++) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (i & 1)], (i >> 1) & 1, wctx, 0x57));
       if (!ok) break;
+#ifdef AR_WAIT_TEST
+      if (g_test_late_ns[2] > 0) __nanosleep(g_test_late_ns[2]);  // Test build only: every step comes late, as do the last products.
+#endif
       tc_fence_after();
       ok = kb + i * HALF + HALF > low[t] || kb + i * HALF + HALF > end ? step(std::true_type{}, i) : step(std::false_type{}, i);
       if (!ok) break;
     }
     if (ok && nh[t] > 0) {
-      // the last two PV report: both may be under way, and a parity tells one phase from the next only
-      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], 0, wctx, 0x58));
-      if (nh[t] > 1) ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_done[t], 1, wctx, 0x58));
+#ifdef AR_WAIT_TEST
+      if (g_test_late_ns[2] > 0) __nanosleep(g_test_late_ns[2]);
+#endif
+      // the last two PV report on a barrier each: both may be under way or done, and a parity does not count phases
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[2 * t + ((nh[t] - 1) & 1)], 0, wctx, 0x58));
+      if (nh[t] > 1) ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_done[2 * t + (nh[t] & 1)], 0, wctx, 0x58));
       tc_fence_after();
     }
     if (ok) {
@@ -629,12 +636,13 @@ cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int parts, cudaStream_t 
 }  // namespace ar
 
 #ifdef AR_WAIT_TEST
-// Test build only: which tile of keys the producers leave out, -1 for none; by how many nanoseconds those of K and V come late.
+// Test build only: which tile of keys the producers leave out, -1 for none; by how many nanoseconds those of K and V, and the rows at their end,
+// come late.
 extern "C" int ar_test_skip_cache_tile(int j) {
   return (int)cudaMemcpyToSymbol(ar::g_test_skip_cache_tile, &j, sizeof(int));
 }
-extern "C" int ar_test_late_cache_tiles(int k_ns, int v_ns) {
-  const int ns[2] = {k_ns, v_ns};
+extern "C" int ar_test_late_cache_tiles(int k_ns, int v_ns, int rows_ns) {
+  const int ns[3] = {k_ns, v_ns, rows_ns};
   return (int)cudaMemcpyToSymbol(ar::g_test_late_ns, ns, sizeof(ns));
 }
 #endif

@@ -1,5 +1,5 @@
 """The waits of the cache attention's tensor-core kernel, in the second build of the library (lib/waittest: a wait budget of about a
-millisecond, and hooks that make tiles late or leave one out).  Tiles that come late change no bit of the result: whoever
+millisecond, and hooks that make tiles or rows late or leave a tile out).  Tiles and rows that come late change no bit of the result: whoever
 depends on one waits for it.  A tile that never comes ends the launch in order: the host reads AR_ERR_DEVICE_WAIT, later CTAs
 leave at once, and the next launch on the same GPU gives the bits of the launch before.  In a child process, so that the
 two libraries never meet in one address space."""
@@ -44,11 +44,11 @@ CHILD = textwrap.dedent('''
         run = lambda: ops.kv_cache_attention(cache, q, table, lengths, few)
         want = run()
         assert ops.last_status(None) == _abi.AR_OK
-        for late in ((5000, 0), (0, 5000), (3000, 3000), (20000, 1000)):
+        for late in ((5000, 0, 0), (0, 5000, 0), (3000, 3000, 0), (20000, 1000, 0), (0, 0, 5000), (0, 0, 20000)):
             assert L.ar_test_late_cache_tiles(*late) == 0
             assert torch.equal(run(), want), late
             assert ops.last_status(None) == _abi.AR_OK
-        assert L.ar_test_late_cache_tiles(0, 0) == 0
+        assert L.ar_test_late_cache_tiles(0, 0, 0) == 0
         for tile in (0, 1):
             assert L.ar_test_skip_cache_tile(tile) == 0
             t0 = time.perf_counter()
