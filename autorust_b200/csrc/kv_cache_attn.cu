@@ -12,8 +12,10 @@
 //
 // V scales differ by page, and P in f16 must neither overflow nor vanish: with s_v = 2^e * f, 1 <= f < 2, the exponent joins the
 // logit: x = logit * log2(e) + e - e_ref, u = 2^(x - m + 12), where m follows the maximum of x (it may lag by up to 2, so
-// that accumulators are rescaled rarely) and e_ref is the exponent of the piece's first page; P = u * f < 2^15, and the row
-// sum takes u * 2^(e_ref - e).  O is then in units of 2^(m - 12 + e_ref), the sum l in units of 2^(m - 12).
+// that accumulators are rescaled rarely) and e_ref is the exponent of the piece's first page, held inside [-5, 20]; P = u * f < 2^15,
+// and the row sum takes u * 2^(e_ref - e).  Scales that an append writes are 2^-60 to 2^121: e - e_ref is then -80 to 126, which
+// leaves the factor and the sums of 2^31 keys normal f32 numbers.  Beside a page of huge values u may vanish where the row's sum needs
+// it: from the first scale above 2^20 on, a warp's groups sum 2^(x - (e - e_ref) - m + 12) instead, exponentials of their own.  O is then in units of 2^(m - 12 + e_ref), the sum l in units of 2^(m - 12).
 //
 // Rows go in tiles of 8: the query heads of one kv head's group next to one another, then the next token.  S = Q K^T has the
 // digits or terms of 8 rows on the 16-row side of the MMA (two digits of the same rows side by side: one thread gets both
@@ -49,7 +51,8 @@ constexpr int LEAST_UNITS = 8;   // of a share
 // warps at its end) takes a CTA about as long as that many groups (64 ragged sequences: 75 us with 4, 66 with 9, 67 with 12).
 constexpr int START_UNITS = 9;
 constexpr float P_SHIFT = 12.0f, LAG = 2.0f;
-constexpr int E_LIMIT = 100;    // largest |e - e_ref|
+constexpr float WIDE = 1048576.0f;  // 2^20
+constexpr int E_REF_LEAST = -5, E_REF_MOST = 20, E_LIMIT = 126;  // the last: largest e - e_ref
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60, the least scale a page is given
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -67,6 +70,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// x * 2^d, d <= 0, where 2^d by itself may be below the f32 numbers and x * 2^d is not.
+__device__ __forceinline__ float times_ex2(float x, float d) { return x * ex2f(fmaxf(d, -100.0f)) * ex2f(fminf(d + 100.0f, 0.0f)); }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
 // The two codes of the low (HI = 0) or high half of w -> f16x2.  INT8 (w with the sign bits flipped, so the bytes are code +
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       const int pg = table[key >> log2];
       return pg >= 0 && pg < a.pool.pages ? pg : -1;
     };
-    // e_ref: the exponent of the piece's first V scale
+    // e_ref: the exponent of the piece's first V scale, but inside limits
     auto exponent_of = [](float s) {  // a NaN keeps its NaN in the factor
       const int e = (int)((__float_as_uint(s) >> 23) & 0xffu) - 127;
       return e == 128 ? 0 : max(e, -60);
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       cp_async_commit();
     };
     look(0);
-    if (page0 >= 0) e_ref = exponent_of(a.pool.v_scale[(long long)page0 * Hkv + h]);
+    if (page0 >= 0) e_ref = min(max(exponent_of(a.pool.v_scale[(long long)page0 * Hkv + h]), E_REF_LEAST), E_REF_MOST);
 #pragma unroll
     for (int it = 0; it < S::STAGES - 1; it++) {
       fetch(it);
@@ -448,7 +453,9 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       l[nt] = 0.f;
     }
 
-    // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out.
+    bool wide = false;  // a V scale above WIDE has been met
+
+    // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out, or V scales are wide apart.
     auto step = [&](auto edge_c, int it) {
       constexpr bool EDGE = decltype(edge_c)::value;
       const uint8_t* kt = ring + (it % S::STAGES) * 2 * S::TILE;
@@ -508,7 +515,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           const int e = exponent_of(sv[blk]);
           const float vs = sv[blk] < SCALE_FLOOR ? SCALE_FLOOR : sv[blk];  // (a NaN stays)
           f[blk] = vs * __uint_as_float((uint32_t)(127 - min(e, 126)) << 23) * (e == 127 ? 0.5f : 1.0f);
-          const int rel = min(max(e - e_ref, -E_LIMIT), E_LIMIT);
+          const int rel = min(e - e_ref, E_LIMIT);
           ex[blk] = (float)rel;
           w_l[blk] = __uint_as_float((uint32_t)(127 - rel) << 23);
         }
@@ -540,8 +547,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const float m_new = fmaxf(m[nt], top);
           const float alpha = m[nt] == -INFINITY ? 0.f : ex2f(m[nt] - m_new);
+          l[nt] = m[nt] == -INFINITY ? l[nt] * 0.f : EDGE ? times_ex2(l[nt], m[nt] - m_new) : l[nt] * alpha;
           m[nt] = m_new;
-          l[nt] *= alpha;
           // the accumulators of this thread are rows 2c and 2c + 1
           const float al[2] = {__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4)};
 #pragma unroll
@@ -561,7 +568,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const float p = ex2f(s[nt][n8][i] - ref);
-            sum[n8 >> 1] += p;
+            sum[n8 >> 1] += EDGE && wide ? ex2f(s[nt][n8][i] - ref - ex[n8 >> 1]) : p;
             s[nt][n8][i] = p * f[n8 >> 1];
             // a row that does not see the key takes 0 * f: a page's NaN must not reach it
             if (EDGE && key0 + n8 * 8 + 2 * c + i >= lim[nt]) s[nt][n8][i] = 0.f;
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           ph[nt][n8] = pack_half2(x0, x1);
           if constexpr (F32) pl[nt][n8] = pack_half2(x0 - half_lo(ph[nt][n8]), x1 - half_hi(ph[nt][n8]));
         }
-        l[nt] += sum[0] * w_l[0] + sum[1] * w_l[1];
+        l[nt] += EDGE && wide ? sum[0] + sum[1] : sum[0] * w_l[0] + sum[1] * w_l[1];
       }
 
       // O^T += V^T P^T, 16 keys per step: tokens 2c, 2c + 1, 2c + 8, 2c + 9, channels 16g .. or 8g ..; tile i has channels 2i, 2i + 1 of those
@@ -608,8 +615,9 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       look(it + S::STAGES);
       cp_async_wait<S::STAGES - 1>();
       __syncwarp();
-      const float* sc = scales + (it % S::STAGES) * 4;
-      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || sc[0] < 0.f || sc[2] < 0.f)
+      const float4 sc = *(const float4*)(scales + (it % S::STAGES) * 4);
+      wide = wide || fmaxf(sc.y, sc.w) > WIDE;
+      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || fminf(sc.x, sc.z) < 0.f || wide)
         step(std::true_type{}, it);
       else
         step(std::false_type{}, it);
@@ -668,10 +676,11 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 #pragma unroll
       for (int v = 0; v < WARPS; v++) {
         if (x[v].x == -INFINITY && x[v].y == 0.f) continue;  // (a row of NaN has no maximum but a NaN sum)
-        const float scale = x[v].x == mm ? 1.0f : ex2f(x[v].x - mm);
+        const bool top = x[v].x == mm;
+        const float scale = top ? 1.0f : ex2f(x[v].x - mm);
         const float4 y = *(const float4*)((const float*)(smem + v * S::RING) + at);
         sum.x += y.x * scale; sum.y += y.y * scale; sum.z += y.z * scale; sum.w += y.w * scale;
-        ll += x[v].y * scale;
+        ll += top ? x[v].y : times_ex2(x[v].y, x[v].x - mm);
       }
       if (direct) {
         const int token = by_g(r0 + r), head = h * G + (r0 + r) - token * G;
@@ -756,8 +765,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
           A_new = fmaxf(A_new, e[i].x);
           M_new = fmaxf(M_new, e[i].y);
         }
-        const float old_o = A == -INFINITY ? 0.f : ex2f(A - A_new), old_l = M == -INFINITY ? 0.f : ex2f(M - M_new);
-        l *= old_l;  // (0 * NaN is wanted: a row of NaN has no maximum)
+        const float old_o = A == -INFINITY ? 0.f : ex2f(A - A_new), old_d = M == -INFINITY ? -INFINITY : M - M_new;
+        l = times_ex2(l, old_d);  // (0 * NaN is wanted: a row of NaN has no maximum)
 #pragma unroll
         for (int d = 0; d < V; d++) x[d] *= old_o;
         A = A_new;
@@ -765,8 +774,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
 #pragma unroll
         for (int i = 0; i < JOIN_STEP; i++) {
           const bool none = e[i].y == -INFINITY && e[i].z == 0.f;
-          const float wo = none || A == -INFINITY ? 0.f : ex2f(e[i].x - A), wl = none || M == -INFINITY ? 0.f : ex2f(e[i].y - M);
-          l += e[i].z * wl;
+          const float wo = none || A == -INFINITY ? 0.f : ex2f(e[i].x - A), wd = none || M == -INFINITY ? -INFINITY : e[i].y - M;
+          l += times_ex2(e[i].z, wd);
 #pragma unroll
           for (int d = 0; d < V; d++) x[d] += y[i][d] * wo;
         }
@@ -787,8 +796,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
     for (int d = 0; d < V; d++) x[d] = 0.f;
     for (int i = 0; i < split; i++) {
       const float4 e = sums[k + i * width];
-      const float wo = e.x == -INFINITY ? 0.f : ex2f(e.x - A), wl = e.y == -INFINITY ? 0.f : ex2f(e.y - M);
-      l += e.z * wl;
+      const float wo = e.x == -INFINITY ? 0.f : ex2f(e.x - A), wd = e.y == -INFINITY ? -INFINITY : e.y - M;
+      l += times_ex2(e.z, wd);
 #pragma unroll
       for (int d = 0; d < V; d++) x[d] += acc[k + i * width][lane * V + d] * wo;
     }

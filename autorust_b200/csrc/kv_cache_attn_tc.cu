@@ -3,7 +3,10 @@
 //
 //   x = (q . kcode) * c_row * s_k + log2(s_v / v_ref),   P = 2^(x - m + 8),   O = sum P vcode,   l = sum P * v_ref / s_v,   o = v_ref O / l
 //
-// The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
+// v_ref is the scale of the CTA's first page, held inside [2^-5, 2^20]: scales that an append writes are 2^-60 to 2^121, so that v_ref / s_v
+// and the sums of 2^31 keys stay normal f32 numbers.  Beside a page of huge values P may vanish where the row's sum needs it: a CTA
+// that has a scale above 2^15 v_ref among its pages, which it looks through while the first tiles are on their way, sums
+// 2^((q . kcode) c_row s_k - m + 8), exponentials of their own.  The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
 // exponential, and the tensor cores see the codes as f16 (exact) and P and q in f16 (q scaled by a power of two per row:
 // exact but for elements 2^-14 below its largest; P rounded to nearest, the row sum keeps the unrounded values).
 //
@@ -51,6 +54,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -1e30f;            // where a row's maximum starts; a hidden key is -inf
 constexpr float P_SHIFT = 8.0f, LAG = 6.0f;  // P < 2^14: inside f16, and a weight 2^-22 of the largest still a normal number
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60
+constexpr float V_REF_LEAST = 0.03125f, V_REF_MOST = 1048576.0f;
+constexpr float WIDE = 32768.0f;  // s_v / v_ref
 // Of 8 pairs of columns, those whose exponentials are the polynomial's (1.1e-4, below P's rounding to f16): the two tiles'
 // softmax steps mostly fall together and share the MUFU (none 600 us of the case above, a quarter 576, three eighths 578, half 593).
 constexpr uint32_t POLY_MASK = 0x88u;
@@ -72,6 +77,15 @@ struct Cfg {
   static constexpr int QK_STEPS = D / 16, PV_STEPS = HALF / 16;
 };
 
+// x * 2^d, d <= 0, where 2^d by itself may be below the f32 numbers and x * 2^d is not.
+__device__ __forceinline__ float times_ex2(float x, float d) { return x * ex2f(fmaxf(d, -100.0f)) * ex2f(fminf(d + 100.0f, 0.0f)); }
+// Whether `some` holds in one of the 256 threads of the softmax, all of which come here.
+__device__ __forceinline__ bool softmax_any(bool some) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"((uint32_t)some) : "memory");
+  return __shfl_sync(0xffffffffu, any, 0) != 0;
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -170,6 +184,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const float s = a.pool.v_scale[(long long)pg * Hkv + h];
     return s < SCALE_FLOOR ? SCALE_FLOOR : s;  // (a NaN stays)
   };
+  auto v_reference = [&]() {
+    const int pg = page_of(kb);
+    const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
+    return s == s ? fminf(fmaxf(s, V_REF_LEAST), V_REF_MOST) : 1.0f;
+  };
 
   bool lost = false;
   if (warp == W_MMA) {
@@ -214,12 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const int in_page = (1 << log2) - 1;
     const long long page_bytes = ((long long)Hkv << log2) * D;
     const uint8_t* codes = (is_v ? a.pool.v : a.pool.k) + ((long long)h << log2) * D + (key_t & 15) * D + q * 16;
-    float v_ref = 1.0f;
-    if (nkv_max > 0) {
-      const int pg = page_of(kb);
-      const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
-      v_ref = s == s ? s : 1.0f;
-    }
+    const float v_ref = nkv_max > 0 ? v_reference() : 1.0f;
     // page numbers: lane l < 8 of every warp holds that of the tile's l-th block of 16 keys, two tiles ahead
     auto look = [&](int j) { return lane < BLOCKS ? page_of(kb + j * BN + lane * 16) : -2; };
     int pages = look(0), pages1 = look(1);
@@ -372,6 +386,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const uint32_t tS = tmem_addr(tb, lane_base, t * 128), tO = tmem_addr(tb, lane_base, 256 + t * 128);
     const int head = h * G + (in ? row - token * G : 0);
 
+    // a huge V scale somewhere?
+    bool far = false;
+    if (nkv_max > 0) {
+      const float most = WIDE * v_reference();
+#pragma unroll 4
+      for (int blk = (kb >> log2) + tid; blk <= (end - 1) >> log2; blk += 256) {
+        const int pg = table[blk];
+        if (pg >= 0 && pg < a.pool.pages) far = far || a.pool.v_scale[(long long)pg * Hkv + h] > most;
+      }
+    }
+
     // Q: the row times 2^-e, its largest element below 2
     float c_row = 0.f;
     if (nh[t] > 0) {
@@ -402,9 +427,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     }
     float m = NEG, l = 0.f;
 
-    // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's.  False: a wait has run out.
-    auto step = [&](auto edge_c, int i) {
-      constexpr bool EDGE = decltype(edge_c)::value;
+    // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's; FAR: that, and V scales are far apart.  False:
+    // a wait has run out.
+    enum Kind { PLAIN, EDGES, FARS };
+    auto step = [&](auto kind, int i) {
+      constexpr bool EDGE = decltype(kind)::value != PLAIN, FAR = decltype(kind)::value == FARS;
       const float* slot = scales + ((i >> 1) % C::SCALE_RING) * 3 * BLOCKS + (i & 1) * (BLOCKS / 2);
       const int first_out = lim - i * HALF;
       const uint32_t ts = tS + (i & 1) * HALF;
@@ -439,8 +466,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? mc : m;
         const float alpha = ex2f(m - m_new);
+        l = FAR ? times_ex2(l, m - m_new) : l * alpha;
         m = m_new;
-        l *= alpha;
         if (i > 0) {  // PV(i - 1) is done when S(i + 1), issued after it, is there; behind the last scores it reports itself
           const bool last = i + 1 == nh[t];
           uint64_t* bar = (last ? pv_done : s_full) + 2 * t + ((i + 1) & 1);
@@ -464,6 +491,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         }
       }
       const float ref = m - P_SHIFT;
+      if constexpr (FAR) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          float sum = 0.f;
+#pragma unroll
+          for (int x = 0; x < 16; x++)
+            if (b * 16 + x < first_out) sum += ex2f(fmaf(__uint_as_float(sv[b >> 1][(b & 1) * 16 + x]), c[b], -ref));
+          if (add[b] != -INFINITY) l += sum;
+        }
+      }
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
         uint32_t pk[16];
@@ -491,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           }
           float s0, s1;
           unpack_f32x2(sum, s0, s1);
-          l = fmaf(s0 + s1, weight[b], l);
+          if (!FAR) l = fmaf(s0 + s1, weight[b], l);
         }
         tmem_st16(ts + hf * 16, pk);
       }
@@ -501,16 +538,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       return true;
     };
 
-    bool ok = true;
-    for (int i = 0; i < nh[t]; i++) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (i & 1)], (i >> 1) & 1, wctx, 0x57));
-      if (!ok) break;
+    auto scores = [&](int i) {  // false: a wait has run out
+      const bool in = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + (i & 1)], (i >> 1) & 1, wctx, 0x57));
 #ifdef AR_WAIT_TEST
-      if (g_test_late_ns[2] > 0) __nanosleep(g_test_late_ns[2]);  // Test build only: every step comes late, as do the last products.
+      if (in && g_test_late_ns[2] > 0) __nanosleep(g_test_late_ns[2]);  // Test build only: every step comes late, as do the last products.
 #endif
       tc_fence_after();
-      ok = kb + i * HALF + HALF > low[t] || kb + i * HALF + HALF > end ? step(std::true_type{}, i) : step(std::false_type{}, i);
-      if (!ok) break;
+      return in;
+    };
+    bool ok = true;
+    if (!softmax_any(far)) {
+      for (int i = 0; i < nh[t] && ok; i++) {
+        ok = scores(i);
+        if (!ok) break;
+        ok = kb + i * HALF + HALF > low[t] || kb + i * HALF + HALF > end ? step(std::integral_constant<Kind, EDGES>{}, i)
+                                                                         : step(std::integral_constant<Kind, PLAIN>{}, i);
+      }
+    } else {
+      for (int i = 0; i < nh[t] && ok; i++) ok = scores(i) && step(std::integral_constant<Kind, FARS>{}, i);
     }
     if (ok && nh[t] > 0) {
 #ifdef AR_WAIT_TEST
@@ -522,13 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tc_fence_after();
     }
     if (ok) {
-      // v_ref once more: the scale of this CTA's first page
-      float v_ref = 1.0f;
-      if (nh[t] > 0) {
-        const int pg = page_of(kb);
-        const float s = pg >= 0 ? v_scale_of(pg) : 1.0f;
-        v_ref = s == s ? s : 1.0f;
-      }
+      const float v_ref = nh[t] > 0 ? v_reference() : 1.0f;
       const float inv = SPLIT ? 1.0f : nh[t] > 0 && l != 0.f ? v_ref / l : 0.f;
       __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (p.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh;
       float* part = a.partial + (((long long)blockIdx.z * a.batch.T + p.row0 + token) * a.Hq + head) * (D + 4);
@@ -592,8 +631,8 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
   for (int i = 0; i < MOST_PARTS; i++) {
     if (i < parts) {
       const float* src = a.partial + (i * rows + at) * (D + 4) + lane * V;
-      const float wo = ex2f(e[i].x - A), wl = ex2f(e[i].y - M);
-      l = fmaf(e[i].z, wl, l);
+      const float wo = ex2f(e[i].x - A);
+      l += times_ex2(e[i].z, e[i].y - M);
 #pragma unroll
       for (int d = 0; d < V; d += 2) {
         const float2 y = *(const float2*)(src + d);

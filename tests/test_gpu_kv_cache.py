@@ -339,6 +339,43 @@ def test_scales_that_differ_by_orders_of_magnitude(ops, f32, fp8):
 
 
 @pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("order", ["zero first", "largest first"])
+def test_scales_at_both_ends(ops, f32, fp8, order):
+    """All-zero pages (the least scale) and pages of 1e37, either in front: whole tiles, cut ones, many rows, many rows in parts."""
+    import torch
+    L, page, D = 4096, 16, 64
+    s = Setup(ops, 43, [L], Hkv=1, D=D, page=page, fp8=fp8, f32=f32)
+    k, kf = s.rows(L, 1, 0.3)
+    v = s.rng.standard_normal((L, 1, D)).astype(np.float32)
+    size = np.tile([0.0, 1e37, 1e-16, 1.0] if order == "zero first" else [1e37, 1e-16, 0.0, 1.0], L // 64)
+    v = np.clip(v, -4, 4) * np.repeat(size, page).astype(np.float32)[:, None, None]
+    v = torch.from_numpy(v).cuda().to(k.dtype)
+    q, qf = s.rows(40, 4, 2.0)
+    where = (s.dtable, s.ints([L]), s.ints([0, L]))
+    s.ops.kv_cache_append(s.cache, k, v, *where)
+    s.plain.append(kf, v.float().cpu().numpy(), s.table, [L], [0, L])
+    s.check_pool()
+    # (rows that see the first page, the first two, and so on; then all of it)
+    def check(q, qf, lengths, starts, table, bound):
+        got = s.ops.kv_cache_attention(s.cache, q, table, s.ints(lengths), s.ints(starts), max_length=bound)
+        assert_attention_close(got.double().cpu().numpy(), *s.expect(qf, lengths, np.array(starts), True), f32)
+    for last in (16, 32, 48, 64, L):
+        for n in (1, 8, 40):
+            check(q[:n], qf[:n], [last], [0, n], s.dtable, max(last, 64))
+    if f32:
+        return
+    q, qf = s.rows(1000, 4, 2.0)
+    assert ops.kv_cache_attention_workspace(s.cache, 1000, 4, 1, L) == 8 * 1000 * 4 * (D + 4) * 4  # many rows, in eight parts
+    check(q, qf, [L], [0, 1000], s.dtable, L)
+    s.table = np.repeat(s.table, 6, axis=0)
+    lengths = [600, 16, 450, 560, 599, 48]
+    q, qf = s.rows(sum(lengths), 4, 2.0)
+    assert ops.kv_cache_attention_workspace(s.cache, sum(lengths), 4, 6, 600) == 0  # many rows, not cut
+    check(q, qf, lengths, [0, *np.cumsum(lengths)], s.dtable.expand(6, -1).contiguous(), 600)
+
+
+@pytest.mark.parametrize("f32", [False, True])
 def test_large_and_tiny_queries(ops, f32):
     """One key holds all the weight; logits of +-1e4; queries of 1e-30 (uniform weights) and zero."""
     lengths = [200]
