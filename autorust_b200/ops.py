@@ -396,6 +396,9 @@ class KvCache:
         object.__setattr__(self, "_pool", pool)
         object.__setattr__(self, "_device", k.device)
 
+    def __reduce__(self):  # copies and pickles hold tensors of their own, and so a description of their own
+        return KvCache, (self.k, self.v, self.k_scale, self.v_scale, self.k_mean)
+
     @property
     def fp8(self) -> bool:
         return self.k.dtype == torch.uint8
@@ -493,7 +496,8 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     """o = softmax(q k^T / sqrt(D)) v over the cached tokens of each row's sequence (ar_kv_cache_attention).  q [T, Hq, D],
     float32 or bfloat16, packed like the k of kv_cache_append: a sequence's rows are its last tokens, and with `causal`
     each sees the keys up to itself.  max_length: a bound on lengths, for dividing the work (None: the page table's width).
-    `workspace` is a uint8 CUDA tensor of kv_cache_attention_workspace bytes; one is allocated when needed and none is given."""
+    `workspace` is a uint8 CUDA tensor of kv_cache_attention_workspace bytes; one is allocated when needed and none is given.
+    For answering, not for training: nothing here has a gradient."""
     L = _abi.load()
     if q.dim() != 3:
         raise ValueError("q must be [T, Hq, D]")

@@ -310,7 +310,8 @@ typedef struct ar_kv_batch {
  * earlier token of the sequence, else max(s0, s1).  New codes are rn(x * (1 / s)); when s > s0 the earlier codes become
  * rn(code * (s0 / s)) -- exact for E4M3 but in its subnormal range, and for INT8 one more rounding whenever the scale
  * grows.  A value that is not finite makes the scale of its page and head NaN: the page reads back as NaN.
- * A page written by a call must belong to one sequence of that call (sequences may share full pages they only read).
+ * A page written by a call must belong to one sequence of that call and stand once in its row (sequences may share full
+ * pages they only read); else its codes are those of either or a mixture, and nothing outside the page is touched.
  * A page number outside [0, pages) or a position past table_pages * page is skipped on the device and reported by
  * ar_attn_last_status(NULL, ..) as AR_ERR_PAGE; nothing outside the pool is touched. */
 int ar_kv_cache_append(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* k, const int64_t* k_strides,

@@ -620,6 +620,26 @@ def test_a_pool_beyond_32_bit_offsets(ops):
     assert ops.last_status(None) == 0
 
 
+def test_copies_have_tensors_of_their_own(ops):
+    import copy
+    import io
+    import torch
+    s = Setup(ops, 61, [40, 9], Hkv=1, D=64, mean=True)
+    s.append([40, 9], [40, 9])
+    q, _ = s.rows(2, 2)
+    where = (s.dtable, s.ints([40, 9]))
+    want = ops.kv_cache_attention(s.cache, q, *where)
+    file = io.BytesIO()
+    torch.save(s.cache, file)
+    file.seek(0)
+    copies = [copy.deepcopy(s.cache), torch.load(file, weights_only=False)]
+    s.cache.k.zero_()
+    s.cache.v_scale.zero_()
+    for c in copies:
+        assert c.k.data_ptr() != s.cache.k.data_ptr() and not c.fp8
+        assert torch.equal(ops.kv_cache_attention(c, q, *where), want)
+
+
 def test_empty_calls(ops):
     import torch
     s = Setup(ops, 99, [10], Hkv=1, D=64)
