@@ -478,10 +478,15 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     (k, v) [tokens, Hkv, D] of `dtype`.  With starts = running sums of lengths that is everything.  out: (k, v) to write into,
     views with a contiguous last dimension; rows that belong to no sequence are left as they were."""
     pool, dev, tokens = cache._pool, cache._device, int(tokens)
-    shape = (tokens, pool.Hkv, pool.D)
-    k, v = out if out is not None else torch.empty((2, *shape), dtype=dtype, device=dev).unbind()
-    code = _dtype_code(k)
-    ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
+    heads, D = pool.Hkv, pool.D
+    if out is None:
+        k, v = torch.empty((2, tokens, heads, D), dtype=dtype, device=dev).unbind()
+        code, ks = _dtype_code(k), _Strides2(heads * D, D)
+        vs = ks
+    else:
+        k, v = out
+        shape, code = (tokens, heads, D), _dtype_code(k)
+        ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, tokens)
     _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
     if stream is not None and out is None:
@@ -508,8 +513,9 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     qs = _kv_rows("q", q, shape, q.dtype, dev)
     fresh = out is None
     if fresh:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    os = _kv_rows("out", out, shape, q.dtype, dev)
+        out, os = q.new_empty(shape), _Strides2(Hq * pool.D, pool.D)
+    else:
+        os = _kv_rows("out", out, shape, q.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, T)
     bound = batch.table_pages * pool.page if max_length is None else int(max_length)
     have = 0
