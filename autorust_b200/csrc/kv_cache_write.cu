@@ -7,10 +7,11 @@
 // Both are bound by memory: (1 + element size) bytes per value.  One CTA owns one page of one head at a time, so that nothing is
 // shared between CTAs: the page's tokens are loaded once, 32 values per thread, and stay in registers between the maximum and the
 // codes.  Finding the sequence, its length and its page is a chain of dependent loads, about 2.5 us: in large calls a CTA takes
-// several heads of its page one after the other, and asks for the next head's values before it works on this one's.  K and V
+// several heads of its page one after the other, and asks for the next head's values before it works on this one's (writing: by
+// cp.async into shared memory, which leaves registers for more threads).  K and V
 // are the two halves of grid.z.
 //
-// Measured, bf16, 8 kv heads, D = 128, INT8: 32768 tokens written 47 us (4.3 TB/s), read back 38 (5.2 TB/s), 131072 tokens read back 139 (5.8 TB/s).
+// Measured, bf16, 8 kv heads, D = 128, INT8: 32768 tokens written 44.4 us (4.5 TB/s), read back 38 (5.2 TB/s), 131072 tokens read back 139 (5.8 TB/s).
 // Writing also waits for a page's maximum between its values and their codes.
 #include <cuda_bf16.h>
 
@@ -24,6 +25,8 @@ namespace {
 
 constexpr int PER_THREAD = 32;              // values per thread
 constexpr int VECS = PER_THREAD / 8;        // in vectors of 8
+// Threads per SM that the writing kernel is built for (32768 tokens written: 49 us with 512, 45 with 768, 50 with 1024, which spill).
+constexpr int APPEND_THREADS = 768;
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60: an empty or all-zero page needs no case of its own
 
 // 8 values as they lie in memory.
@@ -31,14 +34,6 @@ template <bool F32>
 struct Raw {
   uint4 w[F32 ? 2 : 1];
 };
-template <bool F32>
-__device__ __forceinline__ Raw<F32> load8(const void* base, long long at) {
-  Raw<F32> r;
-  const uint4* p = F32 ? (const uint4*)((const float*)base + at) : (const uint4*)((const __nv_bfloat16*)base + at);
-#pragma unroll
-  for (int i = 0; i < (F32 ? 2 : 1); i++) r.w[i] = p[i];
-  return r;
-}
 template <bool F32>
 __device__ __forceinline__ void values8(const Raw<F32>& r, float (&x)[8]) {
   if constexpr (F32) {
@@ -160,8 +155,15 @@ __device__ __forceinline__ Span span_of(const KvPool& pool, const KvBatch& batch
 
 // E = page * D values of a page and head, E / 32 threads; heads blockIdx.y, blockIdx.y + gridDim.y, ...  A thread has the same 8 channels
 // of every TOKENS-th token.
+// The next head's values on their way: cp.async into places that only the thread which asks reads, so without barriers.  32768 tokens written: 44.4 us;
+// with these values in registers 47.3, with a third stage 45.3, a fourth 46.3.
+template <int E, bool F32>
+struct Ring {
+  static constexpr int STAGE = E * (F32 ? 4 : 2);
+  static constexpr int BYTES = 2 * STAGE;
+};
 template <int E, int D, bool E4M3, bool F32>
-__global__ void __launch_bounds__(E / PER_THREAD, E == 16384 ? 1 : (F32 ? 512 : 768) * PER_THREAD / E)
+__global__ void __launch_bounds__(E / PER_THREAD, (F32 ? 512 : APPEND_THREADS) * PER_THREAD / E)
 kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const KvRows vr) {
   constexpr int THREADS = E / PER_THREAD, TOKENS = THREADS * 8 / D;
   __shared__ uint32_t tops[2][THREADS / 32];
@@ -179,19 +181,27 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
   uint8_t* codes = (is_v ? pool.v : pool.k) + (long long)span.page * pool.Hkv * E;
   float* scales = (is_v ? pool.v_scale : pool.k_scale) + (long long)span.page * pool.Hkv;
   const float* means = is_v ? nullptr : pool.k_mean;
-  Raw<F32> raw[VECS];
-  float next_s0 = 0.f;
-  auto fetch = [&](int h) {
-    if (h >= pool.Hkv) return;
-    if (span.t0 > 0) next_s0 = scales[h];
-    const long long at = first_row + (long long)h * rows.sh;
+  using R = Ring<E, F32>;
+  constexpr int PER_VEC = F32 ? 2 : 1;
+  extern __shared__ __align__(16) uint8_t ring[];
+  uint8_t* const mine = ring + threadIdx.x * 16;
+  auto fetch = [&](int h, int stage) {
+    if (h < pool.Hkv) {
+      const uint32_t to = arptx::smem_u32(mine) + stage * R::STAGE;
+      const long long at = first_row + (long long)h * rows.sh;
 #pragma unroll
-    for (int i = 0; i < VECS; i++)
-      if (in[i]) raw[i] = load8<F32>(rows.p, at + i * step);
+      for (int i = 0; i < VECS; i++)
+        if (in[i]) {
+          const char* from = (const char*)rows.p + (at + i * step) * (F32 ? 4 : 2);
+#pragma unroll
+          for (int j = 0; j < PER_VEC; j++) arptx::cp_async16(to + (i * PER_VEC + j) * THREADS * 16, from + j * 16, true);
+        }
+    }
+    arptx::cp_async_commit();
   };
-  fetch(blockIdx.y);
+  fetch(blockIdx.y, 0);
   for (int h = blockIdx.y, n = 0; h < pool.Hkv; h += gridDim.y, n ^= 1) {
-    const float s0 = next_s0;
+    const float s0 = span.t0 > 0 ? scales[h] : 0.f;
     float x[VECS][8];
     float most = 0.f;
     float4 ma, mb;
@@ -199,10 +209,15 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
       ma = *(const float4*)(means + h * D + d);
       mb = *(const float4*)(means + h * D + d + 4);
     }
+    fetch(h + gridDim.y, n ^ 1);  // (what was read there is in use by now)
+    arptx::cp_async_wait<1>();
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
       if (in[i]) {
-        values8<F32>(raw[i], x[i]);
+        Raw<F32> raw;
+#pragma unroll
+        for (int j = 0; j < PER_VEC; j++) raw.w[j] = *(const uint4*)(mine + n * R::STAGE + (i * PER_VEC + j) * THREADS * 16);
+        values8<F32>(raw, x[i]);
         if (means) {
           const float off[8] = {-ma.x, -ma.y, -ma.z, -ma.w, -mb.x, -mb.y, -mb.z, -mb.w};
 #pragma unroll
@@ -214,7 +229,6 @@ kv_append_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const 
         for (int c = 0; c < 8; c += 2) most = max_abs_nan(most, x[i][c], x[i][c + 1]);
       }
     }
-    fetch(h + gridDim.y);
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // (infinities and NaN are the largest patterns)
     if constexpr (THREADS > 32) {
       if ((threadIdx.x & 31) == 0) tops[n][threadIdx.x >> 5] = top;
@@ -319,8 +333,8 @@ kv_read_kernel(const KvPool pool, const KvBatch batch, const KvRows kr, const Kv
   }
 }
 
-// CTAs up to which every head of a page gets one of its own: 8 per SM (32768 tokens written and read back: 62 + 56 us with 32, 50 + 46
-// with 16, 49 + 44 with 8, 50 + 43 with 4).
+// CTAs up to which every head of a page gets one of its own: 8 per SM (4 of prompts of up to 789 tokens written and read back: 5.7 + 4.1 us,
+// with 4 per SM 7.3 + 4.5; 32768 tokens 44.4 + 39 and 44.6 + 40.4; 12 per SM like 8).
 constexpr int SPREAD_CTAS = 8 * 148;
 
 template <bool WRITE, bool E4M3, bool F32>
@@ -328,8 +342,14 @@ cudaError_t launch(const KvPool& pool, const KvBatch& batch, const KvRows& k, co
   const long long places = kv_places(batch, 1, pool.page_log2, 2);
   const long long per_cta = std::max(1ll, std::min((long long)pool.Hkv, places * pool.Hkv * 2 / SPREAD_CTAS));  // heads
   const dim3 grid((unsigned)places, (unsigned)((pool.Hkv + per_cta - 1) / per_cta), 2);
-  auto go = [&](auto kern, int E) { return launch_early(kern, grid, dim3(E / PER_THREAD), 0, stream, pool, batch, k, v); };
-#define AR_KV_E(E, D) (WRITE ? go(kv_append_kernel<E, D, E4M3, F32>, E) : go(kv_read_kernel<E, D, E4M3, F32>, E))
+  auto go = [&](auto kern, int E, int smem) {
+    if (smem > 47 * 1024) {  // (48 KB with the static part)
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+    }
+    return launch_early(kern, grid, dim3(E / PER_THREAD), smem, stream, pool, batch, k, v);
+  };
+#define AR_KV_E(E, D) (WRITE ? go(kv_append_kernel<E, D, E4M3, F32>, E, Ring<E, F32>::BYTES) : go(kv_read_kernel<E, D, E4M3, F32>, E, 0))
   if (pool.D == 128) {
     switch (pool.page_log2) {
       case 4: return AR_KV_E(2048, 128);
