@@ -56,6 +56,7 @@ SYMBOLS = (
     "ar_kv_cache_read",
     "ar_kv_cache_attention_workspace_bytes",
     "ar_kv_cache_attention",
+    "ar_kv_cache_attention_plan",
     "ar_attn_last_status",
     "ar_attn_plan",
     "ar_attn_selections",
@@ -148,6 +149,8 @@ def load() -> ctypes.CDLL:
     L.ar_kv_cache_attention_workspace_bytes.restype = sz
     L.ar_kv_cache_attention.argtypes = [pool, batch, ci, p, p, p, p, i64, i64, ci, p, sz, p]
     L.ar_kv_cache_attention.restype = ci
+    L.ar_kv_cache_attention_plan.argtypes = [pool, batch, ci, i64, i64, ci, ctypes.POINTER(ctypes.c_int32)]
+    L.ar_kv_cache_attention_plan.restype = ci
     L.ar_attn_last_status.argtypes = [p, p]
     L.ar_attn_last_status.restype = ci
     L.ar_attn_plan.argtypes = [ci, i64, i64, i64, i64, i64, ci, ctypes.POINTER(ctypes.c_int32)]
@@ -165,6 +168,13 @@ def plan(path: int, B: int, Hq: int, Hkv: int, S: int, D: int, causal: bool) -> 
     """Which form of its kernels a call of these sizes takes (ar_attn_plan); needs no GPU."""
     out = (ctypes.c_int32 * 8)()
     check(load().ar_attn_plan(path, B, Hq, Hkv, S, D, int(causal), out), "ar_attn_plan")
+    return list(out)
+
+
+def kv_plan(pool: KvPool, batch: KvBatch, dtype: int, Hq: int, max_length: int, causal: bool) -> list[int]:
+    """How a cache attention is divided (ar_kv_cache_attention_plan): rows of a tile, CTAs that share the keys, parts; needs no GPU."""
+    out = (ctypes.c_int32 * 3)()
+    check(load().ar_kv_cache_attention_plan(pool, batch, dtype, Hq, max_length, int(causal), out), "ar_kv_cache_attention_plan")
     return list(out)
 
 

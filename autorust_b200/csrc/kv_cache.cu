@@ -107,6 +107,20 @@ size_t ar_kv_cache_attention_workspace_bytes(const ar_kv_pool* pool, const ar_kv
   return ar::kv_attn_plan(p, s, dtype, (int)Hq, (int)max_length, causal).workspace;
 }
 
+int ar_kv_cache_attention_plan(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, int64_t Hq, int64_t max_length,
+                               int causal, int32_t* plan) {
+  ar::KvPool p;
+  ar::KvBatch s;
+  if (!plan) return AR_ERR_NULL;
+  const int rc = check_attention(pool, batch, dtype, Hq, max_length, &p, &s);
+  if (rc != AR_OK) return rc;
+  const ar::KvAttnPlan found = s.T == 0 ? ar::KvAttnPlan{0, 0, 0, 0} : ar::kv_attn_plan(p, s, dtype, (int)Hq, (int)max_length, causal);
+  plan[0] = found.rows;
+  plan[1] = found.ctas;
+  plan[2] = found.parts;
+  return AR_OK;
+}
+
 int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* q,
                           const int64_t* q_strides, void* o, const int64_t* o_strides, int64_t Hq, int64_t max_length,
                           int causal, void* workspace, size_t workspace_bytes, void* cu_stream) {

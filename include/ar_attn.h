@@ -336,6 +336,12 @@ size_t ar_kv_cache_attention_workspace_bytes(const ar_kv_pool* pool, const ar_kv
 int ar_kv_cache_attention(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, const void* q,
                           const int64_t* q_strides, void* o, const int64_t* o_strides, int64_t Hq, int64_t max_length,
                           int causal, void* workspace, size_t workspace_bytes, void* cu_stream);
+/* How such a call is divided, for tests and profiles: fills plan[0 .. 2] and returns AR_OK; no device is touched.
+ *   rows of a row tile -- 8 or 16, or 256: the tensor cores' kernel
+ *   CTAs that the keys of all row tiles are shared out over (0: a CTA takes whole row tiles)
+ *   parts that the tensor cores' kernel divides the keys of a row tile into (1: none) */
+int ar_kv_cache_attention_plan(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype, int64_t Hq, int64_t max_length,
+                               int causal, int32_t* plan);
 
 /* Synchronises `cu_stream` and reads a device status word: AR_OK, or AR_ERR_DEVICE_WAIT when a bounded wait
  * expired inside a kernel (the launch then returned without finishing its tile; later CTAs of that launch leave at
