@@ -81,6 +81,23 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
+// ---- references of a softmax ----
+// 2^(m + e): m a logit, e a logarithm of a page's scale.  In one number the scale would be lost beside a logit of 2^24 or more, and keys
+// whose logits are that large and alike would be weighted by their pages' scales.
+struct KvRef {
+  float m, e;
+};
+// log2 of p over q, for a q whose m is not -inf (p's may be).
+__device__ __forceinline__ float kv_over(const KvRef& p, const KvRef& q) { return (p.m - q.m) + (p.e - q.e); }
+// The larger one; m = -inf: there is none.
+__device__ __forceinline__ KvRef kv_larger(const KvRef& p, const KvRef& q) {
+  if (p.m == -INFINITY) return q;
+  return q.m == -INFINITY || kv_over(p, q) > 0.f ? p : q;
+}
+// Where a logit may reach this (in the log2 domain), it is added to the page's exponent only after the reference has been taken off it:
+// in one f32 number the exponent would be rounded to 2^-5 there.
+constexpr float KV_LARGE_LOGIT = 64.0f;  // as |q| * scale, codes up to 448 and 128 channels: below 2^20
+
 // ---- codes ----
 // The four codes of w -> f32.
 template <bool E4M3>

@@ -14,8 +14,10 @@
 // logit: x = logit * log2(e) + e - e_ref, u = 2^(x - m + 12), where m follows the maximum of x (it may lag by up to 2, so
 // that accumulators are rescaled rarely) and e_ref is the exponent of the piece's first page, held inside [-5, 20]; P = u * f < 2^15,
 // and the row sum takes u * 2^(e_ref - e).  Scales that an append writes are 2^-60 to 2^121: e - e_ref is then -80 to 126, which
-// leaves the factor and the sums of 2^31 keys normal f32 numbers.  Beside a page of huge values u may vanish where the row's sum needs
-// it: from the first scale above 2^20 on, a warp's groups sum 2^(x - (e - e_ref) - m + 12) instead, exponentials of their own.  O is then in units of 2^(m - 12 + e_ref), the sum l in units of 2^(m - 12).
+// leaves the factor and the sums of 2^31 keys normal f32 numbers.  O is then in units of 2^(m - 12 + e_ref), the sum l in units of 2^(m - 12).
+// Beside a page of huge values u may vanish where the row's sum needs it, and beside a large logit e - e_ref is rounded off: from the first V
+// scale above 2^20 on, or K scale that with the warp's largest |q| may make a logit of 2^20, a warp's groups keep the reference as a pair (logit, exponent), take
+// it off logit and exponent each, and sum 2^(logit - m + 12), exponentials of their own.
 //
 // Rows go in tiles of 8: the query heads of one kv head's group next to one another, then the next token.  S = Q K^T has the
 // digits or terms of 8 rows on the 16-row side of the MMA (two digits of the same rows side by side: one thread gets both
@@ -117,7 +119,8 @@ struct Sh {
   static constexpr int STAGES = D == 64 ? 4 : NT == 1 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * TILE;            // per warp
   static constexpr int ML = WARPS * RING;                   // [warp][row]{m, l}
-  static constexpr int SCALES = ML + WARPS * ROWS * 8;      // [warp][stage]{s_k, s_v of the first block, s_k, s_v of the second}
+  static constexpr int ME = ML + WARPS * ROWS * 8;          // [warp][row] the reference's exponent (KvRef::e)
+  static constexpr int SCALES = ME + WARPS * ROWS * 4;      // [warp][stage]{s_k, s_v of the first block, s_k, s_v of the second}
   static constexpr int BYTES = SCALES + WARPS * STAGES * 16;
   static_assert(RING >= ROWS * D * 4, "the ring also takes the warp's accumulator at the end of a piece");
   static_assert((BYTES + 1024 + 512) * CTAS_PER_SM <= 228 * 1024, "shared memory of the SM");
@@ -178,7 +181,9 @@ __device__ __forceinline__ Work work_of(const KvAttnArgs& a, int G, int b) {
 }
 
 // Partial results of a cut row tile.  A CTA has two places: 2i for the piece it starts with, which continues the CTA before, and
-// 2i + 1 for the piece it ends with, when that begins a cut tile.  A place: ROWS x D values, then per row {m + e_ref, m, l, -}.
+// 2i + 1 for the piece it ends with, when that begins a cut tile.  A place: ROWS x D values, then per row {m + e_ref, m, l, 0}, or
+// where a warp was far {m, m's exponent, -l, FAR_PIECE + e_ref}: the sign of l (of a zero, too) tells the join, which has no register to spare.
+constexpr float FAR_PIECE = 1024.0f;
 template <int D, int ROWS>
 __host__ __device__ constexpr int place_floats() { return ROWS * (D + 4); }
 // What the join has to know about the cut tile that CTA i begins: packed row of its sequence's first token, first row of
@@ -202,6 +207,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * S::RING;
   float* ml = (float*)(smem + S::ML);
+  float* me = (float*)(smem + S::ME) + warp * ROWS;
   float* scales = (float*)(smem + S::SCALES) + warp * S::STAGES * 4;
   const int G = a.Hq / a.pool.Hkv, Hkv = a.pool.Hkv;
 
@@ -390,6 +396,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       look(it + 1);
     }
 
+    uint32_t q_top = 0;  // of the warp's rows
     uint32_t qa[QOPS][QSTEPS][4] = {};
     float row_c[NT];  // of row g: logit in the log2 domain = accumulator * row_c * s_k
     int lim[NT];      // keys that row g sees
@@ -404,6 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
         for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (top < 0x7f800000u) q_top = max(q_top, top);
       // 2^-e brings the largest element below 2; both factors are normal f32 numbers
       const int e = min(max((int)(top >> 23) - 127, -100), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -453,11 +461,15 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       l[nt] = 0.f;
     }
 
-    bool wide = false;  // a V scale above WIDE has been met
+    // From the first V scale above WIDE, or K scale above sk_most, on: scales and logits may be far apart.
+    bool far = false;
+    const float sk_most = KV_LARGE_LOGIT * __uint_as_float((uint32_t)(127 - min(max((int)(__reduce_max_sync(0xffffffffu, q_top) >> 23) - 127, -100), 126)) << 23);
+    if (lane < ROWS) me[lane] = 0.f;
 
-    // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out, or V scales are wide apart.
+    // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out, or far.
     auto step = [&](auto edge_c, int it) {
       constexpr bool EDGE = decltype(edge_c)::value;
+      const bool pairs = EDGE && far;
       const uint8_t* kt = ring + (it % S::STAGES) * 2 * S::TILE;
       const uint8_t* vt = kt + S::TILE;
       const float4 sc = *(const float4*)(scales + (it % S::STAGES) * 4);
@@ -520,41 +532,79 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           w_l[blk] = __uint_as_float((uint32_t)(127 - rel) << 23);
         }
       }
-      float mx[NT];
-      bool grow = false;
+      auto rescale = [&](int nt, float alpha) {  // the accumulators of this thread are rows 2c and 2c + 1
+        const float al[2] = {__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4)};
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        float top = -INFINITY;
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int n8 = 0; n8 < 4; n8++) {
-          const float k = row_c[nt] * sk[n8 >> 1];
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            float v = fmaf(s[nt][n8][i], k, ex[n8 >> 1]);
-            if (EDGE && (key0 + n8 * 8 + 2 * c + i >= lim[nt] || sk[n8 >> 1] < 0.f)) v = -INFINITY;
-            s[nt][n8][i] = v;
-            top = fmaxf(top, v);
-          }
-        }
-        mx[nt] = top;
-        grow = grow || top > m[nt] + LAG;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
+          for (int x = 0; x < 4; x++) o[nt][i][x] *= al[x & 1];
+      };
+      if (pairs) {  // s becomes the logit alone, the reference a pair
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          float top = mx[nt];
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float m_new = fmaxf(m[nt], top);
-          const float alpha = m[nt] == -INFINITY ? 0.f : ex2f(m[nt] - m_new);
-          l[nt] = m[nt] == -INFINITY ? l[nt] * 0.f : EDGE ? times_ex2(l[nt], m[nt] - m_new) : l[nt] * alpha;
-          m[nt] = m_new;
-          // the accumulators of this thread are rows 2c and 2c + 1
-          const float al[2] = {__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4)};
+          KvRef most{-INFINITY, 0.f};
 #pragma unroll
-          for (int i = 0; i < MT; i++)
+          for (int blk = 0; blk < 2; blk++) {
+            const float k = row_c[nt] * sk[blk];
+            float top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 4; x++) o[nt][i][x] *= al[x & 1];
+            for (int n8 = 2 * blk; n8 < 2 * blk + 2; n8++)
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                float v = __fmul_rn(s[nt][n8][i], k);
+                if (key0 + n8 * 8 + 2 * c + i >= lim[nt] || sk[blk] < 0.f) v = -INFINITY;
+                s[nt][n8][i] = v;
+                top = fmaxf(top, v);
+              }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            most = kv_larger(KvRef{top, ex[blk]}, most);
+          }
+          const KvRef ref{m[nt], me[nt * 8 + g]};
+          float alpha = 1.0f;
+          if (most.m != -INFINITY && (ref.m == -INFINITY || kv_over(most, ref) > LAG)) {
+            const float d = ref.m == -INFINITY ? -INFINITY : kv_over(ref, most);
+            alpha = ex2f(d);
+            l[nt] = times_ex2(l[nt], d);
+            m[nt] = most.m;
+          }
+          __syncwarp();
+          if (c == 0 && alpha != 1.0f) me[nt * 8 + g] = most.e;
+          __syncwarp();
+          if (__any_sync(0xffffffffu, alpha != 1.0f)) rescale(nt, alpha);
+        }
+      } else {
+        float mx[NT];
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int n8 = 0; n8 < 4; n8++) {
+            const float k = row_c[nt] * sk[n8 >> 1];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              float v = fmaf(s[nt][n8][i], k, ex[n8 >> 1]);
+              if (EDGE && (key0 + n8 * 8 + 2 * c + i >= lim[nt] || sk[n8 >> 1] < 0.f)) v = -INFINITY;
+              s[nt][n8][i] = v;
+              top = fmaxf(top, v);
+            }
+          }
+          mx[nt] = top;
+          grow = grow || top > m[nt] + LAG;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            float top = mx[nt];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m[nt], top);
+            const float alpha = m[nt] == -INFINITY ? 0.f : ex2f(m[nt] - m_new);
+            l[nt] = m[nt] == -INFINITY ? l[nt] * 0.f : EDGE ? times_ex2(l[nt], m[nt] - m_new) : l[nt] * alpha;
+            m[nt] = m_new;
+            rescale(nt, alpha);
+          }
         }
       }
       uint32_t ph[NT][4];
@@ -562,13 +612,15 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         float sum[2] = {0.f, 0.f};
-        const float ref = m[nt] == -INFINITY ? 0.f : m[nt] - P_SHIFT;
+        const float ref = m[nt] == -INFINITY ? 0.f : pairs ? m[nt] : m[nt] - P_SHIFT;
+        const float me_row = pairs ? me[nt * 8 + g] - P_SHIFT : 0.f;
 #pragma unroll
         for (int n8 = 0; n8 < 4; n8++) {
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float p = ex2f(s[nt][n8][i] - ref);
-            sum[n8 >> 1] += EDGE && wide ? ex2f(s[nt][n8][i] - ref - ex[n8 >> 1]) : p;
+            const float x = s[nt][n8][i] - ref;
+            const float p = ex2f(pairs ? x + (ex[n8 >> 1] - me_row) : x);
+            sum[n8 >> 1] += pairs ? ex2f(x - me_row) : p;
             s[nt][n8][i] = p * f[n8 >> 1];
             // a row that does not see the key takes 0 * f: a page's NaN must not reach it
             if (EDGE && key0 + n8 * 8 + 2 * c + i >= lim[nt]) s[nt][n8][i] = 0.f;
@@ -577,7 +629,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           ph[nt][n8] = pack_half2(x0, x1);
           if constexpr (F32) pl[nt][n8] = pack_half2(x0 - half_lo(ph[nt][n8]), x1 - half_hi(ph[nt][n8]));
         }
-        l[nt] += EDGE && wide ? sum[0] + sum[1] : sum[0] * w_l[0] + sum[1] * w_l[1];
+        l[nt] += pairs ? sum[0] + sum[1] : sum[0] * w_l[0] + sum[1] * w_l[1];
       }
 
       // O^T += V^T P^T, 16 keys per step: tokens 2c, 2c + 1, 2c + 8, 2c + 9, channels 16g .. or 8g ..; tile i has channels 2i, 2i + 1 of those
@@ -616,8 +668,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       cp_async_wait<S::STAGES - 1>();
       __syncwarp();
       const float4 sc = *(const float4*)(scales + (it % S::STAGES) * 4);
-      wide = wide || fmaxf(sc.y, sc.w) > WIDE;
-      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || fminf(sc.x, sc.z) < 0.f || wide)
+      far = far || fmaxf(sc.y, sc.w) > WIDE || fmaxf(sc.x, sc.z) > sk_most;
+      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || fminf(sc.x, sc.z) < 0.f || far)
         step(std::true_type{}, it);
       else
         step(std::false_type{}, it);
@@ -644,7 +696,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       if (c == 0) *(float2*)(ml + (warp * ROWS + nt * 8 + g) * 2) = make_float2(m[nt], sum);
     }
-    __syncthreads();
+    const bool some_far = __syncthreads_or(far);
     const bool first = g_begin == 0, last = g_end == w.groups;
     const bool direct = first && last;
     float* place = nullptr;
@@ -671,16 +723,27 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
         x[v] = *(const float2*)(ml + (v * ROWS + r) * 2);
         mm = fmaxf(mm, x[v].x);
       }
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ref = 0.f;  // the row's reference is 2^(base + ref)
+      if (some_far) {
+        ref = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < WARPS; v++) {
+          x[v].x = (x[v].x - base) + ((const float*)(smem + S::ME))[v * ROWS + r];
+          ref = fmaxf(ref, x[v].x);
+        }
+        if (ref == -INFINITY) ref = 0.f;
+      }
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       float ll = 0.f;
 #pragma unroll
       for (int v = 0; v < WARPS; v++) {
         if (x[v].x == -INFINITY && x[v].y == 0.f) continue;  // (a row of NaN has no maximum but a NaN sum)
-        const bool top = x[v].x == mm;
-        const float scale = top ? 1.0f : ex2f(x[v].x - mm);
+        const float d = some_far ? x[v].x - ref : x[v].x - base;
+        const float scale = ex2f(d);
         const float4 y = *(const float4*)((const float*)(smem + v * S::RING) + at);
         sum.x += y.x * scale; sum.y += y.y * scale; sum.z += y.z * scale; sum.w += y.w * scale;
-        ll += top ? x[v].y : times_ex2(x[v].y, x[v].x - mm);
+        ll += times_ex2(x[v].y, d);
       }
       if (direct) {
         const int token = by_g(r0 + r), head = h * G + (r0 + r) - token * G;
@@ -692,7 +755,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           *(uint2*)((__nv_bfloat16*)a.o.p + dst) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
       } else {
         *(float4*)(place + r * D + piece * 4) = sum;
-        if (piece == 0) *(float4*)(place + ROWS * D + r * 4) = make_float4(mm + (float)e_ref, mm, ll, 0.f);
+        if (piece == 0) *(float4*)(place + ROWS * D + r * 4) = some_far ? make_float4(mm, ref, -ll, (float)e_ref + FAR_PIECE) : make_float4(mm + (float)e_ref, mm, ll, 0.f);
       }
     }
 
@@ -714,11 +777,55 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 // those the rows y, y + 4, ..; its warps share a row's pieces, each against maxima of its own, and the row's first warp joins
 // them, always in the same order.  A few small CTAs: they are in place and waiting before the last CTA above has left.
 constexpr int JOIN_WARPS = 8, JOIN_STEP = 7, JOIN_Y = 4;
+
+// A lane's values of a row, to `dst` in the tensor.
+template <int D, bool F32>
+__device__ __forceinline__ void store_row(void* dst, const float (&x)[D / 32], float inv) {
+#pragma unroll
+  for (int d = 0; d < D / 32; d += 2) {
+    if constexpr (F32)
+      *(float2*)((float*)dst + d) = make_float2(x[d] * inv, x[d + 1] * inv);
+    else
+      *(uint32_t*)((__nv_bfloat16*)dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+  }
+}
+// Row r of a tile with far pieces, by one warp, references as distances from the largest logit among them.  (A function of its own: such
+// pieces are rare, and the others' loop has no registers to spare.)
+template <int D, bool F32, int ROWS>
+__device__ __noinline__ void join_far(const float* places, int first, int pieces, int r, void* dst) {
+  constexpr int V = D / 32;
+  auto place = [&](int p) { return places + (long long)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * place_floats<D, ROWS>(); };
+  auto row = [&](int p) {  // {m, m's exponent, l, e_ref}
+    const float4 e = *(const float4*)(place(p) + ROWS * D + r * 4);
+    return e.w == 0.f ? make_float4(e.y, 0.f, e.z, e.y == -INFINITY ? 0.f : e.x - e.y) : make_float4(e.x, e.y, -e.z, e.w - FAR_PIECE);
+  };
+  float top = -INFINITY, A = -INFINITY, M = -INFINITY, l = 0.f;
+  for (int p = 0; p < pieces; p++) top = fmaxf(top, row(p).x);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int p = 0; p < pieces; p++) {
+    const float4 e = row(p);
+    M = fmaxf(M, (e.x - base) + e.y);
+    A = fmaxf(A, (e.x - base) + (e.y + e.w));
+  }
+  float x[V];
+#pragma unroll
+  for (int d = 0; d < V; d++) x[d] = 0.f;
+  for (int p = 0; p < pieces; p++) {
+    const float4 e = row(p);
+    const bool none = e.x == -INFINITY;  // zeros, or in a row of NaN a NaN sum: 0 * NaN is wanted
+    const float wo = none ? 0.f : ex2f((e.x - base) + (e.y + e.w) - A);
+    l += times_ex2(e.z, none ? -INFINITY : (e.x - base) + e.y - M);
+#pragma unroll
+    for (int d = 0; d < V; d++) x[d] += place(p)[r * D + (threadIdx.x & 31) * V + d] * wo;
+  }
+  store_row<D, F32>(dst, x, l != 0.f ? exp2f(A - M) / l : 0.f);
+}
+
 template <int D, bool F32, int NT>
 __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAttnArgs a, const Divider by_g, int ctas) {
   constexpr int ROWS = 8 * NT, V = D / 32;
   __shared__ float acc[JOIN_WARPS][D];
-  __shared__ float4 sums[JOIN_WARPS];  // A, M, l
+  __shared__ float4 sums[JOIN_WARPS];  // A, M, l, the signs
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the kernel above has left and is visible
   const int G = a.Hq / a.pool.Hkv;
@@ -734,6 +841,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
     const int r = (int)blockIdx.y + k * JOIN_Y;
     const int pieces = cut.last - first + 1;
     float A = -INFINITY, M = -INFINITY, l = 0.f;
+    uint32_t signs = 0;  // of the pieces' l
     float x[V];
 #pragma unroll
     for (int d = 0; d < V; d++) x[d] = 0.f;
@@ -750,6 +858,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
           if (p < pieces) {  // the first piece is the owner's second place, the others are first places
             const float* src = places + (long long)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * place_floats<D, ROWS>();
             e[i] = *(const float4*)(src + ROWS * D + r * 4);
+            signs |= __float_as_uint(e[i].z);
             if constexpr (D == 128) {
               const float4 v = *(const float4*)(src + r * D + lane * 4);
               y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
@@ -784,12 +893,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
     __syncthreads();  // (the tile before has been read)
 #pragma unroll
     for (int d = 0; d < V; d++) acc[warp][lane * V + d] = x[d];
-    if (lane == 0) sums[warp] = make_float4(A, M, l, 0.f);
+    if (lane == 0) sums[warp] = make_float4(A, M, l, __uint_as_float(signs));
     __syncthreads();
     if (part != 0 || r >= rn) continue;
     for (int i = 1; i < split; i++) {
       A = fmaxf(A, sums[k + i * width].x);
       M = fmaxf(M, sums[k + i * width].y);
+      signs |= __float_as_uint(sums[k + i * width].w);
     }
     l = 0.f;
 #pragma unroll
@@ -801,16 +911,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 3) kv_join_kernel(const KvAtt
 #pragma unroll
       for (int d = 0; d < V; d++) x[d] += acc[k + i * width][lane * V + d] * wo;
     }
-    const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
     const int token = by_g(cut.r0 + r), head = h * G + (cut.r0 + r) - token * G;
-    const long long dst = (cut.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + lane * V;
-#pragma unroll
-    for (int d = 0; d < V; d += 2) {
-      if constexpr (F32)
-        *(float2*)((float*)a.o.p + dst + d) = make_float2(x[d] * inv, x[d + 1] * inv);
-      else
-        *(uint32_t*)((__nv_bfloat16*)a.o.p + dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
-    }
+    const long long at = (cut.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh + lane * V;
+    void* dst = (char*)a.o.p + at * (F32 ? 4 : 2);
+    if (signs >> 31)
+      join_far<D, F32, ROWS>(places, first, pieces, r, dst);
+    else
+      store_row<D, F32>(dst, x, l != 0.f ? exp2f(A - M) / l : 0.f);
   }
 }
 

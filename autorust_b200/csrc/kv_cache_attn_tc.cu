@@ -4,9 +4,10 @@
 //   x = (q . kcode) * c_row * s_k + log2(s_v / v_ref),   P = 2^(x - m + 8),   O = sum P vcode,   l = sum P * v_ref / s_v,   o = v_ref O / l
 //
 // v_ref is the scale of the CTA's first page, held inside [2^-5, 2^20]: scales that an append writes are 2^-60 to 2^121, so that v_ref / s_v
-// and the sums of 2^31 keys stay normal f32 numbers.  Beside a page of huge values P may vanish where the row's sum needs it: a CTA
-// that has a scale above 2^15 v_ref among its pages, which it looks through while the first tiles are on their way, sums
-// 2^((q . kcode) c_row s_k - m + 8), exponentials of their own.  The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
+// and the sums of 2^31 keys stay normal f32 numbers.  Beside a page of huge values P may vanish where the row's sum needs it, and in front of a large
+// logit m's rounding is more than P has room for (the multiply-add takes it off the exact product): a CTA that has a V scale above 2^15 v_ref among its pages, or a K
+// scale that with its rows' largest |q| may make a logit of 2^20, keeps references as pairs (logit, log2 of the V scale), takes them off logit and scale
+// each, and sums 2^((q . kcode) c_row s_k - m + 8), exponentials of their own.  It looks through its pages while the first tiles are on their way.  The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
 // exponential, and the tensor cores see the codes as f16 (exact) and P and q in f16 (q scaled by a power of two per row:
 // exact but for elements 2^-14 below its largest; P rounded to nearest, the row sum keeps the unrounded values).
 //
@@ -51,7 +52,6 @@ constexpr int SOFTMAX_REGS = 144, PRODUCER_REGS = 64, MMA_REGS = 64, LAUNCH_REGS
 static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * MMA_REGS <= LAUNCH_REGS * THREADS, "register pool of the CTA");
 constexpr int BLOCKS = BN / 16;  // column blocks of one page at least
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NEG = -1e30f;            // where a row's maximum starts; a hidden key is -inf
 constexpr float P_SHIFT = 8.0f, LAG = 6.0f;  // P < 2^14: inside f16, and a weight 2^-22 of the largest still a normal number
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;  // 2^-60
 constexpr float V_REF_LEAST = 0.03125f, V_REF_MOST = 1048576.0f;
@@ -112,7 +112,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 }
 
 // SPLIT: the keys are divided over gridDim.z CTAs, which leave partial results for kv_join_rows_kernel: one row of D + 4 values per
-// part, packed row and head -- the accumulated values, then m + log2 v_ref, m, l.
+// part, packed row and head -- the accumulated values, then m, m's part of the scale, l, log2 v_ref.
 template <int D, bool E4M3, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
   using C = Cfg<D>;
@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   uint64_t* pv_done = p_full + 4;      // [tile][buffer], each for one PV: the last of its buffer
   uint32_t* tmem_slot = (uint32_t*)(pv_done + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint32_t* tops = tmem_slot + 2;      // [2]: bits of the rows' largest |q|, of the pages' largest K scale
   const WaitCtx wctx{abort_flag, status, a.batch.sticky, ticket};
 
   asm volatile("griddepcontrol.launch_dependents;");
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     if (lane == 0) {
       lost = launch_lost(status, ticket);
       *abort_flag = lost ? 1u : 0u;
+      tops[0] = tops[1] = 0u;
       for (int i = 0; i < 2; i++) {
         mbar_init(&q_full[i], 4);
         mbar_init(&s_full[2 * i], 1);
@@ -386,14 +388,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
     const uint32_t tS = tmem_addr(tb, lane_base, t * 128), tO = tmem_addr(tb, lane_base, 256 + t * 128);
     const int head = h * G + (in ? row - token * G : 0);
 
-    // a huge V scale somewhere?
+    // a huge V scale somewhere, the largest K scale
     bool far = false;
+    float s_most = 0.f;
+    uint32_t q_top = 0;
     if (nkv_max > 0) {
       const float most = WIDE * v_reference();
 #pragma unroll 4
       for (int blk = (kb >> log2) + tid; blk <= (end - 1) >> log2; blk += 256) {
         const int pg = table[blk];
-        if (pg >= 0 && pg < a.pool.pages) far = far || a.pool.v_scale[(long long)pg * Hkv + h] > most;
+        if (pg >= 0 && pg < a.pool.pages) {
+          far = far || a.pool.v_scale[(long long)pg * Hkv + h] > most;
+          s_most = fmaxf(s_most, a.pool.k_scale[(long long)pg * Hkv + h]);  // (passes over NaN)
+        }
       }
     }
 
@@ -410,6 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
         for (int x = 0; x < 4; x++) top = max(top, max(u[x] << 16 & 0x7fffffffu, u[x] & 0x7fff0000u));
       }
+      if (top < 0x7f800000u) q_top = top;
       const int e = min(max((int)(top >> 23) - 127, -100), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
       c_row = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
@@ -425,10 +433,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       fence_proxy_async_smem();
       warp_arrive(&q_full[t]);
     }
-    float m = NEG, l = 0.f;
+    q_top = __reduce_max_sync(0xffffffffu, q_top);
+    const uint32_t s_top = __reduce_max_sync(0xffffffffu, __float_as_uint(s_most));
+    if (lane == 0) {
+      atomicMax(&tops[0], q_top);
+      atomicMax(&tops[1], s_top);
+    }
+    float m = -INFINITY, l = 0.f, me = 0.f;  // the reference is 2^(m + me), me 0 but in FARS
 
-    // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's; FAR: that, and V scales are far apart.  False:
-    // a wait has run out.
+    // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's; FAR: that, and scales or logits are far
+    // apart.  False: a wait has run out.
     enum Kind { PLAIN, EDGES, FARS };
     auto step = [&](auto kind, int i) {
       constexpr bool EDGE = decltype(kind)::value != PLAIN, FAR = decltype(kind)::value == FARS;
@@ -444,6 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tmem_wait_ld32(sv[0]);
       tmem_wait_ld32(sv[1]);
       float mc = -INFINITY;
+      KvRef far_mc{-INFINITY, 0.f};
 #pragma unroll
       for (int b = 0; b < 4; b++) {
         float top[2] = {-INFINITY, -INFINITY};
@@ -460,14 +475,23 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         }
         // (a block without a page: s_k = 0 and log2 -inf; where all of it is hidden as well, 0 * -inf is NaN, which the
         // maximum passes over)
-        mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c[b], add[b]));
+        if constexpr (FAR) {
+          const float x = fmaxf(top[0], top[1]) * c[b];
+          if (x > -INFINITY && add[b] > -INFINITY) far_mc = kv_larger(KvRef{x, add[b]}, far_mc);
+        } else {
+          mc = fmaxf(mc, fmaf(fmaxf(top[0], top[1]), c[b], add[b]));
+        }
       }
-      const bool need = mc > m + LAG;
+      const bool need = FAR ? far_mc.m != -INFINITY && (m == -INFINITY || kv_over(far_mc, KvRef{m, me}) > LAG) : mc > m + LAG;
       if (__any_sync(0xffffffffu, need)) {
-        const float m_new = need ? mc : m;
-        const float alpha = ex2f(m - m_new);
-        l = FAR ? times_ex2(l, m - m_new) : l * alpha;
-        m = m_new;
+        float by = 0.f;  // log2 of what O and l are multiplied by
+        if (need) by = m == -INFINITY ? -INFINITY : FAR ? kv_over(KvRef{m, me}, far_mc) : m - mc;
+        const float alpha = ex2f(by);
+        l = FAR ? times_ex2(l, by) : l * alpha;
+        if (need) {
+          m = FAR ? far_mc.m : mc;
+          if (FAR) me = far_mc.e;
+        }
         if (i > 0) {  // PV(i - 1) is done when S(i + 1), issued after it, is there; behind the last scores it reports itself
           const bool last = i + 1 == nh[t];
           uint64_t* bar = (last ? pv_done : s_full) + 2 * t + ((i + 1) & 1);
@@ -490,14 +514,18 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           }
         }
       }
-      const float ref = m - P_SHIFT;
-      if constexpr (FAR) {
+      const float ref = m == -INFINITY ? 0.f : FAR ? m : m - P_SHIFT;
+      if constexpr (FAR) {  // the scores become distances from the logit of the reference
 #pragma unroll
         for (int b = 0; b < 4; b++) {
           float sum = 0.f;
 #pragma unroll
-          for (int x = 0; x < 16; x++)
-            if (b * 16 + x < first_out) sum += ex2f(fmaf(__uint_as_float(sv[b >> 1][(b & 1) * 16 + x]), c[b], -ref));
+          for (int x = 0; x < 16; x++) {
+            uint32_t& s = sv[b >> 1][(b & 1) * 16 + x];
+            const float d = __fmul_rn(__uint_as_float(s), c[b]) - ref;
+            s = __float_as_uint(d);
+            if (b * 16 + x < first_out) sum += ex2f(d + (P_SHIFT - me));
+          }
           if (add[b] != -INFINITY) l += sum;
         }
       }
@@ -507,8 +535,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
         for (int b2 = 0; b2 < 2; b2++) {
           const int b = hf * 2 + b2;
-          const float ab = add[b] - ref;
-          const uint64_t c2 = pack_f32x2(c[b], c[b]), add2 = pack_f32x2(ab, ab);
+          const float by = FAR ? 1.0f : c[b], ab = FAR ? add[b] + (P_SHIFT - me) : add[b] - ref;
+          const uint64_t c2 = pack_f32x2(by, by), add2 = pack_f32x2(ab, ab);
           uint64_t sum = pack_f32x2(0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < 8; k++) {
@@ -547,7 +575,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       return in;
     };
     bool ok = true;
-    if (!softmax_any(far)) {
+    far = softmax_any(far);  // (tops are there, too)
+    far = far || __uint_as_float(tops[1]) * __uint_as_float(tops[0] & 0x7f800000u) > KV_LARGE_LOGIT;
+    if (!far) {
       for (int i = 0; i < nh[t] && ok; i++) {
         ok = scores(i);
         if (!ok) break;
@@ -592,7 +622,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           }
         }
       }
-      if (SPLIT && in) *(float4*)(part + D) = make_float4(m + log2f(v_ref), m, l, 0.f);
+      if (SPLIT && in) *(float4*)(part + D) = make_float4(m, me, l, log2f(v_ref));
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -601,8 +631,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   if (warp == W_MMA) tmem_dealloc(tb, 512);
 }
 
-// o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p over the parts of a row, in order; A_p = m_p + log2 v_ref_p.  One warp per
-// packed row and head.
+// o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p over the parts of a row, in order; m_p and A_p = m_p + log2 v_ref_p are held as
+// distances from the largest logit among the references (KvRef).  One warp per packed row and head.
 constexpr int MOST_PARTS = 16;
 template <int D>
 __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, int parts) {
@@ -616,12 +646,18 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
   if (row < p.row0 || row >= p.row0 + p.n) return;  // a row of no sequence
   constexpr int V = D / 32;
   float4 e[MOST_PARTS];
-  float A = NEG, M = NEG;
+  float top = -INFINITY, A = -INFINITY, M = -INFINITY;
 #pragma unroll
   for (int i = 0; i < MOST_PARTS; i++) {
-    e[i] = make_float4(NEG, NEG, 0.f, 0.f);
+    e[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
     if (i < parts) e[i] = *(const float4*)(a.partial + (i * rows + at) * (D + 4) + D);
-    A = fmaxf(A, e[i].x);
+    top = fmaxf(top, e[i].x);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < MOST_PARTS; i++) {
+    e[i].y = (e[i].x - base) + e[i].y;
+    A = fmaxf(A, e[i].y + e[i].w);
     M = fmaxf(M, e[i].y);
   }
   float x[V], l = 0.f;
@@ -631,8 +667,9 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
   for (int i = 0; i < MOST_PARTS; i++) {
     if (i < parts) {
       const float* src = a.partial + (i * rows + at) * (D + 4) + lane * V;
-      const float wo = ex2f(e[i].x - A);
-      l += times_ex2(e[i].z, e[i].y - M);
+      const bool none = e[i].y == -INFINITY;  // (zeros, or in a row of NaN a NaN sum: 0 * NaN is wanted)
+      const float wo = none ? 0.f : ex2f(e[i].y + e[i].w - A);
+      l += times_ex2(e[i].z, none ? -INFINITY : e[i].y - M);
 #pragma unroll
       for (int d = 0; d < V; d += 2) {
         const float2 y = *(const float2*)(src + d);

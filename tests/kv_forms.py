@@ -1,0 +1,79 @@
+"""Calls that take each form of the cache attention, for tests that have to reach all of them, and a bound on the results that looks only at
+what a row sees."""
+from __future__ import annotations
+
+import numpy as np
+
+from autorust_b200 import _abi
+
+# name: lengths, rows of each sequence, kv heads, query heads
+FORMS = {
+    "8 rows whole": ([300, 45], [2, 1], 2, 8),
+    "16 rows whole": ([300, 129], [5, 9], 2, 8),
+    "8 rows cut": ([9000, 200], [2, 1], 1, 4),
+    "16 rows cut": ([9000, 200], [9, 4], 1, 4),
+    "many whole": ([640, 500, 77], [640, 260, 77], 2, 8),
+    "many in parts": ([4000, 700], [300, 133], 1, 4),
+}
+BF16_ONLY = ("many whole", "many in parts")
+
+
+def plan_of(cache, tokens, Hq, sequences, max_length, f32, causal=True):
+    page = cache.k.shape[2]
+    width = -(-max_length // page)
+    batch = _abi.KvBatch(16, 16, 16, width, width, sequences, tokens)  # (placeholders: the sizes decide)
+    return _abi.kv_plan(cache._pool, batch, _abi.DTYPE_F32 if f32 else _abi.DTYPE_BF16, Hq, max_length, causal)
+
+
+def assert_form(name, cache, tokens, Hq, sequences, max_length, f32, causal=True):
+    rows, ctas, parts = plan_of(cache, tokens, Hq, sequences, max_length, f32, causal)
+    want = {"8": 8, "1": 16, "m": 256}[name[0]]
+    assert (rows, ctas > 0, parts > 1) == (want, name.endswith("cut"), name.endswith("parts")), (name, rows, ctas, parts)
+
+
+def attention(q, k, v, positions, causal, page):
+    """One sequence in 64 bits: q [n, Hq, D], k, v [L, Hkv, D].  The result; the weighted average of |v|; the largest sum |q k| / sqrt(D) over the
+    keys a row sees; their number times the largest |v| of the pages they lie on (a later token of the last page may have set its scale).
+    A row that sees no key has zeros everywhere."""
+    n, Hq, D = q.shape
+    L, G = k.shape[0], Hq // k.shape[1]
+    o, size, reach, most = np.zeros((n, Hq, D)), np.zeros((n, Hq, D)), np.zeros((n, Hq, 1)), np.zeros((n, Hq, 1))
+    for i in range(n):
+        last = min(L, positions[i] + 1) if causal else L
+        if last <= 0:
+            continue
+        held = min(L, -(-last // page) * page)
+        for h in range(Hq):
+            kk, vv = k[:last, h // G], v[:last, h // G]
+            s = kk @ q[i, h] / np.sqrt(D)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            o[i, h], size[i, h] = p @ vv, p @ np.abs(vv)
+            reach[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() / np.sqrt(D)
+            most[i, h] = last * np.abs(v[:held, h // G]).max()
+    return o, size, reach, most
+
+
+def expect(s, qf, lengths, starts, causal=True):
+    """The rows of all sequences of a Setup's plain cache."""
+    parts = []
+    for b, length in enumerate(lengths):
+        n = int(starts[b + 1] - starts[b])
+        k, v = (s.plain.tokens(which, s.table[b], int(length)) for which in (0, 1))
+        parts.append(attention(qf[starts[b]:starts[b + 1]].astype(np.float64), k, v, int(length) - n + np.arange(n), causal, s.page))
+    return [np.concatenate(p) for p in zip(*parts)]
+
+
+def assert_close(got, o, size, reach, most, f32, keys, exact_logits=False):
+    """As kv_plain.assert_attention_close derives it, with `most` of what a row sees.  A tensor-core sum of values is cut at 2^-24 of its largest
+    partial sum for each of its products, so that `keys` of them, 16 at a time and in two terms for f32 tensors, add 2^-24 each of the weighted
+    average of |v|.  exact_logits: the call's logits are all the same for a row, or so far apart that only the largest has a weight."""
+    import torch
+    half = torch.finfo(torch.float32 if f32 else torch.bfloat16).eps / 2
+    weight = (2.0 ** -20 if f32 else 2.0 ** -11 + 1.1e-4 + 2.0 ** -20) + keys / 8 * 2.0 ** -24
+    if not exact_logits:
+        weight = weight + 2.0 * 2.0 ** -18 * reach
+    assert np.all(np.isfinite(got))
+    err, tol = np.abs(got - o), half * np.abs(o) + weight * size + 2.0 ** (-36 if f32 else -32) * most
+    worst = np.unravel_index(np.argmax(err - tol), err.shape)
+    assert np.all(err <= tol), (worst, got[worst], o[worst], err[worst], tol[worst])
