@@ -97,6 +97,9 @@ __device__ __forceinline__ KvRef kv_larger(const KvRef& p, const KvRef& q) {
 // Where a logit may reach this (in the log2 domain), it is added to the page's exponent only after the reference has been taken off it:
 // in one f32 number the exponent would be rounded to 2^-5 there.
 constexpr float KV_LARGE_LOGIT = 64.0f;  // as |q| * scale, codes up to 448 and 128 channels: below 2^20
+// The factor of a logit (log2 domain) in front of sum (q / 2^e) code, which is below 2^17: from here on the product may leave f32.  Such a block's
+// logits are NaN, all of them: which ones would be infinite, and of which sign, decides what an infinity is worth.
+constexpr float KV_MOST_FACTOR = 1.298074214633707e33f;  // 2^110
 
 // ---- codes ----
 // The four codes of w -> f32.

@@ -416,6 +416,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       const int e = min(max((int)(top >> 23) - 127, -100), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
       row_c[nt] = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      const bool odd = top >= 0x7f800000u;  // the row is NaN
+      if (odd) row_c[nt] = __uint_as_float(0x7fc00000u);
       if constexpr (E4M3) {
 #pragma unroll
         for (int j = 0; j < D / 16; j++)
@@ -431,8 +433,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
             }
           }
       } else {
-        const bool odd = top >= 0x7f800000u;  // the integer digits cannot carry it
-        row_c[nt] = odd ? __uint_as_float(0x7fc00000u) : row_c[nt] * (1.0f / 2097152.0f);
+        row_c[nt] *= 1.0f / 2097152.0f;
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
           int x0[4], x1[4], x2[4];  // |x0| <= 2^22 and its signed digits: the low bytes of x0, x1 and x2, |x2| <= 64
@@ -545,7 +546,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           KvRef most{-INFINITY, 0.f};
 #pragma unroll
           for (int blk = 0; blk < 2; blk++) {
-            const float k = row_c[nt] * sk[blk];
+            float k = row_c[nt] * sk[blk];
+            if (k > KV_MOST_FACTOR * (E4M3 ? 1.0f : 1.0f / 2097152.0f)) k = __uint_as_float(0x7fc00000u);
             float top = -INFINITY;
 #pragma unroll
             for (int n8 = 2 * blk; n8 < 2 * blk + 2; n8++)

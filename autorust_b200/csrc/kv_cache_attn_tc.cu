@@ -417,13 +417,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
 #pragma unroll
         for (int x = 0; x < 4; x++) top = max(top, max(u[x] << 16 & 0x7fffffffu, u[x] & 0x7fff0000u));
       }
-      if (top < 0x7f800000u) q_top = top;
+      const bool odd = top >= 0x7f800000u;  // such a row is NaN: zeros here, a NaN sum at the end
+      if (!odd) q_top = top;
       const int e = min(max((int)(top >> 23) - 127, -100), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      c_row = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      c_row = odd ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
       uint8_t* dst = sQ + t * C::TILE + r * 128;
 #pragma unroll
       for (int i = 0; i < D / 8; i++) {
+        if (odd) w[i] = make_uint4(0u, 0u, 0u, 0u);
         const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         uint32_t v[4];
 #pragma unroll
@@ -453,7 +455,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tmem_ld32(ts, sv[0]);
       tmem_ld32(ts + 32, sv[1]);
       const float4 sc = *(const float4*)slot, sa = *(const float4*)(slot + BLOCKS), sw = *(const float4*)(slot + 2 * BLOCKS);
-      const float c[4] = {c_row * sc.x, c_row * sc.y, c_row * sc.z, c_row * sc.w}, add[4] = {sa.x, sa.y, sa.z, sa.w};
+      float c[4] = {c_row * sc.x, c_row * sc.y, c_row * sc.z, c_row * sc.w};
+      if constexpr (FAR) {
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+          if (c[b] > KV_MOST_FACTOR) c[b] = __uint_as_float(0x7fc00000u);
+      }
+      const float add[4] = {sa.x, sa.y, sa.z, sa.w};
       const float weight[4] = {sw.x, sw.y, sw.z, sw.w};
       tmem_wait_ld32(sv[0]);
       tmem_wait_ld32(sv[1]);
@@ -597,6 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tc_fence_after();
     }
     if (ok) {
+      if (c_row == 0.f && l > 0.f) l = __uint_as_float(0x7fc00000u);  // a q that is not finite, and a key that it sees
       const float v_ref = nh[t] > 0 ? v_reference() : 1.0f;
       const float inv = SPLIT ? 1.0f : nh[t] > 0 && l != 0.f ? v_ref / l : 0.f;
       __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (p.row0 + (long long)token) * a.o.st + (long long)head * a.o.sh;

@@ -36,7 +36,7 @@ def attention(q, k, v, positions, causal, page):
     keys a row sees; their number times the largest |v| of the pages they lie on (a later token of the last page may have set its scale).
     A row that sees no key has zeros everywhere."""
     n, Hq, D = q.shape
-    L, G = k.shape[0], Hq // k.shape[1]
+    L, G, most_k = k.shape[0], Hq // k.shape[1], np.abs(k).max(initial=0.0)
     o, size, reach, most = np.zeros((n, Hq, D)), np.zeros((n, Hq, D)), np.zeros((n, Hq, 1)), np.zeros((n, Hq, 1))
     for i in range(n):
         last = min(L, positions[i] + 1) if causal else L
@@ -45,7 +45,8 @@ def attention(q, k, v, positions, causal, page):
         held = min(L, -(-last // page) * page)
         for h in range(Hq):
             kk, vv = k[:last, h // G], v[:last, h // G]
-            s = kk @ q[i, h] / np.sqrt(D)
+            # (a matrix product may add equal rows in different orders, which decides between them where logits are huge)
+            s = (kk @ q[i, h] if most_k * np.abs(q[i, h]).max() < 1e9 else (kk * q[i, h]).sum(axis=1)) / np.sqrt(D)
             p = np.exp(s - s.max())
             p /= p.sum()
             o[i, h], size[i, h] = p @ vv, p @ np.abs(vv)

@@ -92,3 +92,58 @@ def test_pages_of_large_keys_among_ordinary_ones(ops, form, f32, fp8):
     q[:, 1::2] *= 1e-4  # (heads of ordinary logits)
     got, qf, starts = call(s, form, q, lengths, new, Hq)
     assert_close(got, *expect(s, qf, lengths, starts), f32, max(lengths))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("form,f32", CASES)
+def test_a_query_that_is_not_finite_makes_its_row_nan(ops, form, f32, bad, fp8):
+    """Whichever channel it stands in, in every form: that row of that head, if it sees a key, and nothing else."""
+    lengths, new, Hkv, Hq = FORMS[form]
+    s = Setup(ops, 6, lengths, Hkv=Hkv, D=128 if fp8 else 64, page=32, fp8=fp8, f32=f32)
+    fill(s, lengths, s.rng.standard_normal((sum(lengths), Hkv, s.D)).astype(np.float32))
+    q = s.rng.standard_normal((sum(new), Hq, s.D)).astype(np.float32)
+    nan = np.zeros((sum(new), Hq), bool)
+    for i, (row, head, channel) in enumerate(zip(range(0, sum(new), max(1, sum(new) // 23)), s.rng.permutation(1000), s.rng.permutation(1000))):
+        q[row, head % Hq, channel % s.D] = bad
+        nan[row, head % Hq] = True
+    got, qf, starts = call(s, form, q, lengths, new, Hq)
+    assert np.array_equal(np.isnan(got).all(axis=2), nan) and np.array_equal(np.isnan(got).any(axis=2), nan)
+    want = expect(s, np.where(np.isfinite(qf), qf, 0), lengths, starts)
+    assert_close(got[~nan], *[w[~nan] for w in want], f32, max(lengths))
+    # every row of a call, in batches of which some rows see nothing: an idle slot, padding, a page that does not exist
+    idle = [0] * len(lengths)
+    got, _, _ = call(s, form, np.full((sum(new), Hq, s.D), bad), lengths, new, Hq)
+    assert np.isnan(got).all()
+    qt = s.torch.full((sum(new), Hq, s.D), bad, device="cuda", dtype=s.torch.float32 if f32 else s.torch.bfloat16)
+    where = (s.ints(idle), s.ints(starts))
+    assert (s.ops.kv_cache_attention(s.cache, qt, s.dtable, *where, max_length=max(lengths)) == 0).all()
+    table = s.dtable.clone()
+    table[0, :] = -1
+    o = s.ops.kv_cache_attention(s.cache, qt, table, s.ints(lengths), s.ints(starts), max_length=max(lengths))
+    assert (o[:new[0]] == 0).all() and s.torch.isnan(o[new[0]:]).all() and s.ops.last_status(None) != 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("form,f32", CASES)
+def test_logits_beyond_f32_make_the_row_nan(ops, form, f32, fp8):
+    """A page of keys of 1e30 in the middle: heads with queries of 1e12 are NaN from there on, in front of it and in the other heads nothing changes."""
+    lengths, new, Hkv, Hq = FORMS[form]
+    s = Setup(ops, 8, lengths, Hkv=Hkv, D=64 if fp8 else 128, page=16, fp8=fp8, f32=f32)
+    k = s.rng.standard_normal((sum(lengths), Hkv, s.D)).astype(np.float32)
+    at = lengths[0] - max(new[0] // 2, 1)  # rows in front of and behind it where there are any
+    k[at // 16 * 16:at // 16 * 16 + 16] = 1e30
+    fill(s, lengths, k)
+    q = s.rng.standard_normal((sum(new), Hq, s.D)).astype(np.float32)
+    q[:, 0] = np.sign(q[:, 0]) * 1e12
+    q[:, 1] = 1e12
+    got, qf, starts = call(s, form, q, lengths, new, Hq)
+    nan = np.zeros((sum(new), Hq), bool)
+    for b, n in enumerate(new):  # (a page's keys share its scale: a row sees it from the page's first token on)
+        huge = np.abs(k[sum(lengths[:b]):sum(lengths[:b + 1])]).max(axis=(1, 2)) > 1e29
+        if huge.any():
+            nan[starts[b]:starts[b + 1], :2] = (lengths[b] - n + np.arange(n) >= np.argmax(huge) // 16 * 16)[:, None]
+    assert nan.any() and np.array_equal(np.isnan(got).all(axis=2), nan) and np.array_equal(np.isnan(got).any(axis=2), nan)
+    with np.errstate(over="ignore"):
+        want = expect(s, qf, lengths, starts)
+    assert_close(got[~nan], *[w[~nan] for w in want], f32, max(lengths))
