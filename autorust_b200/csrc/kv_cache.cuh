@@ -81,6 +81,14 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
+// ---- q ----
+// A row of q is taken times 2^-e, its largest element (`top`: the bits of it) then below 2; a logit's factor is 2^e * scale * constant in this order,
+// so that neither a subnormal q nor one of 2^127 leaves the range on the way.
+__device__ __forceinline__ int kv_binade(uint32_t top) { return min(max((int)(top >> 23) - 127, -126), 127); }
+__device__ __forceinline__ float kv_power(int e) {  // -127 <= e <= 127; 2^-127 is subnormal
+  return __uint_as_float(e == -127 ? 0x00400000u : (uint32_t)(127 + e) << 23);
+}
+
 // ---- references of a softmax ----
 // 2^(m + e): m a logit, e a logarithm of a page's scale.  In one number the scale would be lost beside a logit of 2^24 or more, and keys
 // whose logits are that large and alike would be weighted by their pages' scales.
@@ -97,9 +105,9 @@ __device__ __forceinline__ KvRef kv_larger(const KvRef& p, const KvRef& q) {
 // Where a logit may reach this (in the log2 domain), it is added to the page's exponent only after the reference has been taken off it:
 // in one f32 number the exponent would be rounded to 2^-5 there.
 constexpr float KV_LARGE_LOGIT = 64.0f;  // as |q| * scale, codes up to 448 and 128 channels: below 2^20
-// The factor of a logit (log2 domain) in front of sum (q / 2^e) code, which is below 2^17: from here on the product may leave f32.  Such a block's
+// 2^e * scale: times sum (q / 2^e) code, below 2^17, and log2(e) / sqrt(D), below 2^-2, a logit is below 2^127.  Beyond it a block's
 // logits are NaN, all of them: which ones would be infinite, and of which sign, decides what an infinity is worth.
-constexpr float KV_MOST_FACTOR = 1.298074214633707e33f;  // 2^110
+constexpr float KV_MOST_FACTOR = 5.192296858534828e33f;  // 2^112
 
 // ---- codes ----
 // The four codes of w -> f32.

@@ -398,7 +398,8 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 
     uint32_t q_top = 0;  // of the warp's rows
     uint32_t qa[QOPS][QSTEPS][4] = {};
-    float row_c[NT];  // of row g: logit in the log2 domain = accumulator * row_c * s_k
+    float row_c[NT];  // of row g: logit in the log2 domain = accumulator * (row_c * s_k * unit)
+    const float unit = (1.0f / sqrtf((float)D)) * LOG2E * (E4M3 ? 1.0f : 1.0f / 2097152.0f);
     int lim[NT];      // keys that row g sees
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -412,10 +413,9 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       if (top < 0x7f800000u) q_top = max(q_top, top);
-      // 2^-e brings the largest element below 2; both factors are normal f32 numbers
-      const int e = min(max((int)(top >> 23) - 127, -100), 126);
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      row_c[nt] = __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      const int e = kv_binade(top);
+      const float down = kv_power(-e);
+      row_c[nt] = kv_power(e);
       const bool odd = top >= 0x7f800000u;  // the row is NaN
       if (odd) row_c[nt] = __uint_as_float(0x7fc00000u);
       if constexpr (E4M3) {
@@ -433,7 +433,6 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
             }
           }
       } else {
-        row_c[nt] *= 1.0f / 2097152.0f;
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
           int x0[4], x1[4], x2[4];  // |x0| <= 2^22 and its signed digits: the low bytes of x0, x1 and x2, |x2| <= 64
@@ -464,7 +463,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 
     // From the first V scale above WIDE, or K scale above sk_most, on: scales and logits may be far apart.
     bool far = false;
-    const float sk_most = KV_LARGE_LOGIT * __uint_as_float((uint32_t)(127 - min(max((int)(__reduce_max_sync(0xffffffffu, q_top) >> 23) - 127, -100), 126)) << 23);
+    const float sk_most = KV_LARGE_LOGIT * kv_power(-kv_binade(__reduce_max_sync(0xffffffffu, q_top)));
     if (lane < ROWS) me[lane] = 0.f;
 
     // One group of keys.  EDGE: some row does not see all of them, or there are keys to leave out, or far.
@@ -547,7 +546,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
 #pragma unroll
           for (int blk = 0; blk < 2; blk++) {
             float k = row_c[nt] * sk[blk];
-            if (k > KV_MOST_FACTOR * (E4M3 ? 1.0f : 1.0f / 2097152.0f)) k = __uint_as_float(0x7fc00000u);
+            k = k > KV_MOST_FACTOR ? __uint_as_float(0x7fc00000u) : k * unit;
             float top = -INFINITY;
 #pragma unroll
             for (int n8 = 2 * blk; n8 < 2 * blk + 2; n8++)
@@ -583,7 +582,7 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
           float top = -INFINITY;
 #pragma unroll
           for (int n8 = 0; n8 < 4; n8++) {
-            const float k = row_c[nt] * sk[n8 >> 1];
+            const float k = row_c[nt] * sk[n8 >> 1] * unit;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
               float v = fmaf(s[nt][n8][i], k, ex[n8 >> 1]);

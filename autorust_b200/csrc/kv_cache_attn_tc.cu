@@ -1,13 +1,13 @@
 // Attention of many rows over the 8-bit paged cache (chunks of a prompt, whole prompts): the products on the tcgen05 tensor
 // cores.  The same mathematics as kv_cache_attn.cu, bf16 tensors only:
 //
-//   x = (q . kcode) * c_row * s_k + log2(s_v / v_ref),   P = 2^(x - m + 8),   O = sum P vcode,   l = sum P * v_ref / s_v,   o = v_ref O / l
+//   x = (q . kcode) * (c_row * s_k * log2(e) / sqrt(D)) + log2(s_v / v_ref),   P = 2^(x - m + 8),   O = sum P vcode,   l = sum P * v_ref / s_v,   o = v_ref O / l
 //
 // v_ref is the scale of the CTA's first page, held inside [2^-5, 2^20]: scales that an append writes are 2^-60 to 2^121, so that v_ref / s_v
 // and the sums of 2^31 keys stay normal f32 numbers.  Beside a page of huge values P may vanish where the row's sum needs it, and in front of a large
 // logit m's rounding is more than P has room for (the multiply-add takes it off the exact product): a CTA that has a V scale above 2^15 v_ref among its pages, or a K
 // scale that with its rows' largest |q| may make a logit of 2^20, keeps references as pairs (logit, log2 of the V scale), takes them off logit and scale
-// each, and sums 2^((q . kcode) c_row s_k - m + 8), exponentials of their own.  It looks through its pages while the first tiles are on their way.  The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
+// each, and sums 2^(logit - m + 8), exponentials of their own.  It looks through its pages while the first tiles are on their way.  The scales of a page's keys and values are constants of a column block, so they ride on the multiply-add in front of the
 // exponential, and the tensor cores see the codes as f16 (exact) and P and q in f16 (q scaled by a power of two per row:
 // exact but for elements 2^-14 below its largest; P rounded to nearest, the row sum keeps the unrounded values).
 //
@@ -419,9 +419,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       }
       const bool odd = top >= 0x7f800000u;  // such a row is NaN: zeros here, a NaN sum at the end
       if (!odd) q_top = top;
-      const int e = min(max((int)(top >> 23) - 127, -100), 126);
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      c_row = odd ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23) * ((1.0f / sqrtf((float)D)) * LOG2E);
+      const int e = kv_binade(top);
+      const float down = kv_power(-e);
+      c_row = odd ? 0.f : kv_power(e);
       uint8_t* dst = sQ + t * C::TILE + r * 128;
 #pragma unroll
       for (int i = 0; i < D / 8; i++) {
@@ -455,12 +455,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tmem_ld32(ts, sv[0]);
       tmem_ld32(ts + 32, sv[1]);
       const float4 sc = *(const float4*)slot, sa = *(const float4*)(slot + BLOCKS), sw = *(const float4*)(slot + 2 * BLOCKS);
+      const float unit = (1.0f / sqrtf((float)D)) * LOG2E;
       float c[4] = {c_row * sc.x, c_row * sc.y, c_row * sc.z, c_row * sc.w};
-      if constexpr (FAR) {
 #pragma unroll
-        for (int b = 0; b < 4; b++)
-          if (c[b] > KV_MOST_FACTOR) c[b] = __uint_as_float(0x7fc00000u);
-      }
+      for (int b = 0; b < 4; b++) c[b] = FAR && c[b] > KV_MOST_FACTOR ? __uint_as_float(0x7fc00000u) : c[b] * unit;
       const float add[4] = {sa.x, sa.y, sa.z, sa.w};
       const float weight[4] = {sw.x, sw.y, sw.z, sw.w};
       tmem_wait_ld32(sv[0]);

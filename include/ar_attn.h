@@ -328,7 +328,7 @@ int ar_kv_cache_read(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype
  * sequence's.  A row that sees no key is zero.  Keys on pages that do not exist are left out and reported as above.
  * Logits are f32 numbers of any finite size.  A row is NaN when it sees a key and its q holds an infinity or a NaN, when it sees a page whose
  * scale is NaN, and when it sees a page whose keys may give it a logit beyond the range of f32: when the largest |q| of the row, rounded down
- * to a power of two, times the page's k_scale is above 2^110 sqrt(D) / log2(e).
+ * to a power of two, times the page's k_scale is above 2^112.
  * max_length: a bound on lengths[b] (table_pages * page always is one); it sets how the tokens are divided over the GPU
  * and the workspace, and tokens from max_length on are left out and reported.
  * workspace: ar_kv_cache_attention_workspace_bytes(), 16-byte aligned, may be NULL when that is 0; its contents need not

@@ -147,3 +147,32 @@ def test_logits_beyond_f32_make_the_row_nan(ops, form, f32, fp8):
     with np.errstate(over="ignore"):
         want = expect(s, qf, lengths, starts)
     assert_close(got[~nan], *[w[~nan] for w in want], f32, max(lengths))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("k_exp", [-50, -30])
+@pytest.mark.parametrize("form,f32", CASES)
+def test_queries_at_the_upper_end(ops, form, f32, k_exp, fp8):
+    """|q| of 3e38, beyond 2^127: keys of either sign, of which those with the sign of q share the weight."""
+    lengths, new, Hkv, Hq = FORMS[form]
+    s = Setup(ops, 10, lengths, Hkv=Hkv, D=64 if fp8 else 128, page=32, fp8=fp8, f32=f32)
+    k = np.concatenate([2.0 ** k_exp * (-1.0) ** (np.arange(n) % 3) for n in lengths]).astype(np.float32)
+    fill(s, lengths, np.broadcast_to(k[:, None, None], (sum(lengths), Hkv, s.D)).copy())
+    q = np.full((sum(new), Hq, s.D), 3e38, np.float32)
+    q[:, 1::2] *= -1.0
+    got, qf, starts = call(s, form, q, lengths, new, Hq)
+    assert_close(got, *expect(s, qf, lengths, starts), f32, max(lengths), exact_logits=True)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q_exp", [-125, -118, -104])
+@pytest.mark.parametrize("form,f32", CASES)
+def test_queries_at_the_lower_end(ops, form, f32, q_exp, fp8):
+    """Queries down to the subnormal numbers against keys up to 2^126: ordinary logits."""
+    lengths, new, Hkv, Hq = FORMS[form]
+    s = Setup(ops, 12, lengths, Hkv=Hkv, D=128 if fp8 else 64, page=16, fp8=fp8, f32=f32)
+    k = np.clip(s.rng.standard_normal((sum(lengths), Hkv, s.D)), -3.9, 3.9) * 2.0 ** (-q_exp - 1)
+    fill(s, lengths, k.astype(np.float32))
+    q = s.rng.standard_normal((sum(new), Hq, s.D)) * 2.0 ** q_exp
+    got, qf, starts = call(s, form, q, lengths, new, Hq)
+    assert_close(got, *expect(s, qf, lengths, starts), f32, max(lengths))
