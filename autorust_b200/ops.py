@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -388,13 +389,24 @@ class KvCache:
         _check_dense("v_scale", self.v_scale, k.shape[:2], torch.float32, k.device)
         if self.k_mean is not None:
             _check_dense("k_mean", self.k_mean, (k.shape[1], k.shape[3]), torch.float32, k.device)
-        # what every call passes on; the fields cannot be replaced, so it stays what it is
         pages, Hkv, page, D = k.shape
         pool = _abi.KvPool(k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                            None if self.k_mean is None else self.k_mean.data_ptr(), pages, Hkv, D, page,
                            _abi.KV_E4M3 if self.fp8 else _abi.KV_INT8)
-        object.__setattr__(self, "_pool", pool)
+        object.__setattr__(self, "_description", pool)
+        tensors = (k, self.v, self.k_scale, self.v_scale, k if self.k_mean is None else self.k_mean)
+        object.__setattr__(self, "_places", tuple(t.data_ptr for t in tensors))
+        object.__setattr__(self, "_described", (tuple(t.data_ptr() for t in tensors), k.shape))
         object.__setattr__(self, "_device", k.device)
+
+    @property
+    def _pool(self) -> _abi.KvPool:
+        """What a call passes on.  The fields cannot be replaced, but their memory can (set_, .data, a storage that is freed and grown again): it is
+        described, and checked, anew where it lies elsewhere than it did."""
+        k, v, k_scale, v_scale, k_mean = self._places
+        if ((k(), v(), k_scale(), v_scale(), k_mean()), self.k.shape) != self._described:
+            self.__post_init__()
+        return self._description
 
     def __reduce__(self):  # copies and pickles hold tensors of their own, and so a description of their own
         return KvCache, (self.k, self.v, self.k_scale, self.v_scale, self.k_mean)
@@ -430,7 +442,12 @@ def _kv_batch(cache: KvCache, page_table, lengths, starts, tokens: int) -> _abi.
                         strides[0], width, B, tokens)
 
 
-_Strides2 = ctypes.c_int64 * 2
+@lru_cache(maxsize=256)
+def _strides2(token: int, head: int):
+    """Element strides {token, head} as the C calls read them; they do not write them."""
+    return (ctypes.c_int64 * 2)(token, head)
+
+
 # The handle of torch's current stream on a device, without the Stream object around it (2 us of a call of 15).
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -440,18 +457,17 @@ def _kv_rows(name: str, t: torch.Tensor, shape, dtype, device):
     strides = t.stride()
     if t.shape != shape or t.dtype != dtype or t.device != device or strides[2] != 1:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device} with a contiguous last dimension")
-    return _Strides2(strides[0], strides[1])
+    return _strides2(strides[0], strides[1])
 
 
-def _kv_call(what: str, fn, cache: KvCache, stream, *args) -> None:
+def _kv_call(what: str, fn, pool: _abi.KvPool, dev, stream, *args) -> None:
     """The call on `stream` (None: the current one of the cache's device), with that device current."""
-    dev = cache._device
     handle = stream.cuda_stream if stream is not None else _current_stream(dev.index)
     if torch.cuda.current_device() == dev.index:
-        rc = fn(cache._pool, *args, handle)
+        rc = fn(pool, *args, handle)
     else:
         with torch.cuda.device(dev):
-            rc = fn(cache._pool, *args, handle)
+            rc = fn(pool, *args, handle)
     if rc != _abi.AR_OK:
         _abi.check(rc, what)
 
@@ -469,7 +485,7 @@ def kv_cache_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, page_table
     ks = _kv_rows("k", k, shape, k.dtype, dev)
     vs = _kv_rows("v", v, shape, k.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, T)
-    _kv_call("ar_kv_cache_append", _abi.load().ar_kv_cache_append, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
+    _kv_call("ar_kv_cache_append", _abi.load().ar_kv_cache_append, pool, dev, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
 
 
 def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None, tokens: int,
@@ -481,14 +497,14 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     heads, D = pool.Hkv, pool.D
     if out is None:
         k, v = torch.empty((2, tokens, heads, D), dtype=dtype, device=dev).unbind()
-        code, ks = _dtype_code(k), _Strides2(heads * D, D)
+        code, ks = _dtype_code(k), _strides2(heads * D, D)
         vs = ks
     else:
         k, v = out
         shape, code = (tokens, heads, D), _dtype_code(k)
         ks, vs = _kv_rows("k", k, shape, k.dtype, dev), _kv_rows("v", v, shape, k.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, tokens)
-    _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, cache, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
+    _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, pool, dev, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
     if stream is not None and out is None:
         k.record_stream(stream)  # (of the memory that both lie in)
     return k, v
@@ -513,7 +529,7 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     qs = _kv_rows("q", q, shape, q.dtype, dev)
     fresh = out is None
     if fresh:
-        out, os = q.new_empty(shape), _Strides2(Hq * pool.D, pool.D)
+        out, os = q.new_empty(shape), _strides2(Hq * pool.D, pool.D)
     else:
         os = _kv_rows("out", out, shape, q.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, T)
@@ -527,7 +543,7 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
         have = workspace.numel() * workspace.element_size()
         if workspace.device != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on the cache's device")
-    _kv_call("ar_kv_cache_attention", L.ar_kv_cache_attention, cache, stream, batch, code, q.data_ptr(), qs, out.data_ptr(), os, Hq,
+    _kv_call("ar_kv_cache_attention", L.ar_kv_cache_attention, pool, dev, stream, batch, code, q.data_ptr(), qs, out.data_ptr(), os, Hq,
              bound, causal, workspace.data_ptr() if have else None, have)
     if stream is not None:  # what another stream than the allocating one uses stays until it has done so
         if workspace is not None:
@@ -540,12 +556,13 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
 def kv_cache_attention_workspace(cache: KvCache, tokens: int, Hq: int, sequences: int, max_length: int,
                                  dtype: torch.dtype = torch.bfloat16, causal: bool = True) -> int:
     """Bytes of scratch that kv_cache_attention needs for these sizes, with starts or (one token each) without."""
-    width = max(1, -(-max_length // cache._pool.page))
+    pool = cache._pool
+    width = max(1, -(-max_length // pool.page))
     code = _abi.DTYPE_F32 if dtype == torch.float32 else _abi.DTYPE_BF16
     need = 0
     for starts in ([16, None] if tokens == sequences else [16]):
         batch = _abi.KvBatch(16, 16, starts, width, width, sequences, tokens)  # (placeholders: the sizes decide)
-        need = max(need, _abi.load().ar_kv_cache_attention_workspace_bytes(cache._pool, batch, code, Hq, max_length, int(causal)))
+        need = max(need, _abi.load().ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, max_length, int(causal)))
     return need
 
 
