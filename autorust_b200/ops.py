@@ -460,6 +460,15 @@ def _kv_rows(name: str, t: torch.Tensor, shape, dtype, device):
     return _strides2(strides[0], strides[1])
 
 
+def _empty(shape, dtype, device, stream):
+    """Memory that `stream` writes comes from its own pool (None: the current stream's): a block that was given back on another stream may
+    still be in use by kernels there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _kv_call(what: str, fn, pool: _abi.KvPool, dev, stream, *args) -> None:
     """The call on `stream` (None: the current one of the cache's device), with that device current."""
     handle = stream.cuda_stream if stream is not None else _current_stream(dev.index)
@@ -496,7 +505,7 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     pool, dev, tokens = cache._pool, cache._device, int(tokens)
     heads, D = pool.Hkv, pool.D
     if out is None:
-        k, v = torch.empty((2, tokens, heads, D), dtype=dtype, device=dev).unbind()
+        k, v = _empty((2, tokens, heads, D), dtype, dev, stream).unbind()
         code, ks = _dtype_code(k), _strides2(heads * D, D)
         vs = ks
     else:
@@ -506,7 +515,7 @@ def kv_cache_read(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tenso
     batch = _kv_batch(cache, page_table, lengths, starts, tokens)
     _kv_call("ar_kv_cache_read", _abi.load().ar_kv_cache_read, pool, dev, stream, batch, code, k.data_ptr(), ks, v.data_ptr(), vs)
     if stream is not None and out is None:
-        k.record_stream(stream)  # (of the memory that both lie in)
+        k.record_stream(torch.cuda.current_stream(dev))  # where the caller goes on (of the memory that both lie in)
     return k, v
 
 
@@ -529,7 +538,8 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     qs = _kv_rows("q", q, shape, q.dtype, dev)
     fresh = out is None
     if fresh:
-        out, os = q.new_empty(shape), _strides2(Hq * pool.D, pool.D)
+        out = q.new_empty(shape) if stream is None else _empty(shape, q.dtype, dev, stream)
+        os = _strides2(Hq * pool.D, pool.D)
     else:
         os = _kv_rows("out", out, shape, q.dtype, dev)
     batch = _kv_batch(cache, page_table, lengths, starts, T)
@@ -538,7 +548,7 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
     if workspace is None:
         have = L.ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, bound, causal)
         if have:
-            workspace = torch.empty(have, dtype=torch.uint8, device=dev)
+            workspace = _empty(have, torch.uint8, dev, stream)
     else:
         have = workspace.numel() * workspace.element_size()
         if workspace.device != dev or not workspace.is_contiguous():
@@ -549,7 +559,7 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
         if workspace is not None:
             workspace.record_stream(stream)
         if fresh:
-            out.record_stream(stream)
+            out.record_stream(torch.cuda.current_stream(dev))  # where the caller goes on
     return out
 
 

@@ -44,3 +44,50 @@ def test_a_pool_whose_memory_is_replaced(ops):
     s.check_attention([40, 12], [3, 1], 4)
     torch.cuda.synchronize()
     assert all((x == 77).all() for x in others)
+
+
+def _busy_block(torch, nbytes, ms=40):
+    """A block of the current stream's pool that was given back while a kernel queued there will still write it; where it lies."""
+    x = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda._sleep(int(ms * 1.9e6))
+    x.fill_(0xff)
+    return x.data_ptr()
+
+
+@pytest.mark.parametrize("what", ["attention", "workspace", "read"])
+def test_memory_for_another_stream(ops, what):
+    """A call on a stream that does not wait for the current one gets no memory that kernels of the current one still write."""
+    import torch
+    s = Setup(ops, 15, [9000, 300], Hkv=1, D=128, page=32)
+    s.append([9000, 300], [9000, 300])
+    where = (s.dtable, s.ints([9000, 300]))
+    q = s.rows(2, 4)[0].contiguous()
+    side = torch.cuda.Stream()
+    out = torch.empty_like(q)
+    need = ops._abi.load().ar_kv_cache_attention_workspace_bytes(s.cache._pool, ops._kv_batch(s.cache, *where, None, 2), 1, 4, 9024, 1)
+    assert need > 0
+    starts = s.ints([0, 9000, 9300])
+    nbytes, run = {"attention": (q.numel() * 2, lambda **kw: ops.kv_cache_attention(s.cache, q, *where, workspace=torch.empty_like(ws), **kw)),
+                   "workspace": (need, lambda **kw: ops.kv_cache_attention(s.cache, q, *where, out=out, **kw)),
+                   "read": (2 * 9300 * 128 * 2, lambda **kw: ops.kv_cache_read(s.cache, *where, starts, 9300, **kw)[1])}[what]
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    want = run().clone()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    at = _busy_block(torch, nbytes)
+    got = run(stream=side)
+    assert what == "workspace" or got.data_ptr() != at
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    # and the result stays while the caller's stream reads it
+    if what != "workspace":
+        got = run(stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(int(40 * 1.9e6))
+        copy = got.clone()
+        del got
+        with torch.cuda.stream(side):
+            torch.empty(nbytes, dtype=torch.uint8, device="cuda").fill_(0xff)
+        torch.cuda.synchronize()
+        assert torch.equal(copy, want)
