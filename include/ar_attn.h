@@ -294,8 +294,8 @@ typedef struct ar_kv_pool {
  *   starts     [B + 1] int32, or NULL: rows starts[b] .. starts[b + 1] of the call's packed [T, H, D] tensors belong to
  *              sequence b, in order and not overlapping; NULL: T = B, one row each.
  * Row i of a sequence's n rows stands at position lengths[b] - n + i: the call's rows are the last tokens.  A row whose
- * position is negative is padding (an idle slot of a fixed batch has length 0): it is not written, reads back as zeros and
- * its attention is zero.  Rows in front of starts[0] and from starts[B] on are neither read nor written. */
+ * position is negative is padding (an idle slot of a fixed batch has length 0): it is not written and reads back as zeros, and
+ * its attention is zero where `causal` is set; else it sees what its sequence holds, like every other row.  Rows in front of starts[0] and from starts[B] on are neither read nor written. */
 typedef struct ar_kv_batch {
   const int32_t* page_table;
   const int32_t* lengths;
