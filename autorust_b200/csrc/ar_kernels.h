@@ -74,9 +74,6 @@ bool make_tile_map(CUtensorMap* m, const void* ptr, int cu_dtype, int esize, lon
                    int* token_major_bit);
 bool attn_tc_has(int mode, int D);
 
-// The library's own status block on the current device (api.cu): word 0 is the launch status of calls that bring
-// no workspace, word 1 accumulates every expiry of a bounded wait until the host reads and clears it.
-// False when the address cannot be resolved.
 // 1 when the current device is compute capability 10.x.
 bool device_ok();
 // Lets other translation units of the library feed the launch counters.
@@ -84,6 +81,9 @@ void count_launches(int mode, int kernels);
 // The library's launch word for a launch with bounded waits that brings no workspace, marked with a ticket of its own, or
 // (in a captured call, whose replays would repeat it) cleared on the stream and without one.
 bool launch_ticket(cudaStream_t stream, uint32_t** status, uint32_t* ticket);
+// The library's own status block on the current device (api.cu): word 0 is the launch status of calls that bring
+// no workspace, word 1 accumulates every expiry of a bounded wait, and STATUS_PAGE of the cache calls, until the host reads and
+// clears it.  False when the address cannot be resolved.
 bool library_status_words(uint32_t** launch_word, uint32_t** sticky_word);
 
 // Layout of the Sage workspace (offsets in bytes from its start; every section 256-byte aligned, the first 256 bytes
@@ -152,7 +152,7 @@ TrainTcPlan train_tc_plan(int B, int Hq, int Hkv, int S, int D, int causal);
 // Launches dQ and dK/dV; *launches is incremented by the number of kernels.
 cudaError_t launch_attn_train_backward_tc(const TrainBwdTcArgs& a, cudaStream_t stream, int* launches);
 
-// The 8-bit key/value cache (kv_cache.cu: checks and dispatch; kv_cache_write.cu, kv_cache_attn.cu: kernels).
+// The 8-bit key/value cache (kv_cache.cu: checks and dispatch; kv_cache_write.cu, kv_cache_attn.cu, kv_cache_attn_tc.cu: kernels).
 constexpr uint32_t STATUS_PAGE = 0x40000000u;  // accumulator bit: a page or a length outside the cache
 struct KvPool {
   uint8_t *k, *v;            // codes [pages, Hkv, 1 << page_log2, D]

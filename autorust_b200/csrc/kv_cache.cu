@@ -1,5 +1,5 @@
-// C ABI of the 8-bit key/value cache (include/ar_attn.h): argument checks and dispatch to the kernels in kv_cache_write.cu and
-// kv_cache_attn.cu.  What the page table, the lengths and the starts hold is checked by the kernels: it lies in device memory.
+// C ABI of the 8-bit key/value cache (include/ar_attn.h): argument checks and dispatch to the kernels in kv_cache_write.cu,
+// kv_cache_attn.cu and kv_cache_attn_tc.cu.  What the page table, the lengths and the starts hold is checked by the kernels: it lies in device memory.
 #include "../../include/ar_attn.h"
 #include "ar_kernels.h"
 
