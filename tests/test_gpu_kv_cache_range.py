@@ -176,3 +176,25 @@ def test_queries_at_the_lower_end(ops, form, f32, q_exp, fp8):
     q = s.rng.standard_normal((sum(new), Hq, s.D)) * 2.0 ** q_exp
     got, qf, starts = call(s, form, q, lengths, new, Hq)
     assert_close(got, *expect(s, qf, lengths, starts), f32, max(lengths))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("D,new,Hq", [(128, 4, 12), (128, 1, 12), (64, 4, 12), (64, 1, 4)])
+def test_long_sums_of_f32_tensors_have_no_bias(ops, D, new, Hq, fp8):
+    """Every token of a head has the same positive values, so that they are the result whatever the weights.  Roundings to f32 are as often up as down:
+    each output is off by a few 2^-24 sqrt(additions), the mean of tens of thousands by less than 2^-24; the constant parts -- two products cut at
+    2^-23 of 16 keys' sum, the weights' second term, the division, 2^-23 each -- stay below 2^-21.  (Cut at every one of 400 products the mean would be off
+    by 2^-18.)"""
+    import torch
+    L, B, Hkv = 12219, 74, 4
+    s = Setup(ops, 14, [L], Hkv=Hkv, D=D, page=64, fp8=fp8, f32=True)
+    k = torch.from_numpy(s.rng.standard_normal((L, Hkv, D)).astype(np.float32)).cuda()
+    v = torch.from_numpy(s.rng.uniform(1, 2, (1, Hkv, D)).astype(np.float32)).cuda().expand(L, Hkv, D).contiguous()
+    ops.kv_cache_append(s.cache, k, v, s.dtable, s.ints([L]), s.ints([0, L]))
+    _, held = ops.kv_cache_read(s.cache, s.dtable, s.ints([L]), s.ints([0, 1]), 1, dtype=torch.float32)
+    table = s.dtable.expand(B, -1).contiguous()  # (sequences may share pages that they only read)
+    q = torch.from_numpy(s.rng.standard_normal((B * new, Hq, D)).astype(np.float32)).cuda()
+    o = ops.kv_cache_attention(s.cache, q, table, s.ints([L] * B), s.ints(range(0, B * new + 1, new)), max_length=L)
+    want = held[0].double().repeat_interleave(Hq // Hkv, dim=0)
+    off = o.double() / want - 1
+    assert off.abs().max() < 400 * 2.0 ** -24 and off.mean().abs() < 2.0 ** -21
