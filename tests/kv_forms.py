@@ -31,37 +31,44 @@ def assert_form(name, cache, tokens, Hq, sequences, max_length, f32, causal=True
     assert (rows, ctas > 0, parts > 1) == (want, name.endswith("cut"), name.endswith("parts")), (name, rows, ctas, parts)
 
 
-def attention(q, k, v, positions, causal, page):
+def attention(q, k, v, positions, causal, page, keep=None):
     """One sequence in 64 bits: q [n, Hq, D], k, v [L, Hkv, D].  The result; the weighted average of |v|; the largest sum |q k| / sqrt(D) over the
     keys a row sees; their number times the largest |v| of the pages they lie on (a later token of the last page may have set its scale).
-    A row that sees no key has zeros everywhere."""
+    A row that sees no key has zeros everywhere.  keep [L]: keys that are not left out."""
     n, Hq, D = q.shape
     L, G, most_k = k.shape[0], Hq // k.shape[1], np.abs(k).max(initial=0.0)
     o, size, reach, most = np.zeros((n, Hq, D)), np.zeros((n, Hq, D)), np.zeros((n, Hq, 1)), np.zeros((n, Hq, 1))
-    for i in range(n):
-        last = min(L, positions[i] + 1) if causal else L
-        if last <= 0:
-            continue
-        held = min(L, -(-last // page) * page)
-        for h in range(Hq):
-            kk, vv = k[:last, h // G], v[:last, h // G]
-            # (a matrix product may add equal rows in different orders, which decides between them where logits are huge)
-            s = (kk @ q[i, h] if most_k * np.abs(q[i, h]).max() < 1e9 else (kk * q[i, h]).sum(axis=1)) / np.sqrt(D)
-            p = np.exp(s - s.max())
-            p /= p.sum()
-            o[i, h], size[i, h] = p @ vv, p @ np.abs(vv)
-            reach[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() / np.sqrt(D)
-            most[i, h] = last * np.abs(v[:held, h // G]).max()
+    last = np.clip(np.asarray(positions) + 1 if causal else np.full(n, L), 0, L)
+    seen = np.arange(L)[None, :] < last[:, None]
+    if keep is not None:
+        seen &= keep[None, :]
+    rows = np.flatnonzero(seen.any(axis=1))
+    if len(rows) == 0:
+        return o, size, reach, most
+    seen, held = seen[rows], np.minimum(L, -(-last[rows] // page) * page)
+    for h in range(Hq):
+        kk, vv, qq = k[:, h // G], v[:, h // G], q[rows, h]
+        if most_k * np.abs(qq).max() < 1e9:
+            s = qq @ kk.T
+        else:  # (a matrix product may add equal rows in different orders, which decides between them where logits are huge)
+            s = np.stack([(kk * x).sum(axis=1) for x in qq])
+        s = np.where(seen, s / np.sqrt(D), -np.inf)
+        p = np.exp(s - s.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        vv = np.nan_to_num(vv, nan=0.0)  # (a row that sees one has no result to compare)
+        o[rows, h], size[rows, h] = p @ vv, p @ np.abs(vv)
+        reach[rows, h, 0] = np.where(seen, np.abs(qq) @ np.abs(np.nan_to_num(kk, nan=0.0)).T, 0.0).max(axis=1) / np.sqrt(D)
+        most[rows, h, 0] = seen.sum(axis=1) * np.maximum.accumulate(np.abs(vv).max(axis=1))[held - 1]
     return o, size, reach, most
 
 
-def expect(s, qf, lengths, starts, causal=True):
-    """The rows of all sequences of a Setup's plain cache."""
+def expect(s, qf, lengths, starts, causal=True, keep=None):
+    """The rows of all sequences of a Setup's plain cache; keep: by sequence, the keys that are not left out."""
     parts = []
     for b, length in enumerate(lengths):
         n = int(starts[b + 1] - starts[b])
         k, v = (s.plain.tokens(which, s.table[b], int(length)) for which in (0, 1))
-        parts.append(attention(qf[starts[b]:starts[b + 1]].astype(np.float64), k, v, int(length) - n + np.arange(n), causal, s.page))
+        parts.append(attention(qf[starts[b]:starts[b + 1]].astype(np.float64), k, v, int(length) - n + np.arange(n), causal, s.page, (keep or {}).get(b)))
     return [np.concatenate(p) for p in zip(*parts)]
 
 
