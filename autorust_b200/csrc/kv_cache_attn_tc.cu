@@ -117,12 +117,13 @@ template <int D, bool E4M3, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
   using C = Cfg<D>;
   constexpr int ST = C::STAGES;
+  const float unit = (1.0f / sqrtf((float)D)) * LOG2E;  // of a logit in the log2 domain
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + TILES * C::TILE;
   uint8_t* sV = sK + ST * C::TILE;
-  float* scales = (float*)(smem + C::SCALES);  // [slot][s_k | log2(s_v / v_ref) | v_ref / s_v][block]
+  float* scales = (float*)(smem + C::SCALES);  // [slot][s_k log2(e) / sqrt(D) | log2(s_v / v_ref) | v_ref / s_v][block]
   uint64_t* bars = (uint64_t*)(smem + C::BARS);
   uint64_t* q_full = bars;             // [2]
   uint64_t* k_full = q_full + 2;       // [ST]
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         float* slot = scales + (j % C::SCALE_RING) * 3 * BLOCKS + ptid;
         float sk = 0.f, lv = -INFINITY, wv = 0.f;  // nothing there: every logit -inf, every weight 0
         if (now >= 0) {
-          sk = a.pool.k_scale[(long long)now * Hkv + h];
+          sk = a.pool.k_scale[(long long)now * Hkv + h] * unit;
           const float vs = v_scale_of(now);
           lv = log2f(vs) - log2f(v_ref);
           wv = vs == vs ? v_ref / vs : 1.0f;
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       atomicMax(&tops[1], s_top);
     }
     float m = -INFINITY, l = 0.f, me = 0.f;  // the reference is 2^(m + me), me 0 but in FARS
+    float ref = 0.f;                         // what is taken off a logit: m - P_SHIFT, in FARS m; 0 as long as there is no m
 
     // One step: S of 64 keys -> P.  EDGE: keys from first_out on are not the row's; FAR: that, and scales or logits are far
     // apart.  False: a wait has run out.
@@ -455,10 +457,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
       tmem_ld32(ts, sv[0]);
       tmem_ld32(ts + 32, sv[1]);
       const float4 sc = *(const float4*)slot, sa = *(const float4*)(slot + BLOCKS), sw = *(const float4*)(slot + 2 * BLOCKS);
-      const float unit = (1.0f / sqrtf((float)D)) * LOG2E;
       float c[4] = {c_row * sc.x, c_row * sc.y, c_row * sc.z, c_row * sc.w};
 #pragma unroll
-      for (int b = 0; b < 4; b++) c[b] = FAR && c[b] > KV_MOST_FACTOR ? __uint_as_float(0x7fc00000u) : c[b] * unit;
+      for (int b = 0; b < 4; b++) c[b] = FAR && c[b] > KV_MOST_FACTOR * unit ? __uint_as_float(0x7fc00000u) : c[b];
       const float add[4] = {sa.x, sa.y, sa.z, sa.w};
       const float weight[4] = {sw.x, sw.y, sw.z, sw.w};
       tmem_wait_ld32(sv[0]);
@@ -496,6 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
         l = FAR ? times_ex2(l, by) : l * alpha;
         if (need) {
           m = FAR ? far_mc.m : mc;
+          ref = FAR ? m : m - P_SHIFT;
           if (FAR) me = far_mc.e;
         }
         if (i > 0) {  // PV(i - 1) is done when S(i + 1), issued after it, is there; behind the last scores it reports itself
@@ -520,7 +522,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           }
         }
       }
-      const float ref = m == -INFINITY ? 0.f : FAR ? m : m - P_SHIFT;
       if constexpr (FAR) {  // the scores become distances from the logit of the reference
 #pragma unroll
         for (int b = 0; b < 4; b++) {
