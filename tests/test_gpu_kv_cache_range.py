@@ -198,3 +198,15 @@ def test_long_sums_of_f32_tensors_have_no_bias(ops, D, new, Hq, fp8):
     want = held[0].double().repeat_interleave(Hq // Hkv, dim=0)
     off = o.double() / want - 1
     assert off.abs().max() < 400 * 2.0 ** -24 and off.mean().abs() < 2.0 ** -21
+
+
+def test_late_and_missing_tiles_with_large_logits(attn_lib):
+    """The waits' test (its library, its late and missing tiles) on logits that take the kernels' other loop."""
+    import subprocess
+    import sys
+    from test_gpu_kv_cache_waits import CHILD, ROOT
+    ordinary = "q = rand(m + 49, 2 * heads, D)"
+    assert CHILD.count(ordinary) == 1
+    out = subprocess.run([sys.executable, "-c", CHILD.replace(ordinary, ordinary + " * 3000"), str(ROOT)], capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "done" in out.stdout, out.stdout + out.stderr
