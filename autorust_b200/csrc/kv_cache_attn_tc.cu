@@ -112,7 +112,8 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 }
 
 // SPLIT: the keys are divided over gridDim.z CTAs, which leave partial results for kv_join_rows_kernel: one row of D + 4 values per
-// part, packed row and head -- the accumulated values, then m, m's part of the scale, l, log2 v_ref.
+// part, packed row and head -- the accumulated values, then m + log2 v_ref, m, l, or where the CTA was far, which the sign of l tells,
+// m, m's part of the scale, -l, log2 v_ref.
 template <int D, bool E4M3, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs a, uint32_t* status, uint32_t ticket) {
   using C = Cfg<D>;
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
           }
         }
       }
-      if (SPLIT && in) *(float4*)(part + D) = make_float4(m, me, l, log2f(v_ref));
+      if (SPLIT && in) *(float4*)(part + D) = far ? make_float4(m, me, -l, log2f(v_ref)) : make_float4(m + log2f(v_ref), m, l, 0.f);
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -639,9 +640,46 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attn_tc_kernel(const KvAttnArgs
   if (warp == W_MMA) tmem_dealloc(tb, 512);
 }
 
-// o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p over the parts of a row, in order; m_p and A_p = m_p + log2 v_ref_p are held as
-// distances from the largest logit among the references (KvRef).  One warp per packed row and head.
+// o = 2^(A - M) sum_p 2^(A_p - A) O_p / sum_p 2^(m_p - M) l_p over the parts of a row, in order; A_p = m_p + log2 v_ref_p.  One warp per
+// packed row and head.
 constexpr int MOST_PARTS = 16;
+constexpr float NEG = -1e30f;  // below every m of a part that is not far (2^20), but -inf, which there is none of
+template <int D>
+__device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&x)[D / 32], float inv) {
+#pragma unroll
+  for (int d = 0; d < D / 32; d += 2) *(uint32_t*)(dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+}
+// A row of which some part is far: references as distances from the largest logit among them.  `src`: the lane's values of part 0, `entry`
+// the row's entry in it, `next` from part to part.
+template <int D>
+__device__ __noinline__ void join_far_row(const float* src, const float* entry, long long next, int parts, __nv_bfloat16* dst) {
+  constexpr int V = D / 32;
+  auto row = [&](int p) {  // {m, m's part of the scale, l, log2 v_ref}
+    const float4 e = *(const float4*)(entry + p * next);
+    if (__float_as_uint(e.z) >> 31) return make_float4(e.x, e.y, -e.z, e.w);
+    return make_float4(e.y, 0.f, e.z, e.y == -INFINITY ? 0.f : e.x - e.y);
+  };
+  float top = -INFINITY, A = -INFINITY, M = -INFINITY, l = 0.f;
+  for (int p = 0; p < parts; p++) top = fmaxf(top, row(p).x);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int p = 0; p < parts; p++) {
+    const float4 e = row(p);
+    M = fmaxf(M, (e.x - base) + e.y);
+    A = fmaxf(A, (e.x - base) + (e.y + e.w));
+  }
+  float x[V];
+#pragma unroll
+  for (int d = 0; d < V; d++) x[d] = 0.f;
+  for (int p = 0; p < parts; p++) {
+    const float4 e = row(p);
+    const bool none = e.x == -INFINITY;  // zeros, or in a row of NaN a NaN sum: 0 * NaN is wanted
+    const float wo = none ? 0.f : ex2f((e.x - base) + (e.y + e.w) - A);
+    l += times_ex2(e.z, none ? -INFINITY : (e.x - base) + e.y - M);
+#pragma unroll
+    for (int d = 0; d < V; d++) x[d] = fmaf(src[p * next + d], wo, x[d]);
+  }
+  store_row<D>(dst, x, l != 0.f ? exp2f(A - M) / l : 0.f);
+}
 template <int D>
 __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, int parts) {
   asm volatile("griddepcontrol.launch_dependents;");
@@ -654,19 +692,21 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
   if (row < p.row0 || row >= p.row0 + p.n) return;  // a row of no sequence
   constexpr int V = D / 32;
   float4 e[MOST_PARTS];
-  float top = -INFINITY, A = -INFINITY, M = -INFINITY;
+  float A = NEG, M = NEG;
+  uint32_t signs = 0;
 #pragma unroll
   for (int i = 0; i < MOST_PARTS; i++) {
-    e[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    e[i] = make_float4(NEG, NEG, 0.f, 0.f);
     if (i < parts) e[i] = *(const float4*)(a.partial + (i * rows + at) * (D + 4) + D);
-    top = fmaxf(top, e[i].x);
-  }
-  const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-  for (int i = 0; i < MOST_PARTS; i++) {
-    e[i].y = (e[i].x - base) + e[i].y;
-    A = fmaxf(A, e[i].y + e[i].w);
+    A = fmaxf(A, e[i].x);
     M = fmaxf(M, e[i].y);
+    signs |= __float_as_uint(e[i].z);
+  }
+  __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (long long)row * a.o.st + (long long)head * a.o.sh + lane * V;
+  if (signs >> 31) {
+    const float* entry = a.partial + at * (D + 4) + D;
+    join_far_row<D>(entry - D + lane * V, entry, rows * (D + 4), parts, dst);
+    return;
   }
   float x[V], l = 0.f;
 #pragma unroll
@@ -675,9 +715,8 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
   for (int i = 0; i < MOST_PARTS; i++) {
     if (i < parts) {
       const float* src = a.partial + (i * rows + at) * (D + 4) + lane * V;
-      const bool none = e[i].y == -INFINITY;  // (zeros, or in a row of NaN a NaN sum: 0 * NaN is wanted)
-      const float wo = none ? 0.f : ex2f(e[i].y + e[i].w - A);
-      l += times_ex2(e[i].z, none ? -INFINITY : e[i].y - M);
+      const float wo = ex2f(e[i].x - A);
+      l += times_ex2(e[i].z, e[i].y - M);
 #pragma unroll
       for (int d = 0; d < V; d += 2) {
         const float2 y = *(const float2*)(src + d);
@@ -686,10 +725,7 @@ __global__ void __launch_bounds__(256) kv_join_rows_kernel(const KvAttnArgs a, i
       }
     }
   }
-  const float inv = l != 0.f ? exp2f(A - M) / l : 0.f;
-  __nv_bfloat16* dst = (__nv_bfloat16*)a.o.p + (long long)row * a.o.st + (long long)head * a.o.sh + lane * V;
-#pragma unroll
-  for (int d = 0; d < V; d += 2) *(uint32_t*)(dst + d) = pack_bf16x2(x[d] * inv, x[d + 1] * inv);
+  store_row<D>(dst, x, l != 0.f ? exp2f(A - M) / l : 0.f);
 }
 
 template <int D, bool E4M3>
