@@ -565,13 +565,14 @@ def kv_cache_attention(cache: KvCache, q: torch.Tensor, page_table: torch.Tensor
 
 def kv_cache_attention_workspace(cache: KvCache, tokens: int, Hq: int, sequences: int, max_length: int,
                                  dtype: torch.dtype = torch.bfloat16, causal: bool = True) -> int:
-    """Bytes of scratch that kv_cache_attention needs for these sizes, with starts or (one token each) without."""
+    """Bytes of scratch that kv_cache_attention needs for these sizes, with starts or (one token each) without; sizes that it refuses raise."""
     pool = cache._pool
     width = max(1, -(-max_length // pool.page))
-    code = _abi.DTYPE_F32 if dtype == torch.float32 else _abi.DTYPE_BF16
+    code = _dtype_code(torch.empty(0, dtype=dtype))
     need = 0
     for starts in ([16, None] if tokens == sequences else [16]):
         batch = _abi.KvBatch(16, 16, starts, width, width, sequences, tokens)  # (placeholders: the sizes decide)
+        _abi.kv_plan(pool, batch, code, Hq, max_length, causal)
         need = max(need, _abi.load().ar_kv_cache_attention_workspace_bytes(pool, batch, code, Hq, max_length, int(causal)))
     return need
 

@@ -69,3 +69,15 @@ def test_nothing_is_described_twice():
     c = made()
     assert c._pool is c._pool and c._pool.k_mean == c.k_mean.data_ptr()
     assert made(mean=False)._pool.k_mean is None
+
+
+def test_workspace_of_calls_that_are_refused(attn_lib):
+    """As much as the call would, not the size of another type's call or none at all."""
+    from autorust_b200 import _abi, ops
+    c = made()
+    assert ops.kv_cache_attention_workspace(c, 3, 8, 3, 9008) > 0 == ops.kv_cache_attention_workspace(c, 0, 8, 3, 9008)
+    with pytest.raises(TypeError, match="float16"):
+        ops.kv_cache_attention_workspace(c, 3, 8, 3, 9008, dtype=torch.float16)
+    for sizes in ((3, 7, 3, 9008), (3, 8, 3, 0), (3, 8, 0, 9008), (-1, 8, 3, 9008)):
+        with pytest.raises(_abi.AttnLibraryError, match="shape"):
+            ops.kv_cache_attention_workspace(c, *sizes)
