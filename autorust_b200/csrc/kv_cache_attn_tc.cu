@@ -24,7 +24,7 @@
 // scores.  Step i of tile t: P_t(i) done -> O_t += P_t(i) V(i), then S_t(i + 2) = Q_t K(i + 2) into the same buffer.
 // A row's O may be rescaled only when no PV of its tile is under way: the softmax waits for the last one then, which is rare.
 //
-// Measured, 2 x 1024 rows x 4 heads against 16384 keys, D = 128: 571 us, 933 TFLOP/s.  S in one buffer of 128 keys took 643 us with one
+// Measured, 2 x 1024 rows x 4 heads against 16384 keys, D = 128: 579 us, 920 TFLOP/s (573 before there were references as pairs; 1250 where they are taken).  S in one buffer of 128 keys took 643 us with one
 // issuer and 674 with two.  With the softmax and the producers switched off (a scratch build) the MMAs and their hand-overs
 // alone take 555: a step's 48 MMAs 85 clocks each, against 32 to 64 of arithmetic.  A buffer's round -- PV and QK of both tiles
 // 1400 clocks, the way to the softmax 300, the softmax 1700, the way back 300 -- is what a step waits for; TMEM has room for two

@@ -295,7 +295,8 @@ typedef struct ar_kv_pool {
  *              sequence b, in order and not overlapping; NULL: T = B, one row each.
  * Row i of a sequence's n rows stands at position lengths[b] - n + i: the call's rows are the last tokens.  A row whose
  * position is negative is padding (an idle slot of a fixed batch has length 0): it is not written and reads back as zeros, and
- * its attention is zero where `causal` is set; else it sees what its sequence holds, like every other row.  Rows in front of starts[0] and from starts[B] on are neither read nor written. */
+ * its attention is zero where `causal` is set; else it sees what its sequence holds, like every other row.
+ * Rows in front of starts[0] and from starts[B] on are neither read nor written. */
 typedef struct ar_kv_batch {
   const int32_t* page_table;
   const int32_t* lengths;
@@ -329,7 +330,7 @@ int ar_kv_cache_read(const ar_kv_pool* pool, const ar_kv_batch* batch, int dtype
  * Logits are f32 numbers of any finite size.  A row is NaN when it sees a key and its q holds an infinity or a NaN, when it sees a page whose
  * scale is NaN, and when it sees a page whose keys may give it a logit beyond the range of f32: when the largest |q| of the row, rounded down
  * to a power of two, times the page's k_scale is above 2^112.
- * max_length: a bound on lengths[b] (table_pages * page always is one); it sets how the tokens are divided over the GPU
+ * max_length: a bound on lengths[b], at least 1 (table_pages * page always is one); it sets how the tokens are divided over the GPU
  * and the workspace, and tokens from max_length on are left out and reported.
  * workspace: ar_kv_cache_attention_workspace_bytes(), 16-byte aligned, may be NULL when that is 0; its contents need not
  * survive or be cleared between calls, calls that overlap in time need one each.  One fixed order of summation: a
