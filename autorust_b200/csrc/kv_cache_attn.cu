@@ -679,8 +679,9 @@ __global__ void __launch_bounds__(WARPS * 32, Sh<D, NT>::CTAS_PER_SM) kv_attn_ke
       cp_async_wait<S::STAGES - 1>();
       __syncwarp();
       const float4 sc = *(const float4*)(scales + (it % S::STAGES) * 4);
-      far = far || fmaxf(sc.y, sc.w) > WIDE || fmaxf(sc.x, sc.z) > sk_most;
-      if ((g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || fminf(sc.x, sc.z) < 0.f || far)
+      if (fmaxf(sc.y, sc.w) > WIDE || fmaxf(sc.x, sc.z) > sk_most) far = true;
+      const bool edge = (g_begin + warp + it * WARPS) * GROUP + GROUP > lim_low || fminf(sc.x, sc.z) < 0.f || far;
+      if (__builtin_expect(edge, 0))
         step(std::true_type{}, it);
       else
         step(std::false_type{}, it);
