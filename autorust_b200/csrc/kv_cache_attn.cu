@@ -31,9 +31,9 @@
 // groups of 32 keys, a ring of its own in shared memory filled by cp.async, no barrier in the loop; the CTA's four warps
 // share a piece of one row tile's keys and join at its end.
 //
-// Measured, one token, 32 query and 8 kv heads, D = 128, kernel and join: 8 sequences of 8192 tokens (INT8, 134 MB) 36.3 us, 131072
-// tokens of one (E4M3, 268 MB) 57 us, 4.7 TB/s; from the difference of lengths the loop streams at 6.6 TB/s, and some 15 us of a call are its beginning
-// (start, length, page, first codes) and its end (join of the warps, of the pieces).  64 ragged sequences of up to 4096 tokens 66 us.
+// Measured, one token, 32 query and 8 kv heads, D = 128, kernel and join: 8 sequences of 8192 tokens (INT8, 134 MB) 36.9 us, 131072
+// tokens of one (E4M3, 268 MB) 56 us, 4.8 TB/s; from the difference of lengths the loop streams at 6.6 TB/s, and some 15 us of a call are its beginning
+// (start, length, page, first codes) and its end (join of the warps, of the pieces).  64 ragged sequences of up to 4096 tokens 67 us.
 #include <cuda_bf16.h>
 
 #include "ar_ptx.cuh"
